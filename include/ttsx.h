@@ -521,4 +521,8 @@ int ttsx_debug_fail_next_wait(unsigned kinds);
 #ifdef __cplusplus
 }
 #endif
+
+/* sequence operators: gated linear recurrence, adapters of many voices */
+#include "ttsx_seq.h"
+
 #endif /* TTSX_H */

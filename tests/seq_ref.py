@@ -1,0 +1,71 @@
+"""The sequence operators in float64 on the CPU, written from their formulas (test infrastructure)."""
+import torch
+
+F32 = torch.finfo(torch.float32).eps / 2
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def scan(x, g, h0=None, lengths=None, reverse=False, block=64):
+    """h, h_last, states of the gated recurrence, step by step."""
+    x, g = x.double(), g.double()
+    B, T, D = x.shape
+    f, w = 1 / (1 + torch.exp(-g)), 1 / (1 + torch.exp(g))
+    h = torch.zeros(B, T, D, dtype=torch.float64)
+    last = torch.zeros(B, D, dtype=torch.float64)
+    states = torch.zeros(B, -(-T // block), D, dtype=torch.float64)
+    for b in range(B):
+        n = T if lengths is None else int(lengths[b])
+        s = torch.zeros(D, dtype=torch.float64) if h0 is None else h0[b].double()
+        for p in range(n):
+            if p % block == 0:
+                states[b, p // block] = s
+            t = n - 1 - p if reverse else p
+            s = f[b, t] * s + w[b, t] * x[b, t]
+            h[b, t] = s
+        states[b, -(-n // block):] = s
+        last[b] = s
+    return h, last, states
+
+
+def scan_backward(dh, x, g, h0=None, dh_last=None, lengths=None, reverse=False):
+    """dx, dg, dh0 and, for error bounds, G and the state in front of every step."""
+    dh, x, g = dh.double(), x.double(), g.double()
+    B, T, D = x.shape
+    f, w = 1 / (1 + torch.exp(-g)), 1 / (1 + torch.exp(g))
+    h, _, _ = scan(x, g, h0, lengths, reverse)
+    dx, dg, G_all, before = (torch.zeros(B, T, D, dtype=torch.float64) for _ in range(4))
+    dh0 = torch.zeros(B, D, dtype=torch.float64)
+    for b in range(B):
+        n = T if lengths is None else int(lengths[b])
+        r = torch.zeros(D, dtype=torch.float64) if dh_last is None else dh_last[b].double()
+        for p in range(n - 1, -1, -1):
+            t = n - 1 - p if reverse else p
+            prev = t + 1 if reverse else t - 1
+            if p == 0:
+                hp = torch.zeros(D, dtype=torch.float64) if h0 is None else h0[b].double()
+            else:
+                hp = h[b, prev]
+            G = dh[b, t] + r
+            dx[b, t], dg[b, t] = w[b, t] * G, f[b, t] * w[b, t] * (hp - x[b, t]) * G
+            r = f[b, t] * G
+            G_all[b, t], before[b, t] = G, hp
+        dh0[b] = r
+    return dx, dg, dh0, G_all, before
+
+
+def scan_error(x, g, h0, T, lengths=None):
+    """Bound on the error of a state kept in fp32.  Per step f carries 3 F32 (the sum 1 + e, the reciprocal's 2) and w
+    (|g| + 6) F32 (the exponent's argument, the exponential, the product), the update 2 more; as w |g| <= 0.28 that is
+    below 8 F32 of the largest magnitude m of x and h0, which bounds h too.  Composing pairs instead of steps
+    rounds each factor at most twice: 16.  The errors of n steps add up while the memory 1 / w lasts."""
+    x, g = x.double(), g.double()
+    if lengths is not None:
+        live = torch.arange(x.shape[1])[None, :] < torch.as_tensor(lengths)[:, None]
+        x = torch.where(live[:, :, None], x, 0.0)
+        g = torch.where(live[:, :, None], g, 0.0)
+    m = max(float(x.abs().max()), 0.0 if h0 is None else float(h0.abs().max()))
+    memory = 1.0 + float(torch.exp(g.max()))
+    return 16 * F32 * m * min(T, memory)

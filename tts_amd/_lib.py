@@ -5,7 +5,7 @@ caller gets an exception.
 """
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_long, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int64, c_long, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, os.environ.get("TTSX_LIB", "libttsx.so"))
@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(_HERE, os.environ.get("TTSX_LIB", "libttsx.so"))
 OK, ERR_ARG, ERR_HIP, ERR_STATE = 0, -1, -2, -3
 NORM_SOFTMAX, NORM_SIGMOID = 0, 1
 PAD_CONSTANT, PAD_REFLECT = 0, 1
+F32, BF16, F16 = 0, 1, 2
 
 _fp = c_void_p  # device pointers travel as integers
 
@@ -143,6 +144,15 @@ PROTOTYPES = {
     "ttsx_debug_fail_next_wait": (c_int, [ctypes.c_uint]),
 }
 
+# the same for include/ttsx_seq.h (activations travel as pointer, batch stride, row stride)
+_act = [_fp, c_int64, c_int64]
+SEQ_PROTOTYPES = {
+    "ttsx_gated_scan": (c_int, _act + _act + [_fp, _fp] + [c_int] * 5 + [_fp, _fp, _fp, _fp, c_size_t, c_void_p]),
+    "ttsx_gated_scan_backward": (c_int, _act * 3 + [_fp] * 3 + [c_int] * 5 + [_fp] * 4 + [c_size_t, c_void_p]),
+    "ttsx_gated_scan_workspace": (c_long, [c_int] * 5),
+    "ttsx_gated_step": (c_int, [_fp, c_int64, _fp, c_int64, _fp, c_int, c_int, c_int, _fp, _fp, c_void_p]),
+}
+
 _lib = None
 
 
@@ -165,7 +175,7 @@ def load():
             raise TtsxError("%s not found: build it with `make -C tts_amd/csrc` (or "
                             "`python -c 'import __graft_entry__ as g; g.build()'`)" % LIB_PATH)
         lib = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in PROTOTYPES.items():
+        for name, (res, args) in list(PROTOTYPES.items()) + list(SEQ_PROTOTYPES.items()):
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
         if lib.ttsx_version() != VERSION:

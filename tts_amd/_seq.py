@@ -1,0 +1,73 @@
+"""Argument checks shared by the sequence operators (`recurrence`, `adapters`)."""
+import torch
+
+from . import _lib
+
+DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def are_tensors(what, **tensors):
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            raise ValueError("%s: %s must be a tensor, got %s" % (what, name, type(t).__name__))
+
+
+def on_device(what, **tensors):
+    """All on one GPU (None stands for an argument left out)."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.TtsxError("%s runs on the GPU only: %s is on %s (there is no CPU path)" % (what, name, t.device))
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError("%s: %s is on %s, the others are on %s" % (what, name, t.device, dev))
+
+
+def no_graph(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("%s records no autograd graph: call it under torch.no_grad(); gradients are a call of their "
+                         "own" % what)
+
+
+def rows(t):
+    """t with a contiguous last axis (any other strides stay)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def lengths_on(what, lengths, B, T, device):
+    """Lengths as int32 on the device.  On the device already, they are clamped there by the kernels; on the host they
+    are checked here."""
+    if lengths is None:
+        return None
+    lengths = torch.as_tensor(lengths)
+    if lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64):
+        raise ValueError("%s: lengths must be int32 or int64 [%d], got %s %s"
+                         % (what, B, lengths.dtype, tuple(lengths.shape)))
+    if lengths.is_cuda:
+        if lengths.device != device:
+            raise ValueError("%s: lengths is on %s, the others are on %s" % (what, lengths.device, device))
+    elif B and (int(lengths.min()) < 0 or int(lengths.max()) > T):
+        raise ValueError("%s: lengths must lie in 0..%d" % (what, T))
+    if lengths.dtype == torch.int64:
+        lengths = lengths.clamp(0, T)
+    return lengths.to(device=device, dtype=torch.int32).contiguous()
+
+
+def _span(t):
+    first = t.data_ptr()
+    return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def overlaps(a, b):
+    """Whether the two tensors' memory ranges meet (strided tensors may interleave and still count)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def same_place(a, b):
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
