@@ -65,6 +65,34 @@ long ttsx_gated_scan_workspace(int B, int T, int D, int dtype, int backward);
 int ttsx_gated_step(const void* x, int64_t x_batch_stride, const void* g, int64_t g_batch_stride, const float* h, int B,
                     int D, int dtype, void* y, float* h_out, void* stream);
 
+/* ------------------------------------------------------------------ low-rank adapters of many voices
+ * Beside a shared projection y = x W^T, each request of a batch adds the adapter of its own voice:
+ *   out[b,t,:] = y[b,t,:] + scale[v] (x[b,t,:] down[v]^T) up[v]        v = voices[b]
+ *   y, out   [B,T,N]   out may be y itself (in place), and overlaps no other argument
+ *   x        [B,T,K]
+ *   down     [V,R,K], up [V,R,N], contiguous, of x's type; 1 <= R <= TTSX_ADAPTER_MAX_RANK
+ *   voices   [B] int32; a voice outside 0..V-1 has no adapter
+ *   scale    [V] fp32 or NULL (= 1)
+ * Rows without an adapter (no voice, or at positions >= length) are y's.  x down^T and the sum are fp32; out is
+ * rounded once. */
+#define TTSX_ADAPTER_MAX_RANK 64
+int ttsx_adapter_add(const void* y, int64_t y_batch_stride, int64_t y_row_stride, const void* x, int64_t x_batch_stride,
+                     int64_t x_row_stride, const void* down, const void* up, const int32_t* voices, const float* scale,
+                     const int32_t* lengths, int B, int T, int K, int N, int R, int V, int dtype, void* out,
+                     int64_t out_batch_stride, int64_t out_row_stride, void* stream);
+
+/* Gradients of ttsx_adapter_add from dy [B,T,N], the gradient of out (that of y is dy itself):
+ *   dx       [B,T,K] contiguous; zero in rows without an adapter
+ *   ddown    [V,R,K], dup [V,R,N] contiguous, of x's type: sums over the rows of each voice in the order of the
+ *            batch (two runs agree to the bit); zero for a voice that no request has
+ *   workspace  ttsx_adapter_backward_workspace(B, T, K, N, R, dtype) bytes, aligned to 16 */
+int ttsx_adapter_backward(const void* dy, int64_t dy_batch_stride, int64_t dy_row_stride, const void* x,
+                          int64_t x_batch_stride, int64_t x_row_stride, const void* down, const void* up,
+                          const int32_t* voices, const float* scale, const int32_t* lengths, int B, int T, int K, int N,
+                          int R, int V, int dtype, void* dx, void* ddown, void* dup, void* workspace,
+                          size_t workspace_bytes, void* stream);
+long ttsx_adapter_backward_workspace(int B, int T, int K, int N, int R, int dtype);
+
 #ifdef __cplusplus
 }
 #endif

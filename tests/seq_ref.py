@@ -69,3 +69,64 @@ def scan_error(x, g, h0, T, lengths=None):
     m = max(float(x.abs().max()), 0.0 if h0 is None else float(h0.abs().max()))
     memory = 1.0 + float(torch.exp(g.max()))
     return 16 * F32 * m * min(T, memory)
+
+
+# u handed from one product to the next as two 16-bit numbers: each leaves at most half a step of the type
+SPLIT = {torch.float64: 0.0, torch.float32: 0.0, torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -22}
+
+
+def _live(lengths, b, T):
+    return T if lengths is None else max(0, min(T, int(lengths[b])))
+
+
+def adapter(y, x, down, up, voices, scale=None, lengths=None):
+    """out and a bound on its error before the one rounding to y's type.  Sums of n fp32 products are off by at most
+    n F32 of the sum of their magnitudes; u carries that into the second product, and the split of its type."""
+    dtype, T = y.dtype, y.shape[1]
+    y, x, down, up = (t.double() for t in (y, x, down, up))
+    out, tol = y.clone(), torch.zeros_like(y)
+    K, R = x.shape[2], down.shape[1]
+    for b in range(y.shape[0]):
+        n, v = _live(lengths, b, T), int(voices[b])
+        if not 0 <= v < down.shape[0] or n == 0:
+            continue
+        s = 1.0 if scale is None else float(scale[v])
+        u = x[b, :n] @ down[v].t()
+        size = x[b, :n].abs() @ down[v].abs().t()
+        out[b, :n] += s * (u @ up[v])
+        top = u.abs().amax(1, keepdim=True)
+        eu = (K + 4) * F32 * size + SPLIT[dtype] * top
+        tol[b, :n] = abs(s) * ((eu @ up[v].abs()) + (2 * R + 4) * F32 * ((u.abs() + eu) @ up[v].abs()))
+        tol[b, :n] += 2 * F32 * (y[b, :n].abs() + out[b, :n].abs())
+    return out, tol
+
+
+def adapter_backward(dy, x, down, up, voices, scale=None, lengths=None):
+    """(dx, bound), (ddown, bound), (dup, bound)."""
+    dtype, T = dy.dtype, dy.shape[1]
+    dy, x, down, up = (t.double() for t in (dy, x, down, up))
+    dx, gd, gu = torch.zeros_like(x), torch.zeros_like(down), torch.zeros_like(up)
+    tx, td, tu = torch.zeros_like(x), torch.zeros_like(down), torch.zeros_like(up)
+    K, N, R = x.shape[2], dy.shape[2], down.shape[1]
+    rows = torch.zeros(down.shape[0])
+    for b in range(dy.shape[0]):
+        n, v = _live(lengths, b, T), int(voices[b])
+        if 0 <= v < down.shape[0]:
+            rows[v] += n
+    for b in range(dy.shape[0]):
+        n, v = _live(lengths, b, T), int(voices[b])
+        if not 0 <= v < down.shape[0] or n == 0:
+            continue
+        s = 1.0 if scale is None else float(scale[v])
+        xb, d = x[b, :n], dy[b, :n]
+        u, du = s * xb @ down[v].t(), s * d @ up[v].t()
+        eu = abs(s) * (K + 4) * F32 * (xb.abs() @ down[v].abs().t()) + SPLIT[dtype] * u.abs().amax(1, keepdim=True)
+        edu = abs(s) * (N + 4) * F32 * (d.abs() @ up[v].abs().t()) + SPLIT[dtype] * du.abs().amax(1, keepdim=True)
+        dx[b, :n] = du @ down[v]
+        tx[b, :n] = edu @ down[v].abs() + (2 * R + 4) * F32 * ((du.abs() + edu) @ down[v].abs())
+        gd[v] += du.t() @ xb
+        gu[v] += u.t() @ d
+        many = (2 * float(rows[v]) + 4) * F32
+        td[v] += edu.t() @ xb.abs() + many * ((du.abs() + edu).t() @ xb.abs())
+        tu[v] += eu.t() @ d.abs() + many * ((u.abs() + eu).t() @ d.abs())
+    return (dx, tx), (gd, td), (gu, tu)

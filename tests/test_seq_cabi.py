@@ -110,3 +110,77 @@ def test_lengths_are_checked_on_the_host():
     for bad in ([6, 1], [-1, 1], [1], [0.5, 1.0]):
         with pytest.raises(ValueError):
             lengths_on("f", bad, 2, 5, torch.device("cpu"))
+
+
+def _add(lib, y=ONE, x=ONE, down=ONE, up=ONE, voices=ONE, B=2, T=8, K=16, N=24, R=4, V=3, dtype=0, out=ONE, out_rows=24):
+    return lib.ttsx_adapter_add(y, 192, 24, x, 128, 16, down, up, voices, None, None, B, T, K, N, R, V, dtype, out, 192,
+                                out_rows, None)
+
+
+def _add_backward(lib, dy=ONE, voices=ONE, B=2, T=8, K=16, N=24, R=4, V=3, dtype=0, dx=ONE, dup=ONE, ws=ONE, n=1 << 30):
+    return lib.ttsx_adapter_backward(dy, 192, 24, ONE, 128, 16, ONE, ONE, voices, None, None, B, T, K, N, R, V, dtype, dx,
+                                     ONE, dup, ws, n, None)
+
+
+@pytest.mark.parametrize("call,bad", [
+    (_add, dict(y=None)), (_add, dict(x=None)), (_add, dict(down=None)), (_add, dict(up=None)), (_add, dict(voices=None)),
+    (_add, dict(out=None)), (_add, dict(B=0)), (_add, dict(T=0)), (_add, dict(K=0)), (_add, dict(N=0)), (_add, dict(R=0)),
+    (_add, dict(R=65)), (_add, dict(V=0)), (_add, dict(dtype=3)), (_add, dict(out_rows=25)),
+    (_add_backward, dict(dy=None)), (_add_backward, dict(voices=None)), (_add_backward, dict(dx=None)),
+    (_add_backward, dict(dup=None)), (_add_backward, dict(ws=None)), (_add_backward, dict(n=64)),
+    (_add_backward, dict(ws=ctypes.c_void_p(260))), (_add_backward, dict(B=0)), (_add_backward, dict(R=65)),
+    (_add_backward, dict(dtype=-1)),
+])
+def test_bad_arguments_of_the_adapters(call, bad):
+    from tts_amd import _lib
+    lib = _lib.load()
+    assert call(lib, **bad) == _lib.ERR_ARG
+    assert lib.ttsx_last_error_string().decode().startswith("ttsx_adapter_")
+
+
+def test_workspace_and_rank_limit_of_the_adapters():
+    from tts_amd import _lib, adapters
+    lib = _lib.load()
+    header = open(os.path.join(ROOT, "include", "ttsx_seq.h")).read()
+    assert int(re.search(r"#define TTSX_ADAPTER_MAX_RANK (\d+)", header).group(1)) == adapters.MAX_RANK
+    assert lib.ttsx_adapter_backward_workspace(1, 1, 1, 1, 65, 0) == _lib.ERR_ARG
+    assert lib.ttsx_adapter_backward_workspace(1, 1, 1, 1, 1, 3) == _lib.ERR_ARG
+    small = lib.ttsx_adapter_backward_workspace(1, 1, 1, 1, 1, 0)
+    assert 0 < small < lib.ttsx_adapter_backward_workspace(64, 800, 512, 2048, 32, 1)
+
+
+def test_python_refusals_of_the_adapters():
+    from tts_amd import _lib
+    from tts_amd.adapters import adapter_add, adapter_backward
+    y, x, down, up = torch.zeros(2, 5, 6), torch.zeros(2, 5, 8), torch.zeros(3, 4, 8), torch.zeros(3, 4, 6)
+    v = torch.zeros(2, dtype=torch.int32)
+    for call in (adapter_add, adapter_backward):
+        with pytest.raises(_lib.TtsxError, match="no CPU path"):
+            call(y, x, down, up, v)
+        for args, kw, why in [
+                ((y, x[:, :4], down, up, v), {}, "must agree"), ((y[0, 0], x[0, 0], down, up, v), {}, "must agree"),
+                ((y, x, down[..., :7], up, v), {}, "down and up must be"), ((y, x, down[:2], up, v), {}, "down and up must be"),
+                ((y, x, down[:, :0], up[:, :0], v), {}, "rank must lie"),
+                ((y, x, torch.zeros(3, 65, 8), torch.zeros(3, 65, 6), v), {}, "rank must lie"),
+                ((y.half(), x, down, up, v), {}, "must all be"), ((y, x, down.bfloat16(), up, v), {}, "must all be"),
+                ((y.double(), x.double(), down.double(), up.double(), v), {}, "must all be"),
+                ((y, x, torch.zeros(3, 8, 4).transpose(1, 2), up, v), {}, "must be contiguous"),
+                ((y, x, down, up, v), dict(scale=torch.zeros(2)), "scale must be"),
+                ((y, x, down, up, v), dict(scale=torch.zeros(3).half()), "scale must be"),
+                ((y, x, down, None, v), {}, "must be a tensor"),
+                ((y, x, down, up.clone().requires_grad_(), v), {}, "records no autograd graph")]:
+            with pytest.raises(ValueError, match=why):
+                call(*args, **kw)
+
+
+def test_columns_of_one_buffer():
+    from tts_amd._seq import columns_apart, overlaps, writable_rows
+    buf = torch.zeros(3, 10, 40)
+    assert overlaps(buf[..., :16], buf[..., 16:]) and columns_apart(buf[..., :16], buf[..., 16:])
+    assert columns_apart(buf[..., 30:], buf[..., :30])
+    assert not columns_apart(buf[..., :17], buf[..., 16:])
+    assert not columns_apart(buf[:, :5, :20], buf[:, 5:, :20])          # not the same rows: decided by ranges alone
+    writable_rows("f", "out", buf.transpose(0, 1))
+    for bad in (buf[:1].expand(3, -1, -1), buf.transpose(1, 2), torch.zeros(60).as_strided((2, 3, 8), (24, 4, 1))):
+        with pytest.raises(ValueError):
+            writable_rows("f", "out", bad)

@@ -151,6 +151,9 @@ SEQ_PROTOTYPES = {
     "ttsx_gated_scan_backward": (c_int, _act * 3 + [_fp] * 3 + [c_int] * 5 + [_fp] * 4 + [c_size_t, c_void_p]),
     "ttsx_gated_scan_workspace": (c_long, [c_int] * 5),
     "ttsx_gated_step": (c_int, [_fp, c_int64, _fp, c_int64, _fp, c_int, c_int, c_int, _fp, _fp, c_void_p]),
+    "ttsx_adapter_add": (c_int, _act + _act + [_fp] * 5 + [c_int] * 7 + _act + [c_void_p]),
+    "ttsx_adapter_backward": (c_int, _act + _act + [_fp] * 5 + [c_int] * 7 + [_fp] * 4 + [c_size_t, c_void_p]),
+    "ttsx_adapter_backward_workspace": (c_long, [c_int] * 6),
 }
 
 _lib = None

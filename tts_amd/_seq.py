@@ -71,3 +71,24 @@ def overlaps(a, b):
 
 def same_place(a, b):
     return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
+
+
+def columns_apart(a, b):
+    """Whether two [B,T,n] tensors are different columns of the same rows (slices of one buffer)."""
+    if a.stride()[:2] != b.stride()[:2] or a.shape[:2] != b.shape[:2] or a.element_size() != b.element_size():
+        return False
+    d = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    first, second = (a.shape[2], b.shape[2]) if d >= 0 else (b.shape[2], a.shape[2])
+    pitch = min([s for s, n in zip(a.stride()[:2], a.shape[:2]) if n > 1] or [abs(d) + second])
+    return first <= abs(d) and abs(d) + second <= pitch
+
+
+def writable_rows(what, name, t):
+    """Refuses an output [B,T,n] whose rows are not contiguous or share memory."""
+    if t.stride(2) != 1 and t.shape[2] > 1:
+        raise ValueError("%s: the last axis of %s must be contiguous" % (what, name))
+    need = t.shape[2]
+    for stride, n in sorted((s, n) for s, n in zip(t.stride()[:2], t.shape[:2]) if n > 1):
+        if stride < need:
+            raise ValueError("%s: rows of %s share memory" % (what, name))
+        need = stride * (n - 1) + need

@@ -1,0 +1,162 @@
+"""Low-rank adapters of many voices beside a shared projection, running on libttsx (gfx950).
+
+    out[b,t] = y[b,t] + scale[v] (x[b,t] down[v]^T) up[v],        v = voices[b],   y = x W^T
+
+A voice of the reference is one embedding added to the encoder outputs (Tacotron2/TTS/models.py:838-849).  An adapter
+lets it change a projection too, at R (K + N) numbers per voice, and a batch may hold as many voices as requests: the
+shared product runs once for all of them, `adapter_add` adds each request's own part.
+
+    out             = adapter_add(y, x, down, up, voices)        # whole sequences [B,T,.] or single positions [B,.]
+    dx, ddown, dup  = adapter_backward(dy, x, down, up, voices)  # for fitting the adapters
+
+Activations and adapters are float32, bfloat16 or float16 tensors on the GPU, alike in type; products are summed in
+float32.  As elsewhere in this package there is no CPU path and no autograd graph: gradients are a call of their own, so
+inputs that require them are refused outside `torch.no_grad()`.  Calls work on the current stream of the tensors' device,
+allocate through torch and do not synchronise (`voices` or `lengths` on the host are copied over first, which does), so
+they can be captured into a graph.
+"""
+import functools
+
+import torch
+
+from . import _lib
+from ._seq import (DTYPES, are_tensors, columns_apart, lengths_on, no_graph, on_device, overlaps, rows, same_place,
+                   writable_rows)
+
+MAX_RANK = 64   # TTSX_ADAPTER_MAX_RANK
+
+
+@functools.lru_cache(maxsize=512)
+def _workspace_bytes(B, T, K, N, R, dtype):
+    n = _lib.load().ttsx_adapter_backward_workspace(B, T, K, N, R, dtype)
+    if n < 0:
+        _lib.check(int(n), "ttsx_adapter_backward_workspace")
+    return n
+
+
+def _check(what, name, wide, x, down, up, scale):
+    """Shapes and types: `wide` is y or dy."""
+    are_tensors(what, **{name: wide, "x": x, "down": down, "up": up})
+    if scale is not None:
+        are_tensors(what, scale=scale)
+    if wide.dim() not in (2, 3) or x.shape[:-1] != wide.shape[:-1]:
+        raise ValueError("%s: %s [B,T,N] and x [B,T,K] (or [B,N] and [B,K]) must agree, got %s and %s"
+                         % (what, name, tuple(wide.shape), tuple(x.shape)))
+    K, N = x.shape[-1], wide.shape[-1]
+    if down.dim() != 3 or up.dim() != 3 or down.shape[:2] != up.shape[:2] or down.shape[2] != K or up.shape[2] != N:
+        raise ValueError("%s: down and up must be [V,R,%d] and [V,R,%d], got %s and %s"
+                         % (what, K, N, tuple(down.shape), tuple(up.shape)))
+    V, R = down.shape[:2]
+    if not 1 <= R <= MAX_RANK or V < 1:
+        raise ValueError("%s: the rank must lie in 1..%d, with at least one voice, got down %s"
+                         % (what, MAX_RANK, tuple(down.shape)))
+    if x.dtype not in DTYPES or not x.dtype == wide.dtype == down.dtype == up.dtype:
+        raise ValueError("%s: %s, x, down and up must all be float32, bfloat16 or float16, got %s, %s, %s and %s"
+                         % (what, name, wide.dtype, x.dtype, down.dtype, up.dtype))
+    if not down.is_contiguous() or not up.is_contiguous():
+        raise ValueError("%s: down and up must be contiguous" % what)
+    if scale is not None and (scale.shape != (V,) or scale.dtype != torch.float32):
+        raise ValueError("%s: scale must be float32 [%d], got %s %s" % (what, V, scale.dtype, tuple(scale.shape)))
+    no_graph(what, wide, x, down, up, scale)
+    on_device(what, **{name: wide, "x": x, "down": down, "up": up, "scale": scale})
+
+
+def _voices_on(what, voices, B, V, device):
+    voices = torch.as_tensor(voices)
+    if voices.shape != (B,) or voices.dtype not in (torch.int32, torch.int64):
+        raise ValueError("%s: voices must be int32 or int64 [%d], got %s %s" % (what, B, voices.dtype, tuple(voices.shape)))
+    if voices.is_cuda:
+        if voices.device != device:
+            raise ValueError("%s: voices is on %s, the others are on %s" % (what, voices.device, device))
+    elif B and (int(voices.min()) < -1 or int(voices.max()) >= V):
+        raise IndexError("%s: voices must lie in -1..%d" % (what, V - 1))
+    if voices.dtype == torch.int64:
+        voices = voices.clamp(-1, V)
+    return voices.to(device=device, dtype=torch.int32).contiguous()
+
+
+def adapter_add(y, x, down, up, voices, scale=None, lengths=None, out=None):
+    """y [B,T,N] plus each request's adapter applied to x [B,T,K]; y [B,N] and x [B,K] are one position per request.
+
+    down [V,R,K], up [V,R,N]: the adapters (ranks 1 to 64); voices [B]: which one each request has, -1 for none (on the
+    device any number outside 0..V-1 is none); scale [V] float32: a factor per voice; lengths [B]: rows at positions >=
+    lengths[b] stay y's and x is not read there.  `out` takes the result; out=y works in place and leaves rows without
+    an adapter untouched.  The result has y's type, rounded once."""
+    what = "adapter_add"
+    _check(what, "y", y, x, down, up, scale)
+    if y.dim() == 2:
+        into = None
+        if out is not None:
+            are_tensors(what, out=out)
+            if out.shape != y.shape:
+                raise ValueError("%s: out must be %s %s like y, got %s %s"
+                                 % (what, y.dtype, tuple(y.shape), out.dtype, tuple(out.shape)))
+            into = out.unsqueeze(1)
+        got = adapter_add(y.unsqueeze(1), x.unsqueeze(1), down, up, voices, scale, lengths, into)
+        return out if out is not None else got.squeeze(1)
+    B, T, N = y.shape
+    K, (V, R) = x.shape[2], down.shape[:2]
+    if out is not None:
+        are_tensors(what, out=out)
+        on_device(what, y=y, out=out)
+        no_graph(what, out)
+        if out.shape != y.shape or out.dtype != y.dtype:
+            raise ValueError("%s: out must be %s %s like y, got %s %s"
+                             % (what, y.dtype, tuple(y.shape), out.dtype, tuple(out.shape)))
+        writable_rows(what, "out", out)
+        if overlaps(out, y) and not (same_place(out, y) or columns_apart(out, y)):
+            raise ValueError("%s: out overlaps y" % what)
+        if overlaps(out, x) and not columns_apart(out, x):
+            raise ValueError("%s: out overlaps x" % what)
+        if overlaps(out, down) or overlaps(out, up):
+            raise ValueError("%s: out overlaps an adapter" % what)
+    dev = y.device
+    if out is None:
+        out = torch.empty(B, T, N, dtype=y.dtype, device=dev)
+    if B == 0 or T == 0 or N == 0:
+        return out
+    if K == 0:
+        return out if same_place(out, y) else out.copy_(y)
+    if not same_place(out, y):
+        y = rows(y)
+    x = rows(x)
+    with torch.cuda.device(dev):
+        voices = _voices_on(what, voices, B, V, dev)
+        lengths = lengths_on(what, lengths, B, T, dev)
+        scale = None if scale is None else scale.contiguous()
+        _lib.check(_lib.load().ttsx_adapter_add(
+            y.data_ptr(), y.stride(0), y.stride(1), x.data_ptr(), x.stride(0), x.stride(1), down.data_ptr(), up.data_ptr(),
+            voices.data_ptr(), _lib.ptr(scale), _lib.ptr(lengths), B, T, K, N, R, V, DTYPES[y.dtype], out.data_ptr(),
+            out.stride(0), out.stride(1), _lib.current_stream()), "ttsx_adapter_add")
+    return out
+
+
+def adapter_backward(dy, x, down, up, voices, scale=None, lengths=None):
+    """Gradients of `adapter_add` for x, down and up from dy [B,T,N], the gradient of its result (y's own gradient is dy).
+    Returns dx [B,T,K] (zero in rows without an adapter; not summed over axes that x was broadcast along), ddown
+    [V,R,K] and dup [V,R,N] of their inputs' type: sums over all rows of a voice, kept in float32 and in a fixed order,
+    so that two runs agree to the bit.  `scale` is a constant."""
+    what = "adapter_backward"
+    _check(what, "dy", dy, x, down, up, scale)
+    if dy.dim() == 2:
+        dx, ddown, dup = adapter_backward(dy.unsqueeze(1), x.unsqueeze(1), down, up, voices, scale, lengths)
+        return dx.squeeze(1), ddown, dup
+    B, T, N = dy.shape
+    K, (V, R), dev = x.shape[2], down.shape[:2], dy.device
+    dx = torch.empty(B, T, K, dtype=x.dtype, device=dev)
+    if B == 0 or T == 0 or K == 0 or N == 0:
+        return dx.zero_(), torch.zeros_like(down), torch.zeros_like(up)
+    ddown, dup = torch.empty_like(down), torch.empty_like(up)
+    dtype = DTYPES[x.dtype]
+    need = _workspace_bytes(B, T, K, N, R, dtype)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    dy, x = rows(dy), rows(x)
+    with torch.cuda.device(dev):
+        voices = _voices_on(what, voices, B, V, dev)
+        lengths = lengths_on(what, lengths, B, T, dev)
+        scale = None if scale is None else scale.contiguous()
+        _lib.check(_lib.load().ttsx_adapter_backward(
+            dy.data_ptr(), dy.stride(0), dy.stride(1), x.data_ptr(), x.stride(0), x.stride(1), down.data_ptr(),
+            up.data_ptr(), voices.data_ptr(), _lib.ptr(scale), _lib.ptr(lengths), B, T, K, N, R, V, dtype, dx.data_ptr(),
+            ddown.data_ptr(), dup.data_ptr(), ws.data_ptr(), need, _lib.current_stream()), "ttsx_adapter_backward")
+    return dx, ddown, dup

@@ -1,0 +1,535 @@
+// Low-rank adapters of many voices beside a shared projection (ttsx_adapter_add, ttsx_adapter_backward).
+//
+//   out[b,t,:] = y[b,t,:] + s_v (x[b,t,:] A_v^T) B_v,   v = voices[b],   A_v = down[v] [R,K], B_v = up[v] [R,N]
+//
+//   du = s_v dy B_v^T;  dx = du A_v;  dA_v = sum of du^T x,  dB_v = sum of s_v (x A_v^T)^T dy over the rows of a voice
+//
+// A and B both have their long axis contiguous, so "contract the long axis" and "expand from R" are one kernel each way:
+// dx is the same call as the forward pass with dy in the place of x and the two matrices swapped.
+//
+// One launch does both products of a tile of 32 rows of one request: the four waves share the long axis of the first
+// (each streams x and A from memory straight into matrix operands), the partial sums meet in LDS, and then the waves
+// take blocks of 16 VEC output columns each, read B once per block, and add to y as they write.  u = x A^T never
+// leaves the chip, and y is read and written once: the launch is bound by x, y and out.
+//
+// 16-bit types: the first product is exact up to its fp32 sums.  u is fp32 and is handed to the second product as the
+// sum of two 16-bit numbers (16 or more bits of it), at no cost up to rank 16, where both halves fill one matrix
+// instruction.  fp16 has no range for that, so its rows of u are scaled by a power of two first.
+// Where a column block's lanes read 16 bytes of B from 8 ranks, the 8 x 8 block is transposed in registers; lane
+// l & 15 then owns VEC neighbouring columns, so y and out move 16 bytes per lane.
+#include "../../include/ttsx_seq.h"
+#include "seq_io.h"
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int ROWS = 32;  // rows of a tile: two matrix fragments
+constexpr int WAVES = 4;
+
+struct AddArgs {
+  const void *x, *y, *down, *up;
+  void* out;
+  int64_t x_bs, x_ts, y_bs, y_ts, o_bs, o_ts;
+  const int32_t *voices, *lengths;
+  const float* scale;
+  float* keep;  // [B][RP][keep_pitch]: s u by rank, for the weights' gradients
+  int T, K, N, R, V, tiles, splits, in_place, keep_pitch;
+};
+
+template <class IO>
+__device__ static inline f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (IO::VEC == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+    return c;
+  } else if constexpr (IO::INF2 == IoBf16::INF2) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+}
+
+// 8 x 8 of 16-bit elements: r[i] holds row i, t[j] is column j.
+__device__ static inline void transpose8(const u32x4* r, u32x4* t) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const uint32_t a = r[2 * m][c], b = r[2 * m + 1][c];
+      t[2 * c][m] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+      t[2 * c + 1][m] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    }
+}
+
+// v as the sum of two numbers of the 16-bit type (the second is zero where the first is not finite).
+template <class IO>
+__device__ static inline void two_parts(float v, typename IO::elem& hi, typename IO::elem& lo) {
+  hi = (typename IO::elem)v;
+  const float h = (float)hi;
+  lo = (typename IO::elem)(fabsf(h) < INFINITY ? v - h : 0.0f);
+}
+
+__device__ static inline int voice_of(const int32_t* voices, int b, int V) {
+  const int v = voices[b];
+  return v >= 0 && v < V ? v : -1;
+}
+
+// u of a tile, as the matrix operand of the second product: [ROWS][RP] fp32, or two 16-bit planes and a factor per row.
+template <class IO, int RP>
+struct Hidden {
+  typedef typename IO::elem E;
+  E hi[ROWS][RP + 8], lo[ROWS][RP + 8];
+  float factor[ROWS];
+};
+template <int RP>
+struct Hidden<IoF32, RP> {
+  float u[ROWS][RP + 4];
+};
+
+// ADD: out = y + z, else out = z.  EXPAND: the second product too.
+template <class IO, int RP, bool ADD, bool EXPAND>
+__global__ __launch_bounds__(WAVES * 64) void adapter_kernel(AddArgs a) {
+  constexpr int VEC = IO::VEC, NJ = RP / 16, KSTEP = VEC * 4, CB = 16 * VEC;
+  constexpr bool WIDE = VEC == 4;
+  typedef typename IO::elem E;
+  __shared__ float part[WAVES][ROWS][RP + 1];
+  __shared__ Hidden<IO, RP> hid;
+  const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits % a.tiles, b = blockIdx.x / a.splits / a.tiles;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
+  const int row0 = tile * ROWS, rows = min(ROWS, a.T - row0);
+  const int len = valid_rows(a.lengths, b, a.T), v = voice_of(a.voices, b, a.V);
+  const int live = min(rows, len - row0);  // rows of the tile that count (may be negative)
+  const E* yb = static_cast<const E*>(a.y) + b * a.y_bs + row0 * a.y_ts;
+  E* ob = static_cast<E*>(a.out) + b * a.o_bs + row0 * a.o_ts;
+  const int blocks = ceil_div(a.N, CB);
+
+  if (v < 0 || live <= 0) {
+    if (!EXPAND || (ADD && a.in_place)) return;
+    for (int cb = split * WAVES + wave; cb < blocks; cb += a.splits * WAVES) {
+      const int c = cb * CB + l16 * VEC, n = min(max(a.N - c, 0), VEC);
+      if (n == 0) continue;
+      for (int r = q; r < rows; r += 4)
+        store_some<IO>(ob + r * a.o_ts + c, ADD ? load_some<IO>(yb + r * a.y_ts + c, n) : (u32x4){0, 0, 0, 0}, n);
+    }
+    return;
+  }
+
+  // u = x A^T: lane group q holds VEC consecutive k of a row, the same of x and of A
+  const E* xb = static_cast<const E*>(a.x) + b * a.x_bs + row0 * a.x_ts;
+  const E* A = static_cast<const E*>(a.down) + (int64_t)v * a.R * a.K;
+  f32x4 acc[2][NJ];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[m][j] = (f32x4){0, 0, 0, 0};
+  for (int k0 = wave * KSTEP; k0 < a.K; k0 += WAVES * KSTEP) {
+    const int k = k0 + q * VEC, n = min(max(a.K - k, 0), VEC);
+    u32x4 xr[2], ar[NJ];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int r = 16 * m + l16;
+      xr[m] = r < live && n > 0 ? load_some<IO>(xb + r * a.x_ts + k, n) : (u32x4){0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int r = 16 * j + l16;
+      ar[j] = r < a.R && n > 0 ? load_some<IO>(A + (int64_t)r * a.K + k, n) : (u32x4){0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[m][j] = mma<IO>(xr[m], ar[j], acc[m][j]);
+  }
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[wave][16 * m + 4 * q + i][16 * j + l16] = acc[m][j][i];
+  __syncthreads();
+  {
+    // 8 threads to a row
+    const int r = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (RP / 8);
+    const float s = a.scale ? a.scale[v] : 1.0f;
+    float u[RP / 8], top = 0.0f;
+#pragma unroll
+    for (int c = 0; c < RP / 8; ++c) {
+      u[c] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) u[c] += part[w][r][c0 + c];
+      u[c] *= s;
+      top = fmaxf(top, fabsf(u[c]));
+      if (a.keep && split == 0) a.keep[((int64_t)b * RP + c0 + c) * a.keep_pitch + row0 + r] = u[c];
+    }
+    if constexpr (!EXPAND) {
+      return;
+    } else if constexpr (WIDE) {
+#pragma unroll
+      for (int c = 0; c < RP / 8; ++c) hid.u[r][c0 + c] = u[c];
+    } else {
+      float up = 1.0f;
+      if constexpr (IO::INF2 == IoF16::INF2) {
+        // the row's largest magnitude to [2^13, 2^14): both parts and their products stay inside fp16 and fp32
+        top = fmaxf(top, __shfl_xor(top, 1, 64));
+        top = fmaxf(top, __shfl_xor(top, 2, 64));
+        top = fmaxf(top, __shfl_xor(top, 4, 64));
+        if (top > 1e-30f && top < INFINITY) {
+          int e;
+          frexpf(top, &e);
+          up = ldexpf(1.0f, 14 - e);
+        }
+        if ((threadIdx.x & 7) == 0) hid.factor[r] = 1.0f / up;
+      }
+#pragma unroll
+      for (int c = 0; c < RP / 8; ++c) two_parts<IO>(u[c] * up, hid.hi[r][c0 + c], hid.lo[r][c0 + c]);
+    }
+  }
+  __syncthreads();
+
+  if constexpr (EXPAND) {
+    const E* Bm = static_cast<const E*>(a.up) + (int64_t)v * a.R * a.N;
+    constexpr int KB = WIDE ? 1 : (RP + 31) / 32;  // blocks of 32 ranks
+    for (int cb = split * WAVES + wave; cb < blocks; cb += a.splits * WAVES) {
+      const int c = cb * CB + l16 * VEC, n = min(max(a.N - c, 0), VEC);
+      u32x4 bt[WIDE ? RP / 4 : KB * 8];
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int s = 0; s < RP / 4; ++s) {
+          const int r = q * (RP / 4) + s;
+          bt[s] = r < a.R && n > 0 ? load_some<IO>(Bm + (int64_t)r * a.N + c, n) : (u32x4){0, 0, 0, 0};
+        }
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          u32x4 br[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = RP == 16 ? 8 * (q & 1) + i : kb * 32 + 8 * q + i;
+            br[i] = r < a.R && n > 0 ? load_some<IO>(Bm + (int64_t)r * a.N + c, n) : (u32x4){0, 0, 0, 0};
+          }
+          transpose8(br, bt + 8 * kb);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        if (16 * m >= rows) break;
+        f32x4 z[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) z[j] = (f32x4){0, 0, 0, 0};
+        const int r = 16 * m + l16;
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int s = 0; s < RP / 4; ++s) {
+            const float u = hid.u[r][q * (RP / 4) + s];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              z[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(u, __uint_as_float(bt[s][j]), z[j], 0, 0, 0);
+          }
+        } else if constexpr (RP == 16) {
+          const E* src = q < 2 ? &hid.hi[r][8 * q] : &hid.lo[r][8 * (q - 2)];
+          const u32x4 u = *reinterpret_cast<const u32x4*>(src);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) z[j] = mma<IO>(u, bt[j], z[j]);
+        } else {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            const u32x4 uh = *reinterpret_cast<const u32x4*>(&hid.hi[r][32 * kb + 8 * q]);
+            const u32x4 ul = *reinterpret_cast<const u32x4*>(&hid.lo[r][32 * kb + 8 * q]);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              z[j] = mma<IO>(ul, bt[8 * kb + j], z[j]);
+              z[j] = mma<IO>(uh, bt[8 * kb + j], z[j]);
+            }
+          }
+        }
+        if (n == 0) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 16 * m + 4 * q + i;
+          if (row >= rows || (ADD && a.in_place && row >= live)) continue;
+          float o[VEC];
+          u32x4 yr = (u32x4){0, 0, 0, 0};
+          if constexpr (ADD) yr = load_some<IO>(yb + row * a.y_ts + c, n);
+          if (row < live) {
+            IO::unpack(yr, o);
+            float k = 1.0f;
+            if constexpr (!WIDE && IO::INF2 == IoF16::INF2) k = hid.factor[row];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) o[j] = fmaf(k, z[j][i], o[j]);
+            yr = IO::pack(o);
+          }
+          store_some<IO>(ob + row * a.o_ts + c, yr, n);
+        }
+      }
+    }
+  }
+}
+
+// Weights' gradients, one request (and slice of its rows) at a time: part[b][chunk][rank][column] = sum of u x over
+// the slice's rows, the columns of x (from du) first, those of dy (from u) behind them.  A wave owns 16 VEC columns.
+struct OuterArgs {
+  const void *x, *dy;
+  int64_t x_bs, x_ts, dy_bs, dy_ts;
+  const float *du, *u;  // [B][RP][pitch]
+  const int32_t *voices, *lengths;
+  float* part;
+  int T, K, N, V, chunks, span, pitch, groups;
+};
+
+template <class IO, int RP>
+__global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
+  constexpr int VEC = IO::VEC, NJ = RP / 16, CB = 16 * VEC;
+  constexpr bool SPLIT = IO::INF2 == IoBf16::INF2;  // the others multiply in fp32: fp16 has no range for u
+  typedef typename IO::elem E;
+  const int group = blockIdx.x % a.groups, chunk = blockIdx.x / a.groups % a.chunks, b = blockIdx.x / a.groups / a.chunks;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
+  const int kblocks = ceil_div(a.K, CB), nblocks = ceil_div(a.N, CB);
+  int cb = group * WAVES + wave;
+  if (cb >= kblocks + nblocks) return;
+  const int len = valid_rows(a.lengths, b, a.T);
+  const int first = chunk * a.span, last = min(first + a.span, len);
+  if (voice_of(a.voices, b, a.V) < 0 || first >= last) return;
+  const bool of_x = cb < kblocks;
+  if (!of_x) cb -= kblocks;
+  const int width = of_x ? a.K : a.N;
+  const int c = cb * CB + l16 * VEC, n = min(max(width - c, 0), VEC);
+  const int64_t ts = of_x ? a.x_ts : a.dy_ts;
+  const E* src = (of_x ? static_cast<const E*>(a.x) + b * a.x_bs : static_cast<const E*>(a.dy) + b * a.dy_bs) + c;
+  const float* ub = (of_x ? a.du : a.u) + (int64_t)b * RP * a.pitch;
+  f32x4 acc[NJ][VEC];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[j][i] = (f32x4){0, 0, 0, 0};
+  for (int r0 = first; r0 < last; r0 += 32) {
+    u32x4 xr[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + 8 * q + i;
+      xr[i] = r < last && n > 0 ? load_some<IO>(src + r * ts, n) : (u32x4){0, 0, 0, 0};
+    }
+    u32x4 bt[8];
+    if constexpr (SPLIT) transpose8(xr, bt);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      // rows behind the last one were kept as zeros up to the end of their tile of 32
+      const float4* up = reinterpret_cast<const float4*>(ub + (int64_t)(16 * j + l16) * a.pitch + r0 + 8 * q);
+      const float4 u0 = up[0], u1 = up[1];
+      const float u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+      if constexpr (SPLIT) {
+        float h[8], l[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          E hi, lo;
+          two_parts<IO>(u[i], hi, lo);
+          h[i] = (float)hi, l[i] = (float)lo;
+        }
+        const u32x4 uh = IO::pack(h), ul = IO::pack(l);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          acc[j][i] = mma<IO>(ul, bt[i], acc[j][i]);
+          acc[j][i] = mma<IO>(uh, bt[i], acc[j][i]);
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          float xv[VEC];
+          IO::unpack(xr[s], xv);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(u[s], xv[i], acc[j][i], 0, 0, 0);
+        }
+      }
+    }
+  }
+  const int total = a.K + a.N;
+  float* out = a.part + (int64_t)(b * a.chunks + chunk) * RP * total + (of_x ? 0 : a.K) + c;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float o[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) o[k] = acc[j][k][i];
+      store_f32<VEC>(out + (int64_t)(16 * j + 4 * q + i) * total, n, o);
+    }
+}
+
+// Sum over the requests of a voice, in their order.
+struct GatherArgs {
+  const float* part;
+  const int32_t *voices, *lengths;
+  void *ddown, *dup;
+  int B, T, K, N, R, RP, chunks, span;
+};
+template <class IO>
+__global__ __launch_bounds__(256) void gather_kernel(GatherArgs a) {
+  typedef typename IO::elem E;
+  const int total = a.K + a.N, cols = ceil_div(total, 256);
+  const int col = blockIdx.x % cols * 256 + threadIdx.x, r = blockIdx.x / cols % a.R, v = blockIdx.x / cols / a.R;
+  if (col >= total) return;
+  float s = 0.0f;
+  for (int b = 0; b < a.B; ++b) {
+    if (a.voices[b] != v) continue;
+    const int used = ceil_div(valid_rows(a.lengths, b, a.T), a.span);
+    const float* p = a.part + ((int64_t)b * a.chunks * a.RP + r) * total + col;
+    for (int k = 0; k < used; ++k) s += p[(int64_t)k * a.RP * total];
+  }
+  if (col < a.K)
+    static_cast<E*>(a.ddown)[((int64_t)v * a.R + r) * a.K + col] = (E)s;
+  else
+    static_cast<E*>(a.dup)[((int64_t)v * a.R + r) * a.N + col - a.K] = (E)s;
+}
+
+int padded_rank(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : 64; }
+
+// Workgroups share the columns of a tile of rows where the tiles alone do not fill 256 CUs twice (each then repeats the
+// first product).
+int column_splits(int64_t tiles, int N, int vec) {
+  const int most = ceil_div(ceil_div(N, 16 * vec), WAVES);
+  const int64_t want = tiles >= 512 ? 1 : (512 + tiles - 1) / tiles;
+  return (int)(want < most ? want : most);
+}
+
+template <class IO, int RP, bool ADD, bool EXPAND>
+int launch_tile(AddArgs a, int B, hipStream_t s) {
+  a.tiles = ceil_div(a.T, ROWS);
+  const int64_t tiles = (int64_t)B * a.tiles;
+  a.splits = EXPAND ? column_splits(tiles, a.N, IO::VEC) : 1;
+  TTSX_ARG(tiles * a.splits <= 0x7fffffff, "ttsx_adapter: too many rows");
+  adapter_kernel<IO, RP, ADD, EXPAND><<<(unsigned)(tiles * a.splits), WAVES * 64, 0, s>>>(a);
+  TTSX_LAUNCH_CHECK();
+  return TTSX_OK;
+}
+
+template <class IO>
+int run_add(const AddArgs& a, int B, hipStream_t s) {
+  switch (padded_rank(a.R)) {
+    case 16: return launch_tile<IO, 16, true, true>(a, B, s);
+    case 32: return launch_tile<IO, 32, true, true>(a, B, s);
+    default: return launch_tile<IO, 64, true, true>(a, B, s);
+  }
+}
+
+struct BackPlan {
+  int RP, pitch, chunks, span;
+  size_t hidden, part;  // floats
+};
+// Slices of a request's rows: enough waves (one per 16 VEC columns and slice) to fill the chip, 64 rows at least.
+BackPlan back_plan(int B, int T, int K, int N, int R, int vec) {
+  BackPlan p;
+  p.RP = padded_rank(R);
+  p.pitch = round_up(T, ROWS);
+  const int64_t waves = (int64_t)B * (ceil_div(K, 16 * vec) + ceil_div(N, 16 * vec));
+  const int want = waves >= 2048 ? 1 : (int)((2048 + waves - 1) / waves), most = ceil_div(T, 64);
+  p.span = round_up(ceil_div(T, want < most ? want : most), ROWS);
+  p.chunks = ceil_div(T, p.span);
+  p.hidden = (size_t)B * p.RP * p.pitch;
+  p.part = (size_t)B * p.chunks * p.RP * ((size_t)K + N);
+  return p;
+}
+
+template <class IO, int RP>
+int run_backward(const AddArgs& dx, const BackPlan& p, int B, float* ws, void* ddown, void* dup, hipStream_t s) {
+  float *du = ws, *u = du + p.hidden, *part = u + p.hidden;
+  // dx = (s dy B^T) A, keeping s dy B^T
+  AddArgs a = dx;
+  a.keep = du, a.keep_pitch = p.pitch;
+  int rc = launch_tile<IO, RP, false, true>(a, B, s);
+  if (rc != TTSX_OK) return rc;
+  // s x A^T
+  AddArgs c = dx;
+  c.x = dx.y, c.x_bs = dx.y_bs, c.x_ts = dx.y_ts, c.K = dx.N, c.N = dx.K;
+  c.down = dx.up, c.up = nullptr, c.out = nullptr;
+  c.keep = u, c.keep_pitch = p.pitch;
+  rc = launch_tile<IO, RP, false, false>(c, B, s);
+  if (rc != TTSX_OK) return rc;
+  OuterArgs o{};
+  o.x = dx.y, o.x_bs = dx.y_bs, o.x_ts = dx.y_ts;
+  o.dy = dx.x, o.dy_bs = dx.x_bs, o.dy_ts = dx.x_ts;
+  o.du = du, o.u = u, o.voices = dx.voices, o.lengths = dx.lengths, o.part = part;
+  o.T = dx.T, o.K = dx.N, o.N = dx.K, o.V = dx.V, o.chunks = p.chunks, o.span = p.span, o.pitch = p.pitch;
+  o.groups = ceil_div(ceil_div(o.K, 16 * IO::VEC) + ceil_div(o.N, 16 * IO::VEC), WAVES);
+  const int64_t grid = (int64_t)B * p.chunks * o.groups;
+  TTSX_ARG(grid <= 0x7fffffff, "ttsx_adapter_backward: too many rows");
+  outer_kernel<IO, RP><<<(unsigned)grid, WAVES * 64, 0, s>>>(o);
+  TTSX_LAUNCH_CHECK();
+  GatherArgs g{};
+  g.part = part, g.voices = dx.voices, g.lengths = dx.lengths, g.ddown = ddown, g.dup = dup;
+  g.B = B, g.T = dx.T, g.K = o.K, g.N = o.N, g.R = dx.R, g.RP = RP, g.chunks = p.chunks, g.span = p.span;
+  const int64_t outs = (int64_t)dx.V * dx.R * ceil_div(o.K + o.N, 256);
+  TTSX_ARG(outs <= 0x7fffffff, "ttsx_adapter_backward: too many voices");
+  gather_kernel<IO><<<(unsigned)outs, 256, 0, s>>>(g);
+  TTSX_LAUNCH_CHECK();
+  return TTSX_OK;
+}
+
+template <class IO>
+int run_backward_any(const AddArgs& a, const BackPlan& p, int B, float* ws, void* ddown, void* dup, hipStream_t s) {
+  switch (p.RP) {
+    case 16: return run_backward<IO, 16>(a, p, B, ws, ddown, dup, s);
+    case 32: return run_backward<IO, 32>(a, p, B, ws, ddown, dup, s);
+    default: return run_backward<IO, 64>(a, p, B, ws, ddown, dup, s);
+  }
+}
+
+bool shape_ok(int B, int T, int K, int N, int R, int V) {
+  return B >= 1 && T >= 1 && K >= 1 && N >= 1 && R >= 1 && R <= TTSX_ADAPTER_MAX_RANK && V >= 1 && T <= (1 << 30) &&
+         K <= (1 << 24) && N <= (1 << 24) && V <= (1 << 24);
+}
+bool dtype_ok(int d) { return d == TTSX_F32 || d == TTSX_BF16 || d == TTSX_F16; }
+
+}  // namespace
+
+extern "C" int ttsx_adapter_add(const void* y, int64_t y_batch_stride, int64_t y_row_stride, const void* x,
+                                int64_t x_batch_stride, int64_t x_row_stride, const void* down, const void* up,
+                                const int32_t* voices, const float* scale, const int32_t* lengths, int B, int T, int K,
+                                int N, int R, int V, int dtype, void* out, int64_t out_batch_stride,
+                                int64_t out_row_stride, void* stream) {
+  TTSX_ARG(y && x && down && up && voices && out, "ttsx_adapter_add: null argument");
+  TTSX_ARG(shape_ok(B, T, K, N, R, V), "ttsx_adapter_add: bad shape B=%d T=%d K=%d N=%d R=%d V=%d (1 <= R <= %d)", B, T,
+           K, N, R, V, TTSX_ADAPTER_MAX_RANK);
+  TTSX_ARG(dtype_ok(dtype), "ttsx_adapter_add: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
+  TTSX_ARG(out != y || (out_batch_stride == y_batch_stride && out_row_stride == y_row_stride),
+           "ttsx_adapter_add: out is y with other strides");
+  AddArgs a{};
+  a.x = x, a.x_bs = x_batch_stride, a.x_ts = x_row_stride, a.y = y, a.y_bs = y_batch_stride, a.y_ts = y_row_stride;
+  a.out = out, a.o_bs = out_batch_stride, a.o_ts = out_row_stride, a.down = down, a.up = up;
+  a.voices = voices, a.scale = scale, a.lengths = lengths, a.T = T, a.K = K, a.N = N, a.R = R, a.V = V;
+  a.in_place = out == y;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  return dtype == TTSX_F32 ? run_add<IoF32>(a, B, s) : dtype == TTSX_BF16 ? run_add<IoBf16>(a, B, s) : run_add<IoF16>(a, B, s);
+}
+
+extern "C" long ttsx_adapter_backward_workspace(int B, int T, int K, int N, int R, int dtype) {
+  TTSX_ARG(shape_ok(B, T, K, N, R, 1) && dtype_ok(dtype), "ttsx_adapter_backward_workspace: bad shape or type");
+  const BackPlan p = back_plan(B, T, K, N, R, dtype == TTSX_F32 ? 4 : 8);
+  return (long)(sizeof(float) * (2 * p.hidden + p.part));
+}
+
+extern "C" int ttsx_adapter_backward(const void* dy, int64_t dy_batch_stride, int64_t dy_row_stride, const void* x,
+                                     int64_t x_batch_stride, int64_t x_row_stride, const void* down, const void* up,
+                                     const int32_t* voices, const float* scale, const int32_t* lengths, int B, int T,
+                                     int K, int N, int R, int V, int dtype, void* dx, void* ddown, void* dup,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  TTSX_ARG(dy && x && down && up && voices && dx && ddown && dup && workspace, "ttsx_adapter_backward: null argument");
+  TTSX_ARG(shape_ok(B, T, K, N, R, V), "ttsx_adapter_backward: bad shape B=%d T=%d K=%d N=%d R=%d V=%d (1 <= R <= %d)",
+           B, T, K, N, R, V, TTSX_ADAPTER_MAX_RANK);
+  TTSX_ARG(dtype_ok(dtype), "ttsx_adapter_backward: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
+  const BackPlan p = back_plan(B, T, K, N, R, dtype == TTSX_F32 ? 4 : 8);
+  TTSX_ARG(workspace_bytes >= sizeof(float) * (2 * p.hidden + p.part) && (uintptr_t)workspace % 16 == 0,
+           "ttsx_adapter_backward: workspace too small or not aligned to 16 bytes");
+  // the forward kernel with dy for x and the matrices swapped; its y is the x of this call
+  AddArgs a{};
+  a.x = dy, a.x_bs = dy_batch_stride, a.x_ts = dy_row_stride, a.y = x, a.y_bs = x_batch_stride, a.y_ts = x_row_stride;
+  a.out = dx, a.o_bs = (int64_t)T * K, a.o_ts = K, a.down = up, a.up = down;
+  a.voices = voices, a.scale = scale, a.lengths = lengths, a.T = T, a.K = N, a.N = K, a.R = R, a.V = V;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  float* ws = static_cast<float*>(workspace);
+  return dtype == TTSX_F32    ? run_backward_any<IoF32>(a, p, B, ws, ddown, dup, s)
+         : dtype == TTSX_BF16 ? run_backward_any<IoBf16>(a, p, B, ws, ddown, dup, s)
+                              : run_backward_any<IoF16>(a, p, B, ws, ddown, dup, s);
+}
