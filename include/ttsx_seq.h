@@ -34,7 +34,7 @@ extern "C" {
 /* ------------------------------------------------------------------ gated linear recurrence
  *   f_t = sigmoid(g_t)      h_t = f_t h_{t-1} + (1 - f_t) x_t
  * per channel, over the rows 0 .. length-1 of each request, or from row length-1 down to 0 where `reverse` is set.
- *   x, g     [B,T,D]  values and gate logits (may be two slices of one projection)
+ *   x, g     [B,T,D]  values and gate logits (may be two slices of one projection); D and the row strides up to 2^20
  *   h0       [B,D] fp32 state in front of the first step, or NULL (= 0)
  *   h        [B,T,D] contiguous, of x's type; rows at positions >= length are zero
  *   h_last   [B,D] fp32 state behind the last step (h0 for an empty request)

@@ -6,16 +6,42 @@ from . import _lib
 DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
-def are_tensors(what, **tensors):
-    for name, t in tensors.items():
+# What torch.cuda.current_stream() and torch.cuda.device() wrap: a call of the smallest size is bound by the host.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_functions = {}
+
+
+def call(name, device, *args):
+    """The entry point `name` with `args` and the current stream of `device`, run on that device."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_lib.load(), name)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc != _lib.OK:
+        _lib.check(rc, name)
+
+
+def are_tensors(what, *named):
+    for name, t in named:
         if not isinstance(t, torch.Tensor):
             raise ValueError("%s: %s must be a tensor, got %s" % (what, name, type(t).__name__))
 
 
-def on_device(what, **tensors):
-    """All on one GPU (None stands for an argument left out)."""
+def on_device(what, *named):
+    """All on one GPU, none part of an autograd graph (None stands for an argument left out)."""
+    if torch.is_grad_enabled():
+        for _, t in named:
+            if t is not None and t.requires_grad:
+                raise ValueError("%s records no autograd graph: call it under torch.no_grad(); gradients are a call of "
+                                 "their own" % what)
     dev = None
-    for name, t in tensors.items():
+    for name, t in named:
         if t is None:
             continue
         if not t.is_cuda:
@@ -24,17 +50,19 @@ def on_device(what, **tensors):
             dev = t.device
         elif t.device != dev:
             raise ValueError("%s: %s is on %s, the others are on %s" % (what, name, t.device, dev))
+    return dev
 
 
-def no_graph(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("%s records no autograd graph: call it under torch.no_grad(); gradients are a call of their "
-                         "own" % what)
+def pointer(t):
+    return None if t is None else t.data_ptr()
 
 
-def rows(t):
-    """t with a contiguous last axis (any other strides stay)."""
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+def rows(t, furthest=None):
+    """t with a contiguous last axis; other strides stay, up to `furthest` between rows."""
+    strides = t.stride()
+    if (strides[-1] != 1 and t.shape[-1] > 1) or (furthest is not None and strides[-2] > furthest):
+        return t.contiguous()
+    return t
 
 
 def lengths_on(what, lengths, B, T, device):
@@ -42,18 +70,19 @@ def lengths_on(what, lengths, B, T, device):
     are checked here."""
     if lengths is None:
         return None
-    lengths = torch.as_tensor(lengths)
+    if not isinstance(lengths, torch.Tensor):
+        lengths = torch.as_tensor(lengths)
     if lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64):
         raise ValueError("%s: lengths must be int32 or int64 [%d], got %s %s"
                          % (what, B, lengths.dtype, tuple(lengths.shape)))
-    if lengths.is_cuda:
-        if lengths.device != device:
-            raise ValueError("%s: lengths is on %s, the others are on %s" % (what, lengths.device, device))
-    elif B and (int(lengths.min()) < 0 or int(lengths.max()) > T):
-        raise ValueError("%s: lengths must lie in 0..%d" % (what, T))
-    if lengths.dtype == torch.int64:
-        lengths = lengths.clamp(0, T)
-    return lengths.to(device=device, dtype=torch.int32).contiguous()
+    if not lengths.is_cuda:
+        if B and (int(lengths.min()) < 0 or int(lengths.max()) > T):
+            raise ValueError("%s: lengths must lie in 0..%d" % (what, T))
+    elif lengths.device != device:
+        raise ValueError("%s: lengths is on %s, the others are on %s" % (what, lengths.device, device))
+    elif lengths.dtype == torch.int32 and lengths.is_contiguous():
+        return lengths
+    return lengths.clamp(0, T).to(device=device, dtype=torch.int32).contiguous()
 
 
 def _span(t):

@@ -20,7 +20,7 @@ import functools
 import torch
 
 from . import _lib
-from ._seq import (DTYPES, are_tensors, columns_apart, lengths_on, no_graph, on_device, overlaps, rows, same_place,
+from ._seq import (DTYPES, are_tensors, call, columns_apart, lengths_on, on_device, overlaps, pointer, rows, same_place,
                    writable_rows)
 
 MAX_RANK = 64   # TTSX_ADAPTER_MAX_RANK
@@ -36,9 +36,9 @@ def _workspace_bytes(B, T, K, N, R, dtype):
 
 def _check(what, name, wide, x, down, up, scale):
     """Shapes and types: `wide` is y or dy."""
-    are_tensors(what, **{name: wide, "x": x, "down": down, "up": up})
+    are_tensors(what, (name, wide), ("x", x), ("down", down), ("up", up))
     if scale is not None:
-        are_tensors(what, scale=scale)
+        are_tensors(what, ("scale", scale))
     if wide.dim() not in (2, 3) or x.shape[:-1] != wide.shape[:-1]:
         raise ValueError("%s: %s [B,T,N] and x [B,T,K] (or [B,N] and [B,K]) must agree, got %s and %s"
                          % (what, name, tuple(wide.shape), tuple(x.shape)))
@@ -57,22 +57,22 @@ def _check(what, name, wide, x, down, up, scale):
         raise ValueError("%s: down and up must be contiguous" % what)
     if scale is not None and (scale.shape != (V,) or scale.dtype != torch.float32):
         raise ValueError("%s: scale must be float32 [%d], got %s %s" % (what, V, scale.dtype, tuple(scale.shape)))
-    no_graph(what, wide, x, down, up, scale)
-    on_device(what, **{name: wide, "x": x, "down": down, "up": up, "scale": scale})
+    return on_device(what, (name, wide), ("x", x), ("down", down), ("up", up), ("scale", scale))
 
 
 def _voices_on(what, voices, B, V, device):
-    voices = torch.as_tensor(voices)
+    if not isinstance(voices, torch.Tensor):
+        voices = torch.as_tensor(voices)
     if voices.shape != (B,) or voices.dtype not in (torch.int32, torch.int64):
         raise ValueError("%s: voices must be int32 or int64 [%d], got %s %s" % (what, B, voices.dtype, tuple(voices.shape)))
-    if voices.is_cuda:
-        if voices.device != device:
-            raise ValueError("%s: voices is on %s, the others are on %s" % (what, voices.device, device))
-    elif B and (int(voices.min()) < -1 or int(voices.max()) >= V):
-        raise IndexError("%s: voices must lie in -1..%d" % (what, V - 1))
-    if voices.dtype == torch.int64:
-        voices = voices.clamp(-1, V)
-    return voices.to(device=device, dtype=torch.int32).contiguous()
+    if not voices.is_cuda:
+        if B and (int(voices.min()) < -1 or int(voices.max()) >= V):
+            raise IndexError("%s: voices must lie in -1..%d" % (what, V - 1))
+    elif voices.device != device:
+        raise ValueError("%s: voices is on %s, the others are on %s" % (what, voices.device, device))
+    elif voices.dtype == torch.int32 and voices.is_contiguous():
+        return voices
+    return voices.clamp(-1, V).to(device=device, dtype=torch.int32).contiguous()
 
 
 def adapter_add(y, x, down, up, voices, scale=None, lengths=None, out=None):
@@ -83,52 +83,48 @@ def adapter_add(y, x, down, up, voices, scale=None, lengths=None, out=None):
     lengths[b] stay y's and x is not read there.  `out` takes the result; out=y works in place and leaves rows without
     an adapter untouched.  The result has y's type, rounded once."""
     what = "adapter_add"
-    _check(what, "y", y, x, down, up, scale)
-    if y.dim() == 2:
-        into = None
-        if out is not None:
-            are_tensors(what, out=out)
-            if out.shape != y.shape:
-                raise ValueError("%s: out must be %s %s like y, got %s %s"
-                                 % (what, y.dtype, tuple(y.shape), out.dtype, tuple(out.shape)))
-            into = out.unsqueeze(1)
-        got = adapter_add(y.unsqueeze(1), x.unsqueeze(1), down, up, voices, scale, lengths, into)
-        return out if out is not None else got.squeeze(1)
-    B, T, N = y.shape
-    K, (V, R) = x.shape[2], down.shape[:2]
+    dev = _check(what, "y", y, x, down, up, scale)
+    single = y.dim() == 2
+    into = None
     if out is not None:
-        are_tensors(what, out=out)
-        on_device(what, y=y, out=out)
-        no_graph(what, out)
+        are_tensors(what, ("out", out))
+        on_device(what, ("y", y), ("out", out))
         if out.shape != y.shape or out.dtype != y.dtype:
             raise ValueError("%s: out must be %s %s like y, got %s %s"
                              % (what, y.dtype, tuple(y.shape), out.dtype, tuple(out.shape)))
-        writable_rows(what, "out", out)
-        if overlaps(out, y) and not (same_place(out, y) or columns_apart(out, y)):
+        into = out.unsqueeze(1) if single else out
+    if single:
+        y, x = y.unsqueeze(1), x.unsqueeze(1)
+    B, T, N = y.shape
+    K, (V, R) = x.shape[2], down.shape[:2]
+    in_place = False
+    if into is not None:
+        writable_rows(what, "out", into)
+        in_place = same_place(into, y)
+        if not in_place and overlaps(into, y) and not columns_apart(into, y):
             raise ValueError("%s: out overlaps y" % what)
-        if overlaps(out, x) and not columns_apart(out, x):
+        if overlaps(into, x) and not columns_apart(into, x):
             raise ValueError("%s: out overlaps x" % what)
-        if overlaps(out, down) or overlaps(out, up):
+        if overlaps(into, down) or overlaps(into, up):
             raise ValueError("%s: out overlaps an adapter" % what)
-    dev = y.device
-    if out is None:
-        out = torch.empty(B, T, N, dtype=y.dtype, device=dev)
-    if B == 0 or T == 0 or N == 0:
-        return out
-    if K == 0:
-        return out if same_place(out, y) else out.copy_(y)
-    if not same_place(out, y):
-        y = rows(y)
-    x = rows(x)
-    with torch.cuda.device(dev):
-        voices = _voices_on(what, voices, B, V, dev)
-        lengths = lengths_on(what, lengths, B, T, dev)
-        scale = None if scale is None else scale.contiguous()
-        _lib.check(_lib.load().ttsx_adapter_add(
-            y.data_ptr(), y.stride(0), y.stride(1), x.data_ptr(), x.stride(0), x.stride(1), down.data_ptr(), up.data_ptr(),
-            voices.data_ptr(), _lib.ptr(scale), _lib.ptr(lengths), B, T, K, N, R, V, DTYPES[y.dtype], out.data_ptr(),
-            out.stride(0), out.stride(1), _lib.current_stream()), "ttsx_adapter_add")
-    return out
+    voices = _voices_on(what, voices, B, V, dev)
+    lengths = lengths_on(what, lengths, B, T, dev)
+    if into is None:
+        into = torch.empty((B, T, N), dtype=y.dtype, device=dev)
+    if B and T and N:
+        if K == 0:
+            if not in_place:
+                into.copy_(y)
+        else:
+            if not in_place:
+                y = rows(y)
+            x = rows(x)
+            scale = None if scale is None else scale.contiguous()
+            ys, xs, os = y.stride(), x.stride(), into.stride()
+            call("ttsx_adapter_add", dev, y.data_ptr(), ys[0], ys[1], x.data_ptr(), xs[0], xs[1], down.data_ptr(),
+                 up.data_ptr(), voices.data_ptr(), pointer(scale), pointer(lengths), B, T, K, N, R, V, DTYPES[y.dtype],
+                 into.data_ptr(), os[0], os[1])
+    return out if out is not None else into.squeeze(1) if single else into
 
 
 def adapter_backward(dy, x, down, up, voices, scale=None, lengths=None):
@@ -137,26 +133,26 @@ def adapter_backward(dy, x, down, up, voices, scale=None, lengths=None):
     [V,R,K] and dup [V,R,N] of their inputs' type: sums over all rows of a voice, kept in float32 and in a fixed order,
     so that two runs agree to the bit.  `scale` is a constant."""
     what = "adapter_backward"
-    _check(what, "dy", dy, x, down, up, scale)
-    if dy.dim() == 2:
-        dx, ddown, dup = adapter_backward(dy.unsqueeze(1), x.unsqueeze(1), down, up, voices, scale, lengths)
-        return dx.squeeze(1), ddown, dup
+    dev = _check(what, "dy", dy, x, down, up, scale)
+    single = dy.dim() == 2
+    if single:
+        dy, x = dy.unsqueeze(1), x.unsqueeze(1)
     B, T, N = dy.shape
-    K, (V, R), dev = x.shape[2], down.shape[:2], dy.device
-    dx = torch.empty(B, T, K, dtype=x.dtype, device=dev)
-    if B == 0 or T == 0 or K == 0 or N == 0:
-        return dx.zero_(), torch.zeros_like(down), torch.zeros_like(up)
+    K, (V, R) = x.shape[2], down.shape[:2]
+    voices = _voices_on(what, voices, B, V, dev)
+    lengths = lengths_on(what, lengths, B, T, dev)
+    dx = torch.empty((B, T, K), dtype=x.dtype, device=dev)
+    if not (B and T and K and N):
+        dx.zero_()
+        return dx.squeeze(1) if single else dx, torch.zeros_like(down), torch.zeros_like(up)
     ddown, dup = torch.empty_like(down), torch.empty_like(up)
     dtype = DTYPES[x.dtype]
     need = _workspace_bytes(B, T, K, N, R, dtype)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     dy, x = rows(dy), rows(x)
-    with torch.cuda.device(dev):
-        voices = _voices_on(what, voices, B, V, dev)
-        lengths = lengths_on(what, lengths, B, T, dev)
-        scale = None if scale is None else scale.contiguous()
-        _lib.check(_lib.load().ttsx_adapter_backward(
-            dy.data_ptr(), dy.stride(0), dy.stride(1), x.data_ptr(), x.stride(0), x.stride(1), down.data_ptr(),
-            up.data_ptr(), voices.data_ptr(), _lib.ptr(scale), _lib.ptr(lengths), B, T, K, N, R, V, dtype, dx.data_ptr(),
-            ddown.data_ptr(), dup.data_ptr(), ws.data_ptr(), need, _lib.current_stream()), "ttsx_adapter_backward")
-    return dx, ddown, dup
+    scale = None if scale is None else scale.contiguous()
+    ds, xs = dy.stride(), x.stride()
+    call("ttsx_adapter_backward", dev, dy.data_ptr(), ds[0], ds[1], x.data_ptr(), xs[0], xs[1], down.data_ptr(),
+         up.data_ptr(), voices.data_ptr(), pointer(scale), pointer(lengths), B, T, K, N, R, V, dtype, dx.data_ptr(),
+         ddown.data_ptr(), dup.data_ptr(), ws.data_ptr(), need)
+    return dx.squeeze(1) if single else dx, ddown, dup

@@ -25,6 +25,9 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+template <class IO>
+using Full = Lane<IO, IO::VEC>;  // 16 bytes of a lane
+
 constexpr int ROWS = 32;  // rows of a tile: two matrix fragments
 constexpr int WAVES = 4;
 
@@ -45,7 +48,7 @@ __device__ static inline f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     for (int j = 0; j < 4; ++j)
       c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
     return c;
-  } else if constexpr (IO::INF2 == IoBf16::INF2) {
+  } else if constexpr (IO::INF == IoBf16::INF) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   } else {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_kernel(AddArgs a) {
       const int c = cb * CB + l16 * VEC, n = min(max(a.N - c, 0), VEC);
       if (n == 0) continue;
       for (int r = q; r < rows; r += 4)
-        store_some<IO>(ob + r * a.o_ts + c, ADD ? load_some<IO>(yb + r * a.y_ts + c, n) : (u32x4){0, 0, 0, 0}, n);
+        Full<IO>::store_some(ob + r * a.o_ts + c, ADD ? Full<IO>::load_some(yb + r * a.y_ts + c, n) : (u32x4){0, 0, 0, 0}, n);
     }
     return;
   }
@@ -131,12 +134,12 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_kernel(AddArgs a) {
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const int r = 16 * m + l16;
-      xr[m] = r < live && n > 0 ? load_some<IO>(xb + r * a.x_ts + k, n) : (u32x4){0, 0, 0, 0};
+      xr[m] = r < live && n > 0 ? Full<IO>::load_some(xb + r * a.x_ts + k, n) : (u32x4){0, 0, 0, 0};
     }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int r = 16 * j + l16;
-      ar[j] = r < a.R && n > 0 ? load_some<IO>(A + (int64_t)r * a.K + k, n) : (u32x4){0, 0, 0, 0};
+      ar[j] = r < a.R && n > 0 ? Full<IO>::load_some(A + (int64_t)r * a.K + k, n) : (u32x4){0, 0, 0, 0};
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -171,7 +174,7 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_kernel(AddArgs a) {
       for (int c = 0; c < RP / 8; ++c) hid.u[r][c0 + c] = u[c];
     } else {
       float up = 1.0f;
-      if constexpr (IO::INF2 == IoF16::INF2) {
+      if constexpr (IO::INF == IoF16::INF) {
         // the row's largest magnitude to [2^13, 2^14): both parts and their products stay inside fp16 and fp32
         top = fmaxf(top, __shfl_xor(top, 1, 64));
         top = fmaxf(top, __shfl_xor(top, 2, 64));
@@ -199,7 +202,7 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_kernel(AddArgs a) {
 #pragma unroll
         for (int s = 0; s < RP / 4; ++s) {
           const int r = q * (RP / 4) + s;
-          bt[s] = r < a.R && n > 0 ? load_some<IO>(Bm + (int64_t)r * a.N + c, n) : (u32x4){0, 0, 0, 0};
+          bt[s] = r < a.R && n > 0 ? Full<IO>::load_some(Bm + (int64_t)r * a.N + c, n) : (u32x4){0, 0, 0, 0};
         }
       } else {
 #pragma unroll
@@ -208,7 +211,7 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_kernel(AddArgs a) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int r = RP == 16 ? 8 * (q & 1) + i : kb * 32 + 8 * q + i;
-            br[i] = r < a.R && n > 0 ? load_some<IO>(Bm + (int64_t)r * a.N + c, n) : (u32x4){0, 0, 0, 0};
+            br[i] = r < a.R && n > 0 ? Full<IO>::load_some(Bm + (int64_t)r * a.N + c, n) : (u32x4){0, 0, 0, 0};
           }
           transpose8(br, bt + 8 * kb);
         }
@@ -252,16 +255,16 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_kernel(AddArgs a) {
           if (row >= rows || (ADD && a.in_place && row >= live)) continue;
           float o[VEC];
           u32x4 yr = (u32x4){0, 0, 0, 0};
-          if constexpr (ADD) yr = load_some<IO>(yb + row * a.y_ts + c, n);
+          if constexpr (ADD) yr = Full<IO>::load_some(yb + row * a.y_ts + c, n);
           if (row < live) {
-            IO::unpack(yr, o);
+            Full<IO>::unpack(yr, o);
             float k = 1.0f;
-            if constexpr (!WIDE && IO::INF2 == IoF16::INF2) k = hid.factor[row];
+            if constexpr (!WIDE && IO::INF == IoF16::INF) k = hid.factor[row];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) o[j] = fmaf(k, z[j][i], o[j]);
-            yr = IO::pack(o);
+            yr = Full<IO>::pack(o);
           }
-          store_some<IO>(ob + row * a.o_ts + c, yr, n);
+          Full<IO>::store_some(ob + row * a.o_ts + c, yr, n);
         }
       }
     }
@@ -282,7 +285,7 @@ struct OuterArgs {
 template <class IO, int RP>
 __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
   constexpr int VEC = IO::VEC, NJ = RP / 16, CB = 16 * VEC;
-  constexpr bool SPLIT = IO::INF2 == IoBf16::INF2;  // the others multiply in fp32: fp16 has no range for u
+  constexpr bool SPLIT = IO::INF == IoBf16::INF;  // the others multiply in fp32: fp16 has no range for u
   typedef typename IO::elem E;
   const int group = blockIdx.x % a.groups, chunk = blockIdx.x / a.groups % a.chunks, b = blockIdx.x / a.groups / a.chunks;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
@@ -309,7 +312,7 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = r0 + 8 * q + i;
-      xr[i] = r < last && n > 0 ? load_some<IO>(src + r * ts, n) : (u32x4){0, 0, 0, 0};
+      xr[i] = r < last && n > 0 ? Full<IO>::load_some(src + r * ts, n) : (u32x4){0, 0, 0, 0};
     }
     u32x4 bt[8];
     if constexpr (SPLIT) transpose8(xr, bt);
@@ -327,7 +330,7 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
           two_parts<IO>(u[i], hi, lo);
           h[i] = (float)hi, l[i] = (float)lo;
         }
-        const u32x4 uh = IO::pack(h), ul = IO::pack(l);
+        const u32x4 uh = Full<IO>::pack(h), ul = Full<IO>::pack(l);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           acc[j][i] = mma<IO>(ul, bt[i], acc[j][i]);
@@ -337,7 +340,7 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
           float xv[VEC];
-          IO::unpack(xr[s], xv);
+          Full<IO>::unpack(xr[s], xv);
 #pragma unroll
           for (int i = 0; i < VEC; ++i)
             acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(u[s], xv[i], acc[j][i], 0, 0, 0);
@@ -354,7 +357,7 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
       float o[VEC];
 #pragma unroll
       for (int k = 0; k < VEC; ++k) o[k] = acc[j][k][i];
-      store_f32<VEC>(out + (int64_t)(16 * j + 4 * q + i) * total, n, o);
+      store_f32_some<VEC>(out + (int64_t)(16 * j + 4 * q + i) * total, n, o);
     }
 }
 

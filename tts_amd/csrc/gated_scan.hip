@@ -9,25 +9,24 @@
 //   dx_t = w_t G_t,  dg_t = f_t w_t (h_{t-1} - x_t) G_t,  dh_0 = f_1 G_1
 // and R -> f (dh + R), with R the product f G that a step hands to the one before it, composes in the same way.
 //
-// One pass over memory: a lane holds L consecutive steps of VEC channels (16 bytes a step) in registers, 8 lanes cover
-// 128 bytes of channels, the wave's 8 lane groups and the workgroup's 4 waves are consecutive in time.  A lane folds
-// its steps into one pair, the pairs are scanned by shuffles inside the wave and through LDS across the waves, and
-// the lane then runs its steps from the state it starts with.  A workgroup walks the tiles of its time chunk with the
-// state in registers.  Where the batch has too few channels to fill the chip the time axis is cut into chunks: a first
-// launch folds every chunk into a pair, and the second combines the pairs in front of its chunk.
+// One pass over memory: a lane holds L consecutive steps of N channels in registers, a group of lanes covers 128 bytes
+// of channels, the groups of a wave and the four waves of a workgroup are consecutive in time.  A lane folds its steps
+// into one pair, the pairs are scanned by shuffles inside the wave and through LDS across the waves, and the lane then
+// runs its steps from the state it starts with.  A workgroup walks the tiles of its time chunk with the state in
+// registers.  Where the batch has too few channels to fill the chip the time axis is cut into chunks: a first launch
+// folds every chunk into a pair, and the second combines the pairs in front of its chunk.
 #include "../../include/ttsx_seq.h"
 #include "seq_io.h"
 
 namespace {
 
-constexpr int GROUP = 8;           // lanes across the channels: 128 bytes
 constexpr int WAVES = 4;
-constexpr int TGROUPS = WAVES * 64 / GROUP;
 constexpr int BLOCK = TTSX_STATE_BLOCK;
 
 struct ScanArgs {
   const void *x, *g, *dh;
-  int64_t x_bs, x_ts, g_bs, g_ts, dh_bs, dh_ts;  // strides of batch and time in elements
+  int64_t x_bs, g_bs, dh_bs;   // strides of the batch, in elements
+  uint32_t x_ts, g_ts, dh_ts;  // strides of the rows, in bytes
   const float *h0, *dh_last, *states_in;
   const int32_t* lengths;
   int T, D, reverse, cols, chunks, per;  // per: tiles of a chunk
@@ -36,57 +35,114 @@ struct ScanArgs {
   float* pairs;  // [B][chunks][2][D]
 };
 
-// f = sigmoid(g), w = 1 - f, each to a few units in its own last place: w = e f with e = exp(-g) keeps its digits
-// where f rounds to one.  Below -87 the exponential overflows: f = 0, w = 1 (f is below 2e-38 there).  Comparisons that
-// a NaN fails leave it as it is.  fp32 logits carry g log2(e) in two parts; the 16-bit types' own steps are far larger.
-template <class IO>
-__device__ static inline void gate(float g, float& f, float& w) {
-  constexpr float L2E = 1.44269502f, L2E_LO = 1.92596303e-8f;
+// How a workgroup covers a tile: N channels and L steps per lane, GROUP lanes across the channels.
+template <class IO, int N_, int GROUP_, int L_>
+struct Shape {
+  typedef IO Type;
+  typedef Lane<IO, N_> Io;
+  typedef typename IO::elem E;
+  static constexpr int N = N_, GROUP = GROUP_, L = L_, TGROUPS = WAVES * 64 / GROUP, TILE = TGROUPS * L;
+  static_assert(TILE % BLOCK == 0 && BLOCK % L == 0, "a tile and some lane of it start at a kept state");
+};
+
+// w = sigmoid(-g); f = 1 - w wherever f is a factor of a state.  Long memories live in w: an error d of f is one of
+// d / w in the state, so w = e / (1 + e) keeps its own digits, with e = exp(-g) from exp2 of the rounded -g log2(e) and
+// what the rounding lost put back, and the difference 1 - w adds half a unit of f.  fw = f w, the slope of f, keeps its
+// digits at both ends.  Below -87 the exponential overflows: f is below 2e-38 there, w = 1.  A NaN stays one.
+__device__ static inline void gate(float g, float& w, float& fw) {
   const bool low = g < -87.0f;
-  if constexpr (IO::VEC == 4) {
-    g = low ? -87.0f : g;
-    g = g > 126.0f ? 126.0f : g;
-    const float t = -L2E * g;
-    const float lo = fmaf(-L2E, g, -t) - L2E_LO * g;
-    const float p = __builtin_amdgcn_exp2f(t);
-    const float e = fmaf(p, 0.693147182f * lo, p);
-    f = __builtin_amdgcn_rcpf(1.0f + e);
-    w = low ? 1.0f : e * f;
-    f = low ? 0.0f : f;
-  } else {
-    const float e = __builtin_amdgcn_exp2f(-L2E * g);
-    f = __builtin_amdgcn_rcpf(1.0f + e);
-    w = low ? 1.0f : e * f;
-  }
+  g = __builtin_elementwise_minimum(g, 126.0f);
+  const float t = -1.44269502f * g;
+  const float rest = fmaf(t, 1.90465421e-9f, fmaf(t, -0.693147182f, -g));  // -g - t ln 2, ln 2 in two parts
+  const float p = __builtin_amdgcn_exp2f(t);
+  const float e = fmaf(p, rest, p);
+  const float f = __builtin_amdgcn_rcpf(1.0f + e);
+  w = e * f;
+  fw = w * f;
+  w = low ? 1.0f : w;
+  fw = low ? 0.0f : fw;
 }
 
-// Element row of processing step p.
-__device__ static inline int row_of(int p, int len, int reverse) { return reverse ? len - 1 - p : p; }
-
 struct Place {
-  int b, chunk, col, lane8, tg, wave, lane;
+  int b, chunk, c, across, tg, wave, lane;  // c: first channel of the lane
+  bool on;                                  // the lane has channels
 };
+template <class S>
 __device__ static inline Place place(const ScanArgs& a) {
   Place q;
   const int id = blockIdx.x;
-  q.col = id % a.cols;
   q.chunk = id / a.cols % a.chunks;
   q.b = id / a.cols / a.chunks;
   q.wave = threadIdx.x >> 6;
   q.lane = threadIdx.x & 63;
-  q.lane8 = q.lane & (GROUP - 1);
-  q.tg = threadIdx.x / GROUP;
+  q.across = q.lane & (S::GROUP - 1);
+  q.tg = threadIdx.x / S::GROUP;
+  q.c = (id % a.cols * S::GROUP + q.across) * S::N;
+  q.on = q.c < a.D;
   return q;
 }
 
-// Inclusive scan of the pairs over the 8 groups of a wave, forward in time; then the pair before each group.
-template <int VEC>
+// The rows of a tile that starts at step p0: step p is row p, or row len-1-p from right to left.  `base` is the lowest
+// row, a scalar; a lane adds a 32-bit offset.  Lanes behind the end read the last row again; what they read becomes
+// +infinity for g (the gate that keeps the state) and zero for the others.
+template <class S>
+struct Tile {
+  int p0, count, reverse;
+  int64_t base;
+  __device__ inline Tile(int p0_, int len, int reverse_) : p0(p0_), reverse(reverse_) {
+    count = min(len - p0, S::TILE);
+    base = reverse ? len - p0 - count : p0;
+  }
+  __device__ inline uint32_t row(const Place& q, int i) const {
+    const int k = min(q.tg * S::L + i, count - 1);
+    return reverse ? count - 1 - k : k;
+  }
+  __device__ inline bool live(const Place& q, int i) const { return q.tg * S::L + i < count; }
+};
+template <class T>
+__device__ static inline T* shifted(T* base, int64_t bytes, uint32_t lane) {
+  typedef typename std::conditional<std::is_const<T>::value, const char, char>::type C;
+  return reinterpret_cast<T*>(reinterpret_cast<C*>(base) + bytes + lane);
+}
+// Strides below 2^22 bytes and rows below 2^9: the product of two 24-bit numbers.
+__device__ static inline uint32_t offset(uint32_t row, uint32_t stride, uint32_t c) { return __umul24(row, stride) + c; }
+
+template <class S>
+__device__ static inline void load_rows(typename S::Io::raw* r, const typename S::E* base, uint32_t stride, const Tile<S>& t,
+                                        const Place& q) {
+  const uint32_t c = (q.on ? q.c : 0) * sizeof(typename S::E);
+#pragma unroll
+  for (int i = 0; i < S::L; ++i)
+    r[i] = S::Io::load(shifted(base, t.base * stride, offset(t.row(q, i), stride, c)));
+}
+template <class S>
+__device__ static inline void blank_rows(typename S::Io::raw* r, uint32_t with, const Tile<S>& t, const Place& q) {
+#pragma unroll
+  for (int i = 0; i < S::L; ++i)
+    if (!t.live(q, i)) r[i] = S::Io::fill(with);
+}
+// To [T,D] contiguous.
+template <class S>
+__device__ static inline void store_row(typename S::E* base, uint32_t pitch, const Tile<S>& t, const Place& q, int i,
+                                        typename S::Io::raw r) {
+  if (t.live(q, i) && q.on)
+    S::Io::store(shifted(base, t.base * pitch, offset(t.row(q, i), pitch, q.c * sizeof(typename S::E))), r);
+}
+// Zero in rows from..to-1 of the tile's span.
+template <class S>
+__device__ static inline void zero_rows(typename S::E* base, uint32_t pitch, int p0, int from, int to, const Place& q) {
+  for (int p = max(p0, from) + q.tg; p < min(p0 + S::TILE, to); p += S::TGROUPS)
+    if (q.on) S::Io::store(shifted(base, (int64_t)p * pitch, q.c * sizeof(typename S::E)), S::Io::fill(0));
+}
+
+// Inclusive scan of the pairs over the lane groups of a wave, forward in time.
+template <class S>
 __device__ static inline void wave_scan(float* A, float* B, int lane) {
 #pragma unroll
-  for (int off = GROUP; off < 64; off *= 2) {
+  for (int off = S::GROUP; off < 64; off *= 2) {
     const bool on = lane >= off;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
+    for (int i = 0; i < S::N; ++i) {
       const float pa = __shfl_up(A[i], off, 64), pb = __shfl_up(B[i], off, 64);
       B[i] = on ? fmaf(A[i], pb, B[i]) : B[i];
       A[i] = on ? A[i] * pa : A[i];
@@ -94,13 +150,13 @@ __device__ static inline void wave_scan(float* A, float* B, int lane) {
   }
 }
 // The same from the last group back: B folds towards the wave's first step.
-template <int VEC>
+template <class S>
 __device__ static inline void wave_scan_back(float* A, float* B, int lane) {
 #pragma unroll
-  for (int off = GROUP; off < 64; off *= 2) {
+  for (int off = S::GROUP; off < 64; off *= 2) {
     const bool on = lane + off < 64;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
+    for (int i = 0; i < S::N; ++i) {
       const float pa = __shfl_down(A[i], off, 64), pb = __shfl_down(B[i], off, 64);
       B[i] = on ? fmaf(A[i], pb, B[i]) : B[i];
       A[i] = on ? A[i] * pa : A[i];
@@ -108,416 +164,458 @@ __device__ static inline void wave_scan_back(float* A, float* B, int lane) {
   }
 }
 
-// Forward pass.  FOLD: only the pair of a chunk (first launch of a cut time axis).
-template <class IO, int L, bool FOLD, bool SAVE>
-__global__ __launch_bounds__(WAVES * 64) void scan_kernel(ScanArgs a) {
-  constexpr int VEC = IO::VEC, TILE = TGROUPS * L;
-  typedef typename IO::elem E;
-  __shared__ float tot[2][WAVES][2][GROUP][VEC];
-  const Place q = place(a);
-  if (FOLD && q.chunk == a.chunks - 1) return;  // nothing starts behind the last chunk
-  const int c0 = (q.col * GROUP + q.lane8) * VEC;
-  const int n = min(max(a.D - c0, 0), VEC);
-  const int len = valid_rows(a.lengths, q.b, a.T);
-  const E* xb = static_cast<const E*>(a.x) + q.b * a.x_bs + c0;
-  const E* gb = static_cast<const E*>(a.g) + q.b * a.g_bs + c0;
-  E* hb = static_cast<E*>(a.h) + (int64_t)q.b * a.T * a.D + c0;
-  const int blocks = ceil_div(a.T, BLOCK);
-
-  float carry[VEC], prod[VEC];  // state in front of the tile; FOLD: the pair so far
+// What a value was computed from is forgotten: later uses start from the value alone instead of keeping the parts, which
+// the backward pass has no registers for.
+__device__ static inline void forget(float& v) { asm("" : "+v"(v)); }
+template <class S>
+__device__ static inline void forget(typename S::Io::raw& r) {
+  if constexpr (S::Io::W == 1) {
+    asm("" : "+v"(r));
+  } else {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) carry[i] = 0.0f, prod[i] = 1.0f;
-  if constexpr (!FOLD) {
-    if (a.h0) load_f32<VEC>(a.h0 + (int64_t)q.b * a.D + c0, n, carry);
-    const float* pr = a.pairs + (int64_t)q.b * a.chunks * 2 * a.D + c0;
-    for (int k = 0; k < q.chunk; ++k, pr += 2 * (int64_t)a.D) {
-      float A[VEC], B[VEC];
-      load_f32<VEC>(pr, n, A);
-      load_f32<VEC>(pr + a.D, n, B);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) carry[i] = fmaf(A[i], carry[i], B[i]);
+    for (int i = 0; i < S::Io::W; ++i) {
+      uint32_t w = r[i];
+      asm("" : "+v"(w));
+      r[i] = w;
     }
   }
+}
 
-  const int first = q.chunk * a.per * TILE, last = min(first + a.per * TILE, a.T);
+// The totals of the waves: product, forward fold, backward fold.
+template <class S>
+struct Totals {
+  float v[WAVES][3][S::GROUP][S::N];
+};
+
+// The pairs of `count` chunks, in order from chunk `first` on (step 1 or -1), applied to h: the lane groups take equal
+// runs of them, so one round trip to memory serves them all.
+template <class S>
+__device__ static inline void apply_chunks(const float* pairs, int D, int first, int step, int count, const Place& q,
+                                           Totals<S>& tot, float* h) {
+  constexpr int N = S::N;
+  const int each = ceil_div(count, S::TGROUPS), from = q.tg * each, to = min(from + each, count);
+  float A[N], B[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) A[j] = 1.0f, B[j] = 0.0f;
+  if (q.on)
+    for (int k = from; k < to; ++k) {
+      const float* pr = pairs + (int64_t)(first + step * k) * 2 * D + q.c;
+      float ka[N], kb[N];
+      load_f32<N>(pr, ka);
+      load_f32<N>(pr + D, kb);
+#pragma unroll
+      for (int j = 0; j < N; ++j) B[j] = fmaf(ka[j], B[j], kb[j]), A[j] *= ka[j];
+    }
+  wave_scan<S>(A, B, q.lane);
+  if (q.lane >= 64 - S::GROUP) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) tot.v[q.wave][0][q.across][j] = A[j], tot.v[q.wave][1][q.across][j] = B[j];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < WAVES; ++k)
+#pragma unroll
+    for (int j = 0; j < N; ++j) h[j] = fmaf(tot.v[k][0][q.across][j], h[j], tot.v[k][1][q.across][j]);
+}
+
+// Forward pass.  FOLD: only the pair of a chunk (first launch of a cut time axis).
+template <class S, bool FOLD, bool SAVE>
+__global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
+  constexpr int N = S::N, L = S::L;
+  typedef typename S::E E;
+  typedef typename S::Io Io;
+  __shared__ Totals<S> tot[2];
+  const Place q = place<S>(a);
+  if (FOLD && q.chunk == a.chunks - 1) return;  // nothing starts behind the last chunk
+  const int len = valid_rows(a.lengths, q.b, a.T), blocks = ceil_div(a.T, BLOCK);
+  const E* xb = static_cast<const E*>(a.x) + q.b * a.x_bs;
+  const E* gb = static_cast<const E*>(a.g) + q.b * a.g_bs;
+  E* hb = static_cast<E*>(a.h) + (int64_t)q.b * a.T * a.D;
+  const uint32_t pitch = a.D * sizeof(E);
+
+  float carry[N], prod[N];  // state in front of the tile; FOLD: the pair so far
+#pragma unroll
+  for (int j = 0; j < N; ++j) carry[j] = 0.0f, prod[j] = 1.0f;
+  if constexpr (!FOLD) {
+    if (a.h0 && q.on) load_f32<N>(a.h0 + (int64_t)q.b * a.D + q.c, carry);
+    if (q.chunk > 0)
+      apply_chunks<S>(a.pairs + (int64_t)q.b * a.chunks * 2 * a.D, a.D, 0, 1, q.chunk, q, tot[1], carry);
+  }
+
+  const int first = q.chunk * a.per * S::TILE, last = min(first + a.per * S::TILE, a.T);
   int flip = 0;
-  for (int p0 = first; p0 < last; p0 += TILE, flip ^= 1) {
+  for (int p0 = first; p0 < last; p0 += S::TILE, flip ^= 1) {
     const int p = p0 + q.tg * L;
+    const bool keeps = SAVE && p % BLOCK == 0 && p < a.T && q.on;
+    float* kept = SAVE ? a.states + ((int64_t)q.b * blocks + p / BLOCK) * a.D + q.c : nullptr;
     if (p0 >= len) {  // behind the end: zero rows, the state stays
       if constexpr (FOLD) break;
-#pragma unroll
-      for (int i = 0; i < L; ++i)
-        if (p + i < a.T && n > 0) store_some<IO>(hb + (int64_t)(p + i) * a.D, (u32x4){0, 0, 0, 0}, n);
-      if (SAVE && p % BLOCK == 0 && p < a.T)
-        store_f32<VEC>(a.states + ((int64_t)q.b * blocks + p / BLOCK) * a.D + c0, n, carry);
+      zero_rows<S>(hb, pitch, p0, len, a.T, q);
+      if (keeps) store_f32<N>(kept, carry);
       continue;
     }
-    u32x4 xr[L], gr[L];
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      // a row behind the end keeps the state: f = 1, w x = 0
-      gr[i] = (u32x4){IO::INF2, IO::INF2, IO::INF2, IO::INF2};
-      xr[i] = (u32x4){0, 0, 0, 0};
-      if (p + i < len && n > 0) {
-        const int64_t t = row_of(p + i, len, a.reverse);
-        gr[i] = load_some<IO>(gb + t * a.g_ts, n);
-        xr[i] = load_some<IO>(xb + t * a.x_ts, n);
-      }
+    const Tile<S> t(p0, len, a.reverse);
+    typename Io::raw xr[L], gr[L];
+    load_rows<S>(gr, gb, a.g_ts, t, q);
+    load_rows<S>(xr, xb, a.x_ts, t, q);
+    if (t.count < S::TILE) {  // the same for the workgroup
+      blank_rows<S>(gr, S::Type::INF, t, q);
+      blank_rows<S>(xr, 0, t, q);
+      if constexpr (!FOLD) zero_rows<S>(hb, pitch, p0, len, a.T, q);
     }
-    float f[L][VEC], v[L][VEC], A[VEC], B[VEC];
+    float f[L][N], v[L][N], A[N], B[N];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) A[i] = 1.0f, B[i] = 0.0f;
+    for (int j = 0; j < N; ++j) A[j] = 1.0f, B[j] = 0.0f;
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      float gv[VEC], xv[VEC];
-      IO::unpack(gr[i], gv);
-      IO::unpack(xr[i], xv);
+      float gv[N], xv[N];
+      Io::unpack(gr[i], gv);
+      Io::unpack(xr[i], xv);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float w;
-        gate<IO>(gv[j], f[i][j], w);
+      for (int j = 0; j < N; ++j) {
+        float w, fw;
+        gate(gv[j], w, fw);
+        f[i][j] = 1.0f - w;
         v[i][j] = w * xv[j];
         A[j] *= f[i][j];
         B[j] = fmaf(f[i][j], B[j], v[i][j]);
       }
     }
-    wave_scan<VEC>(A, B, q.lane);
-    if (q.lane >= 64 - GROUP) {
+    wave_scan<S>(A, B, q.lane);
+    if (q.lane >= 64 - S::GROUP) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) tot[flip][q.wave][0][q.lane8][j] = A[j], tot[flip][q.wave][1][q.lane8][j] = B[j];
+      for (int j = 0; j < N; ++j) tot[flip].v[q.wave][0][q.across][j] = A[j], tot[flip].v[q.wave][1][q.across][j] = B[j];
     }
     __syncthreads();  // the other half of `tot` is written next: one barrier per tile
-    if constexpr (FOLD) {
+    float h[N];       // state in front of the wave, then of the lane
 #pragma unroll
-      for (int k = 0; k < WAVES; ++k)
+    for (int k = 0; k < WAVES; ++k)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float ta = tot[flip][k][0][q.lane8][j];
-          carry[j] = fmaf(ta, carry[j], tot[flip][k][1][q.lane8][j]);
-          prod[j] *= ta;
-        }
-    } else {
-      float h[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float s = carry[j], mine = s;
-#pragma unroll
-        for (int k = 0; k < WAVES; ++k) {
-          if (k == q.wave) mine = s;
-          s = fmaf(tot[flip][k][0][q.lane8][j], s, tot[flip][k][1][q.lane8][j]);
-        }
-        carry[j] = s;
-        const float pa = __shfl_up(A[j], GROUP, 64), pb = __shfl_up(B[j], GROUP, 64);
-        h[j] = q.lane >= GROUP ? fmaf(pa, mine, pb) : mine;
+      for (int j = 0; j < N; ++j) {
+        const float ta = tot[flip].v[k][0][q.across][j], tb = tot[flip].v[k][1][q.across][j];
+        if (k == q.wave) h[j] = carry[j];
+        carry[j] = fmaf(ta, carry[j], tb);
+        if (FOLD) prod[j] *= ta;
       }
-      if (SAVE && p % BLOCK == 0 && p < a.T)
-        store_f32<VEC>(a.states + ((int64_t)q.b * blocks + p / BLOCK) * a.D + c0, n, h);
+    if constexpr (!FOLD) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float pa = __shfl_up(A[j], S::GROUP, 64), pb = __shfl_up(B[j], S::GROUP, 64);
+        h[j] = q.lane >= S::GROUP ? fmaf(pa, h[j], pb) : h[j];
+      }
+      if (keeps) store_f32<N>(kept, h);
 #pragma unroll
       for (int i = 0; i < L; ++i) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) h[j] = fmaf(f[i][j], h[j], v[i][j]);
-        if (p + i < a.T && n > 0) {
-          const bool live = p + i < len;
-          const int64_t t = live ? row_of(p + i, len, a.reverse) : p + i;
-          store_some<IO>(hb + t * a.D, live ? IO::pack(h) : (u32x4){0, 0, 0, 0}, n);
-        }
+        for (int j = 0; j < N; ++j) h[j] = fmaf(f[i][j], h[j], v[i][j]);
+        store_row<S>(hb, pitch, t, q, i, Io::pack(h));
       }
     }
   }
+  if (q.tg != 0 || !q.on) return;
   if constexpr (FOLD) {
-    float* pr = a.pairs + ((int64_t)q.b * a.chunks + q.chunk) * 2 * a.D + c0;
-    if (q.tg == 0) {
-      store_f32<VEC>(pr, n, prod);
-      store_f32<VEC>(pr + a.D, n, carry);
-    }
-  } else if (q.chunk == a.chunks - 1 && q.tg == 0) {
-    store_f32<VEC>(a.h_last + (int64_t)q.b * a.D + c0, n, carry);
+    float* pr = a.pairs + ((int64_t)q.b * a.chunks + q.chunk) * 2 * a.D + q.c;
+    store_f32<N>(pr, prod);
+    store_f32<N>(pr + a.D, carry);
+  } else if (q.chunk == a.chunks - 1) {
+    store_f32<N>(a.h_last + (int64_t)q.b * a.D + q.c, carry);
   }
 }
 
 // Backward pass.  FOLD: only the pair (product of f, folded f dh) of a chunk, from its last step to its first.
-template <class IO, int L, bool FOLD>
-__global__ __launch_bounds__(WAVES * 64) void scan_backward_kernel(ScanArgs a) {
-  constexpr int VEC = IO::VEC, TILE = TGROUPS * L;
-  static_assert(TILE % BLOCK == 0, "a tile starts at a kept state");
-  typedef typename IO::elem E;
-  __shared__ float tot[2][WAVES][3][GROUP][VEC];
-  const Place q = place(a);
+template <class S, bool FOLD>
+__global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a) {
+  constexpr int N = S::N, L = S::L;
+  typedef typename S::E E;
+  typedef typename S::Io Io;
+  __shared__ Totals<S> tot[2];
+  const Place q = place<S>(a);
   if (FOLD && q.chunk == 0) return;  // nothing lies in front of the first chunk
-  const int c0 = (q.col * GROUP + q.lane8) * VEC;
-  const int n = min(max(a.D - c0, 0), VEC);
-  const int len = valid_rows(a.lengths, q.b, a.T);
-  const E* xb = static_cast<const E*>(a.x) + q.b * a.x_bs + c0;
-  const E* gb = static_cast<const E*>(a.g) + q.b * a.g_bs + c0;
-  const E* db = static_cast<const E*>(a.dh) + q.b * a.dh_bs + c0;
-  E* dxb = static_cast<E*>(a.dx) + (int64_t)q.b * a.T * a.D + c0;
-  E* dgb = static_cast<E*>(a.dg) + (int64_t)q.b * a.T * a.D + c0;
-  const int blocks = ceil_div(a.T, BLOCK);
+  const int len = valid_rows(a.lengths, q.b, a.T), blocks = ceil_div(a.T, BLOCK);
+  const E* xb = static_cast<const E*>(a.x) + q.b * a.x_bs;
+  const E* gb = static_cast<const E*>(a.g) + q.b * a.g_bs;
+  const E* db = static_cast<const E*>(a.dh) + q.b * a.dh_bs;
+  E* dxb = static_cast<E*>(a.dx) + (int64_t)q.b * a.T * a.D;
+  E* dgb = static_cast<E*>(a.dg) + (int64_t)q.b * a.T * a.D;
+  const uint32_t pitch = a.D * sizeof(E);
 
-  float carry[VEC], prod[VEC];  // R behind the tile; FOLD: the pair so far
+  float carry[N], prod[N];  // R behind the tile; FOLD: the pair so far
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) carry[i] = 0.0f, prod[i] = 1.0f;
+  for (int j = 0; j < N; ++j) carry[j] = 0.0f, prod[j] = 1.0f;
   if constexpr (!FOLD) {
-    if (a.dh_last) load_f32<VEC>(a.dh_last + (int64_t)q.b * a.D + c0, n, carry);
-    for (int k = a.chunks - 1; k > q.chunk; --k) {
-      const float* pr = a.pairs + ((int64_t)q.b * a.chunks + k) * 2 * a.D + c0;
-      float A[VEC], B[VEC];
-      load_f32<VEC>(pr, n, A);
-      load_f32<VEC>(pr + a.D, n, B);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) carry[i] = fmaf(A[i], carry[i], B[i]);
-    }
+    if (a.dh_last && q.on) load_f32<N>(a.dh_last + (int64_t)q.b * a.D + q.c, carry);
+    if (q.chunk < a.chunks - 1)
+      apply_chunks<S>(a.pairs + (int64_t)q.b * a.chunks * 2 * a.D, a.D, a.chunks - 1, -1, a.chunks - 1 - q.chunk, q,
+                      tot[1], carry);
   }
 
-  const int first = q.chunk * a.per * TILE, last = min(first + a.per * TILE, a.T);
+  const int first = q.chunk * a.per * S::TILE, last = min(first + a.per * S::TILE, a.T);
   int flip = 0;
-  for (int p0 = first + (ceil_div(last - first, TILE) - 1) * TILE; p0 >= first; p0 -= TILE, flip ^= 1) {
-    const int p = p0 + q.tg * L;
+  for (int p0 = first + (ceil_div(last - first, S::TILE) - 1) * S::TILE; p0 >= first; p0 -= S::TILE, flip ^= 1) {
     if (p0 >= len) {
       if constexpr (!FOLD) {
-#pragma unroll
-        for (int i = 0; i < L; ++i)
-          if (p + i < a.T && n > 0) {
-            store_some<IO>(dxb + (int64_t)(p + i) * a.D, (u32x4){0, 0, 0, 0}, n);
-            store_some<IO>(dgb + (int64_t)(p + i) * a.D, (u32x4){0, 0, 0, 0}, n);
-          }
+        zero_rows<S>(dxb, pitch, p0, len, a.T, q);
+        zero_rows<S>(dgb, pitch, p0, len, a.T, q);
       }
       continue;
     }
-    u32x4 xr[L], gr[L], dr[L];
-    float start[VEC];
-    if constexpr (!FOLD) load_f32<VEC>(a.states_in + ((int64_t)q.b * blocks + p0 / BLOCK) * a.D + c0, n, start);
+    const Tile<S> t(p0, len, a.reverse);
+    typename Io::raw xr[L], gr[L], dr[L];
+    float h[N];  // state in front of the tile
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      gr[i] = (u32x4){IO::INF2, IO::INF2, IO::INF2, IO::INF2};
-      xr[i] = dr[i] = (u32x4){0, 0, 0, 0};
-      if (p + i < len && n > 0) {
-        const int64_t t = row_of(p + i, len, a.reverse);
-        gr[i] = load_some<IO>(gb + t * a.g_ts, n);
-        dr[i] = load_some<IO>(db + t * a.dh_ts, n);
-        if constexpr (!FOLD) xr[i] = load_some<IO>(xb + t * a.x_ts, n);
+    for (int j = 0; j < N; ++j) h[j] = 0.0f;
+    load_rows<S>(gr, gb, a.g_ts, t, q);
+    load_rows<S>(dr, db, a.dh_ts, t, q);
+    if constexpr (!FOLD) {
+      load_rows<S>(xr, xb, a.x_ts, t, q);
+      if (q.on) load_f32<N>(a.states_in + ((int64_t)q.b * blocks + p0 / BLOCK) * a.D + q.c, h);
+    }
+    if (t.count < S::TILE) {  // the same for the workgroup
+      blank_rows<S>(gr, S::Type::INF, t, q);
+      blank_rows<S>(dr, 0, t, q);
+      if constexpr (!FOLD) {
+        blank_rows<S>(xr, 0, t, q);
+        zero_rows<S>(dxb, pitch, p0, len, a.T, q);
+        zero_rows<S>(dgb, pitch, p0, len, a.T, q);
       }
     }
-    // A: product of f; B: the forward fold; C: the backward fold of f dh
-    float f[L][VEC], w[L][VEC], A[VEC], A2[VEC], B[VEC], C[VEC];
+    // s: f w, later dg / G.  A: product of f; B: the forward fold; C: the backward fold of f dh
+    float w[L][N], s[L][N], A[N], A2[N], B[N], C[N];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[j] = C[j] = 0.0f;
+    for (int j = 0; j < N; ++j) A[j] = 1.0f, B[j] = C[j] = 0.0f;
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      float gv[VEC], xv[VEC];
-      IO::unpack(gr[i], gv);
-      IO::unpack(xr[i], xv);
+      float gv[N], xv[N];
+      Io::unpack(gr[i], gv);
+      if constexpr (!FOLD) Io::unpack(xr[i], xv);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        gate<IO>(gv[j], f[i][j], w[i][j]);
-        A[j] *= f[i][j];
-        if constexpr (!FOLD) B[j] = fmaf(f[i][j], B[j], w[i][j] * xv[j]);
+      for (int j = 0; j < N; ++j) {
+        gate(gv[j], w[i][j], s[i][j]);
+        A[j] *= 1.0f - w[i][j];
+        if constexpr (!FOLD) B[j] = fmaf(1.0f - w[i][j], B[j], w[i][j] * xv[j]);
+        forget(w[i][j]);
+        if constexpr (!FOLD) forget(s[i][j]);
       }
+      if constexpr (!FOLD) forget<S>(xr[i]);
     }
 #pragma unroll
     for (int i = L - 1; i >= 0; --i) {
-      float dv[VEC];
-      IO::unpack(dr[i], dv);
+      float dv[N];
+      Io::unpack(dr[i], dv);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) C[j] = f[i][j] * (C[j] + dv[j]);
+      for (int j = 0; j < N; ++j) C[j] = (1.0f - w[i][j]) * (C[j] + dv[j]);
+      if constexpr (!FOLD) forget<S>(dr[i]);
     }
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) A2[j] = A[j];
-    wave_scan_back<VEC>(A2, C, q.lane);
-    if constexpr (!FOLD) wave_scan<VEC>(A, B, q.lane);
-    if (q.lane < GROUP) {
+    for (int i = 0; i < L; ++i)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) tot[flip][q.wave][0][q.lane8][j] = A2[j], tot[flip][q.wave][2][q.lane8][j] = C[j];
+      for (int j = 0; j < N; ++j) forget(w[i][j]);
+#pragma unroll
+    for (int j = 0; j < N; ++j) A2[j] = A[j];
+    wave_scan_back<S>(A2, C, q.lane);
+    if constexpr (!FOLD) wave_scan<S>(A, B, q.lane);
+    if (q.lane < S::GROUP) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) tot[flip].v[q.wave][0][q.across][j] = A2[j], tot[flip].v[q.wave][2][q.across][j] = C[j];
     }
-    if (!FOLD && q.lane >= 64 - GROUP) {
+    if (!FOLD && q.lane >= 64 - S::GROUP) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) tot[flip][q.wave][1][q.lane8][j] = B[j];
+      for (int j = 0; j < N; ++j) tot[flip].v[q.wave][1][q.across][j] = B[j];
     }
     __syncthreads();
-    if constexpr (FOLD) {
+    float R[N];  // gradient behind the wave, then behind the lane
 #pragma unroll
-      for (int k = WAVES - 1; k >= 0; --k)
+    for (int k = WAVES - 1; k >= 0; --k)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float ta = tot[flip][k][0][q.lane8][j];
-          carry[j] = fmaf(ta, carry[j], tot[flip][k][2][q.lane8][j]);
-          prod[j] *= ta;
-        }
-    } else {
-      float h[VEC], R[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float s = start[j], mine = s;
-#pragma unroll
-        for (int k = 0; k < WAVES; ++k) {
-          if (k == q.wave) mine = s;
-          s = fmaf(tot[flip][k][0][q.lane8][j], s, tot[flip][k][1][q.lane8][j]);
-        }
-        float pa = __shfl_up(A[j], GROUP, 64), pb = __shfl_up(B[j], GROUP, 64);
-        h[j] = q.lane >= GROUP ? fmaf(pa, mine, pb) : mine;
-        s = carry[j];
-#pragma unroll
-        for (int k = WAVES - 1; k >= 0; --k) {
-          if (k == q.wave) mine = s;
-          s = fmaf(tot[flip][k][0][q.lane8][j], s, tot[flip][k][2][q.lane8][j]);
-        }
-        carry[j] = s;
-        pa = __shfl_down(A2[j], GROUP, 64), pb = __shfl_down(C[j], GROUP, 64);
-        R[j] = q.lane < 64 - GROUP ? fmaf(pa, mine, pb) : mine;
+      for (int j = 0; j < N; ++j) {
+        const float ta = tot[flip].v[k][0][q.across][j];
+        if (k == q.wave) R[j] = carry[j];
+        carry[j] = fmaf(ta, carry[j], tot[flip].v[k][2][q.across][j]);
+        if (FOLD) prod[j] *= ta;
       }
-      // the states of the lane's steps again; dg_t / G_t stays in s
-      float s[L][VEC];
+    if constexpr (!FOLD) {
+      for (int k = 0; k < q.wave; ++k)
+#pragma unroll
+        for (int j = 0; j < N; ++j) h[j] = fmaf(tot[flip].v[k][0][q.across][j], h[j], tot[flip].v[k][1][q.across][j]);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        float pa = __shfl_up(A[j], S::GROUP, 64), pb = __shfl_up(B[j], S::GROUP, 64);
+        h[j] = q.lane >= S::GROUP ? fmaf(pa, h[j], pb) : h[j];
+        pa = __shfl_down(A2[j], S::GROUP, 64), pb = __shfl_down(C[j], S::GROUP, 64);
+        R[j] = q.lane < 64 - S::GROUP ? fmaf(pa, R[j], pb) : R[j];
+      }
+      // the states of the lane's steps again
 #pragma unroll
       for (int i = 0; i < L; ++i) {
-        float xv[VEC];
-        IO::unpack(xr[i], xv);
+        float xv[N];
+        Io::unpack(xr[i], xv);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          s[i][j] = f[i][j] * w[i][j] * (h[j] - xv[j]);
-          h[j] = fmaf(f[i][j], h[j], w[i][j] * xv[j]);
+        for (int j = 0; j < N; ++j) {
+          s[i][j] *= h[j] - xv[j];
+          h[j] = fmaf(1.0f - w[i][j], h[j], w[i][j] * xv[j]);
+          forget(w[i][j]);
+          forget(s[i][j]);
         }
       }
 #pragma unroll
       for (int i = L - 1; i >= 0; --i) {
-        float dv[VEC], gx[VEC], gg[VEC];
-        IO::unpack(dr[i], dv);
+        float dv[N], gx[N], gg[N];
+        Io::unpack(dr[i], dv);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
+        for (int j = 0; j < N; ++j) {
           const float G = dv[j] + R[j];
           gx[j] = w[i][j] * G;
           gg[j] = s[i][j] * G;
-          R[j] = f[i][j] * G;
+          R[j] = (1.0f - w[i][j]) * G;
         }
-        if (p + i < a.T && n > 0) {
-          const bool live = p + i < len;
-          const int64_t t = live ? row_of(p + i, len, a.reverse) : p + i;
-          store_some<IO>(dxb + t * a.D, live ? IO::pack(gx) : (u32x4){0, 0, 0, 0}, n);
-          store_some<IO>(dgb + t * a.D, live ? IO::pack(gg) : (u32x4){0, 0, 0, 0}, n);
-        }
+        store_row<S>(dxb, pitch, t, q, i, Io::pack(gx));
+        store_row<S>(dgb, pitch, t, q, i, Io::pack(gg));
       }
     }
   }
+  if (q.tg != 0 || !q.on) return;
   if constexpr (FOLD) {
-    float* pr = a.pairs + ((int64_t)q.b * a.chunks + q.chunk) * 2 * a.D + c0;
-    if (q.tg == 0) {
-      store_f32<VEC>(pr, n, prod);
-      store_f32<VEC>(pr + a.D, n, carry);
-    }
-  } else if (q.chunk == 0 && q.tg == 0) {
-    store_f32<VEC>(a.dh0 + (int64_t)q.b * a.D + c0, n, carry);
+    float* pr = a.pairs + ((int64_t)q.b * a.chunks + q.chunk) * 2 * a.D + q.c;
+    store_f32<N>(pr, prod);
+    store_f32<N>(pr + a.D, carry);
+  } else if (q.chunk == 0) {
+    store_f32<N>(a.dh0 + (int64_t)q.b * a.D + q.c, carry);
   }
 }
 
-// One step of every request: elementwise, a lane takes 16 bytes of x.
-template <class IO>
+// One step of every request: elementwise.
+template <class IO, int N>
 __global__ __launch_bounds__(256) void step_kernel(const typename IO::elem* x, int64_t x_bs, const typename IO::elem* g,
                                                    int64_t g_bs, const float* h, int B, int D, typename IO::elem* y,
                                                    float* h_out) {
-  constexpr int VEC = IO::VEC;
-  const int cols = ceil_div(D, VEC);
+  typedef Lane<IO, N> Io;
+  const int cols = D / N;
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int b = (int)(id / cols), c = (int)(id % cols) * VEC;
+  const int64_t b = id / cols;
+  const int c = (int)(id % cols) * N;
   if (b >= B) return;
-  const int n = min(D - c, VEC);
-  float xv[VEC], gv[VEC], hv[VEC];
-  IO::unpack(load_some<IO>(x + b * x_bs + c, n), xv);
-  IO::unpack(load_some<IO>(g + b * g_bs + c, n), gv);
-  load_f32<VEC>(h + (int64_t)b * D + c, n, hv);
+  float xv[N], gv[N], hv[N];
+  Io::unpack(Io::load(x + b * x_bs + c), xv);
+  Io::unpack(Io::load(g + b * g_bs + c), gv);
+  load_f32<N>(h + b * D + c, hv);
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    float f, w;
-    gate<IO>(gv[j], f, w);
-    hv[j] = fmaf(f, hv[j], w * xv[j]);
+  for (int j = 0; j < N; ++j) {
+    float w, fw;
+    gate(gv[j], w, fw);
+    hv[j] = fmaf(1.0f - w, hv[j], w * xv[j]);
   }
-  store_some<IO>(y + (int64_t)b * D + c, IO::pack(hv), n);
-  store_f32<VEC>(h_out + (int64_t)b * D + c, n, hv);
+  Io::store(y + b * D + c, Io::pack(hv));
+  store_f32<N>(h_out + b * D + c, hv);
 }
 
-// Steps a lane holds: the forward pass keeps f and w x of each, the backward pass f, w, dg / G and the inputs.
+// Lanes take 8 bytes of a row where D is a whole number of them, else one channel.  A tile costs its scans once, and few
+// channels over many steps make that small: 16 channel-steps per lane forwards (32 are no faster: 60 against 58 us at
+// 64 x 800 x 512 fp32; 16-byte lanes neither), 32 backwards (108 us at 64 x 800 x 1024 bf16; 16: 120, 16-byte lanes: 158).
 template <class IO>
-constexpr int FWD_L = 8;
+using WideFwd = Shape<IO, 2 * IO::PER, 16, 8 / IO::PER>;
 template <class IO>
-constexpr int BWD_L = IO::VEC == 4 ? 8 : 4;
+using WideBwd = Shape<IO, 2 * IO::PER, 16, 16 / IO::PER>;
+template <class IO>
+using Narrow = Shape<IO, 1, 64, 16>;
+template <class IO>
+bool wide(int D) {
+  return D % WideFwd<IO>::N == 0;
+}
 
 struct Plan {
   int cols, chunks, per;
 };
-// How the time axis is cut: enough workgroups to fill 256 CUs three times over, one tile at least to each.
-Plan plan(int B, int T, int D, int vec, int L) {
+// How the time axis is cut: enough workgroups to fill 256 CUs four times over, one tile at least to each.
+template <class S>
+Plan plan(int B, int T, int D) {
   Plan p;
-  const int tiles = ceil_div(T, TGROUPS * L);
-  p.cols = ceil_div(D, GROUP * vec);
+  const int tiles = ceil_div(T, S::TILE);
+  p.cols = ceil_div(D, S::GROUP * S::N);
   const int64_t rows = (int64_t)B * p.cols;
-  const int want = (int)(rows >= 768 ? 1 : 768 / rows);
+  const int want = (int)(rows >= 1024 ? 1 : 1024 / rows);
   p.per = ceil_div(tiles, want < tiles ? want : tiles);
   p.chunks = ceil_div(tiles, p.per);
   return p;
 }
+template <class S>
+size_t pairs_bytes(int B, int T, int D) {
+  const Plan p = plan<S>(B, T, D);
+  return p.chunks == 1 ? 0 : sizeof(float) * 2 * (size_t)B * p.chunks * D;
+}
 
-template <class IO>
-int run_scan(ScanArgs a, int B, size_t ws_bytes, hipStream_t s) {
-  const Plan p = plan(B, a.T, a.D, IO::VEC, FWD_L<IO>);
+template <class S>
+int launch(ScanArgs a, int B, size_t ws_bytes, bool backward, hipStream_t s) {
+  const char* name = backward ? "ttsx_gated_scan_backward" : "ttsx_gated_scan";
+  const Plan p = plan<S>(B, a.T, a.D);
   a.cols = p.cols, a.chunks = p.chunks, a.per = p.per;
-  TTSX_ARG(p.chunks == 1 || (a.pairs && ws_bytes >= sizeof(float) * 2 * B * p.chunks * a.D),
-           "ttsx_gated_scan: workspace too small");
+  TTSX_ARG(p.chunks == 1 || (a.pairs && ws_bytes >= pairs_bytes<S>(B, a.T, a.D)), "%s: workspace too small", name);
   const int64_t grid = (int64_t)B * p.cols * p.chunks;
-  TTSX_ARG(grid <= 0x7fffffff, "ttsx_gated_scan: too many channels");
+  TTSX_ARG(grid <= 0x7fffffff, "%s: too many channels", name);
+  const dim3 g((unsigned)grid), t(WAVES * 64);
   if (p.chunks > 1) {
-    scan_kernel<IO, FWD_L<IO>, true, false><<<(unsigned)grid, WAVES * 64, 0, s>>>(a);
+    if (backward)
+      scan_backward_kernel<S, true><<<g, t, 0, s>>>(a);
+    else
+      scan_kernel<S, true, false><<<g, t, 0, s>>>(a);
     TTSX_LAUNCH_CHECK();
   }
-  if (a.states)
-    scan_kernel<IO, FWD_L<IO>, false, true><<<(unsigned)grid, WAVES * 64, 0, s>>>(a);
+  if (backward)
+    scan_backward_kernel<S, false><<<g, t, 0, s>>>(a);
+  else if (a.states)
+    scan_kernel<S, false, true><<<g, t, 0, s>>>(a);
   else
-    scan_kernel<IO, FWD_L<IO>, false, false><<<(unsigned)grid, WAVES * 64, 0, s>>>(a);
+    scan_kernel<S, false, false><<<g, t, 0, s>>>(a);
   TTSX_LAUNCH_CHECK();
   return TTSX_OK;
+}
+
+// The widest row stride: the offsets inside a tile fit 32 bits.
+constexpr int64_t MAX_STRIDE = 1 << 20;
+bool stride_ok(int64_t s) { return s >= 0 && s <= MAX_STRIDE; }
+
+template <class IO>
+int run_scan(ScanArgs a, int64_t x_ts, int64_t g_ts, int64_t dh_ts, int B, size_t ws_bytes, bool backward, hipStream_t s) {
+  a.x_ts = (uint32_t)(x_ts * sizeof(typename IO::elem));
+  a.g_ts = (uint32_t)(g_ts * sizeof(typename IO::elem));
+  a.dh_ts = (uint32_t)(dh_ts * sizeof(typename IO::elem));
+  if (!wide<IO>(a.D)) return launch<Narrow<IO>>(a, B, ws_bytes, backward, s);
+  return backward ? launch<WideBwd<IO>>(a, B, ws_bytes, true, s) : launch<WideFwd<IO>>(a, B, ws_bytes, false, s);
 }
 
 template <class IO>
-int run_backward(ScanArgs a, int B, size_t ws_bytes, hipStream_t s) {
-  const Plan p = plan(B, a.T, a.D, IO::VEC, BWD_L<IO>);
-  a.cols = p.cols, a.chunks = p.chunks, a.per = p.per;
-  TTSX_ARG(p.chunks == 1 || (a.pairs && ws_bytes >= sizeof(float) * 2 * B * p.chunks * a.D),
-           "ttsx_gated_scan_backward: workspace too small");
-  const int64_t grid = (int64_t)B * p.cols * p.chunks;
-  TTSX_ARG(grid <= 0x7fffffff, "ttsx_gated_scan_backward: too many channels");
-  if (p.chunks > 1) {
-    scan_backward_kernel<IO, BWD_L<IO>, true><<<(unsigned)grid, WAVES * 64, 0, s>>>(a);
-    TTSX_LAUNCH_CHECK();
-  }
-  scan_backward_kernel<IO, BWD_L<IO>, false><<<(unsigned)grid, WAVES * 64, 0, s>>>(a);
+size_t workspace(int B, int T, int D, int backward) {
+  if (!wide<IO>(D)) return pairs_bytes<Narrow<IO>>(B, T, D);
+  return backward ? pairs_bytes<WideBwd<IO>>(B, T, D) : pairs_bytes<WideFwd<IO>>(B, T, D);
+}
+
+template <class IO, int N>
+int launch_step(const void* x, int64_t x_bs, const void* g, int64_t g_bs, const float* h, int B, int D, void* y,
+                float* h_out, hipStream_t s) {
+  typedef typename IO::elem E;
+  const int64_t grid = ((int64_t)B * (D / N) + 255) / 256;
+  TTSX_ARG(grid <= 0x7fffffff, "ttsx_gated_step: too many channels");
+  step_kernel<IO, N><<<(unsigned)grid, 256, 0, s>>>(static_cast<const E*>(x), x_bs, static_cast<const E*>(g), g_bs, h, B,
+                                                    D, static_cast<E*>(y), h_out);
   TTSX_LAUNCH_CHECK();
   return TTSX_OK;
 }
-
 template <class IO>
 int run_step(const void* x, int64_t x_bs, const void* g, int64_t g_bs, const float* h, int B, int D, void* y,
              float* h_out, hipStream_t s) {
-  typedef typename IO::elem E;
-  const int64_t grid = ((int64_t)B * ceil_div(D, IO::VEC) + 255) / 256;
-  TTSX_ARG(grid <= 0x7fffffff, "ttsx_gated_step: too many channels");
-  step_kernel<IO><<<(unsigned)grid, 256, 0, s>>>(static_cast<const E*>(x), x_bs, static_cast<const E*>(g), g_bs, h, B, D,
-                                                 static_cast<E*>(y), h_out);
-  TTSX_LAUNCH_CHECK();
-  return TTSX_OK;
+  return D % 4 == 0 ? launch_step<IO, 4>(x, x_bs, g, g_bs, h, B, D, y, h_out, s)
+                    : launch_step<IO, 1>(x, x_bs, g, g_bs, h, B, D, y, h_out, s);
 }
 
-bool shape_ok(int B, int T, int D) { return B >= 1 && T >= 1 && D >= 1 && T <= (1 << 30) && D <= (1 << 24); }
+bool shape_ok(int B, int T, int D) { return B >= 1 && T >= 1 && D >= 1 && T <= (1 << 30) && D <= (1 << 20); }
 bool dtype_ok(int d) { return d == TTSX_F32 || d == TTSX_BF16 || d == TTSX_F16; }
-
-size_t pairs_bytes(int B, int T, int D, int dtype, int lf, int lh) {
-  const bool wide = dtype == TTSX_F32;
-  const Plan p = plan(B, T, D, wide ? 4 : 8, wide ? lf : lh);
-  return p.chunks == 1 ? 0 : sizeof(float) * 2 * (size_t)B * p.chunks * D;
-}
 
 }  // namespace
 
 extern "C" long ttsx_gated_scan_workspace(int B, int T, int D, int dtype, int backward) {
   TTSX_ARG(shape_ok(B, T, D) && dtype_ok(dtype), "ttsx_gated_scan_workspace: bad shape or type");
-  return (long)(backward ? pairs_bytes(B, T, D, dtype, BWD_L<IoF32>, BWD_L<IoBf16>)
-                         : pairs_bytes(B, T, D, dtype, FWD_L<IoF32>, FWD_L<IoBf16>));
+  return (long)(dtype == TTSX_F32    ? workspace<IoF32>(B, T, D, backward)
+                : dtype == TTSX_BF16 ? workspace<IoBf16>(B, T, D, backward)
+                                     : workspace<IoF16>(B, T, D, backward));
 }
 
 extern "C" int ttsx_gated_scan(const void* x, int64_t x_batch_stride, int64_t x_row_stride, const void* g,
@@ -527,15 +625,17 @@ extern "C" int ttsx_gated_scan(const void* x, int64_t x_batch_stride, int64_t x_
   TTSX_ARG(x && g && h && h_last, "ttsx_gated_scan: null argument");
   TTSX_ARG(shape_ok(B, T, D), "ttsx_gated_scan: bad shape B=%d T=%d D=%d", B, T, D);
   TTSX_ARG(dtype_ok(dtype), "ttsx_gated_scan: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
+  TTSX_ARG(stride_ok(x_row_stride) && stride_ok(g_row_stride), "ttsx_gated_scan: a row stride outside 0..%ld",
+           (long)MAX_STRIDE);
   ScanArgs a{};
-  a.x = x, a.x_bs = x_batch_stride, a.x_ts = x_row_stride;
-  a.g = g, a.g_bs = g_batch_stride, a.g_ts = g_row_stride;
+  a.x = x, a.x_bs = x_batch_stride;
+  a.g = g, a.g_bs = g_batch_stride;
   a.h0 = h0, a.lengths = lengths, a.T = T, a.D = D, a.reverse = reverse != 0;
   a.h = h, a.h_last = h_last, a.states = states, a.pairs = static_cast<float*>(workspace);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == TTSX_F32    ? run_scan<IoF32>(a, B, workspace_bytes, s)
-         : dtype == TTSX_BF16 ? run_scan<IoBf16>(a, B, workspace_bytes, s)
-                              : run_scan<IoF16>(a, B, workspace_bytes, s);
+  return dtype == TTSX_F32    ? run_scan<IoF32>(a, x_row_stride, g_row_stride, 0, B, workspace_bytes, false, s)
+         : dtype == TTSX_BF16 ? run_scan<IoBf16>(a, x_row_stride, g_row_stride, 0, B, workspace_bytes, false, s)
+                              : run_scan<IoF16>(a, x_row_stride, g_row_stride, 0, B, workspace_bytes, false, s);
 }
 
 extern "C" int ttsx_gated_scan_backward(const void* dh, int64_t dh_batch_stride, int64_t dh_row_stride, const void* x,
@@ -547,16 +647,18 @@ extern "C" int ttsx_gated_scan_backward(const void* dh, int64_t dh_batch_stride,
   TTSX_ARG(dh && x && g && states && dx && dg && dh0, "ttsx_gated_scan_backward: null argument");
   TTSX_ARG(shape_ok(B, T, D), "ttsx_gated_scan_backward: bad shape B=%d T=%d D=%d", B, T, D);
   TTSX_ARG(dtype_ok(dtype), "ttsx_gated_scan_backward: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
+  TTSX_ARG(stride_ok(dh_row_stride) && stride_ok(x_row_stride) && stride_ok(g_row_stride),
+           "ttsx_gated_scan_backward: a row stride outside 0..%ld", (long)MAX_STRIDE);
   ScanArgs a{};
-  a.dh = dh, a.dh_bs = dh_batch_stride, a.dh_ts = dh_row_stride;
-  a.x = x, a.x_bs = x_batch_stride, a.x_ts = x_row_stride;
-  a.g = g, a.g_bs = g_batch_stride, a.g_ts = g_row_stride;
+  a.dh = dh, a.dh_bs = dh_batch_stride;
+  a.x = x, a.x_bs = x_batch_stride;
+  a.g = g, a.g_bs = g_batch_stride;
   a.states_in = states, a.dh_last = dh_last, a.lengths = lengths, a.T = T, a.D = D, a.reverse = reverse != 0;
   a.dx = dx, a.dg = dg, a.dh0 = dh0, a.pairs = static_cast<float*>(workspace);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == TTSX_F32    ? run_backward<IoF32>(a, B, workspace_bytes, s)
-         : dtype == TTSX_BF16 ? run_backward<IoBf16>(a, B, workspace_bytes, s)
-                              : run_backward<IoF16>(a, B, workspace_bytes, s);
+  return dtype == TTSX_F32    ? run_scan<IoF32>(a, x_row_stride, g_row_stride, dh_row_stride, B, workspace_bytes, true, s)
+         : dtype == TTSX_BF16 ? run_scan<IoBf16>(a, x_row_stride, g_row_stride, dh_row_stride, B, workspace_bytes, true, s)
+                              : run_scan<IoF16>(a, x_row_stride, g_row_stride, dh_row_stride, B, workspace_bytes, true, s);
 }
 
 extern "C" int ttsx_gated_step(const void* x, int64_t x_batch_stride, const void* g, int64_t g_batch_stride,

@@ -1,117 +1,163 @@
 // Element types of the sequence operators (ttsx_seq.h): 32-bit floats and the two 16-bit kinds, read and written 16
 // bytes per lane.  Everything between a load and a store is fp32.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef u32x4 u32x4_any __attribute__((aligned(2)));  // rows of odd strides: global memory takes any element address
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
+// PER: elements of a 32-bit word; INF: a word of +infinity; VEC: elements of 16 bytes.
 struct IoF32 {
   typedef float elem;
-  static constexpr int VEC = 4;
-  static constexpr uint32_t INF2 = 0x7f800000u;  // one register of +infinity
-  __device__ static inline void unpack(u32x4 r, float* v) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
-  }
-  __device__ static inline u32x4 pack(const float* v) {
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(v[i]);
-    return r;
-  }
+  static constexpr int PER = 1, VEC = 4;
+  static constexpr uint32_t INF = 0x7f800000u;
+  __device__ static inline void unpack(uint32_t w, float* v) { v[0] = __uint_as_float(w); }
+  __device__ static inline uint32_t pack(const float* v) { return __float_as_uint(v[0]); }
 };
 
 struct IoBf16 {
   typedef __bf16 elem;
-  static constexpr int VEC = 8;
-  static constexpr uint32_t INF2 = 0x7f807f80u;
-  __device__ static inline void unpack(u32x4 r, float* v) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(r[i] << 16);
-      v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
-    }
+  static constexpr int PER = 2, VEC = 8;
+  static constexpr uint32_t INF = 0x7f807f80u;
+  __device__ static inline void unpack(uint32_t w, float* v) {
+    v[0] = __uint_as_float(w << 16);
+    v[1] = __uint_as_float(w & 0xffff0000u);
   }
-  __device__ static inline u32x4 pack(const float* v) {  // to nearest, ties to even
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){v[2 * i], v[2 * i + 1]}, bf16x2));
-    return r;
+  __device__ static inline uint32_t pack(const float* v) {  // to nearest, ties to even
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){v[0], v[1]}, bf16x2));
   }
 };
 
 struct IoF16 {
   typedef _Float16 elem;
-  static constexpr int VEC = 8;
-  static constexpr uint32_t INF2 = 0x7c007c00u;
-  __device__ static inline void unpack(u32x4 r, float* v) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = r[i];  // a value of its own: the cast of a vector's element takes the wrong one
-      const f16x2 h = __builtin_bit_cast(f16x2, w);
-      v[2 * i] = (float)h[0];
-      v[2 * i + 1] = (float)h[1];
-    }
+  static constexpr int PER = 2, VEC = 8;
+  static constexpr uint32_t INF = 0x7c007c00u;
+  __device__ static inline void unpack(uint32_t w, float* v) {
+    const f16x2 h = __builtin_bit_cast(f16x2, w);
+    v[0] = (float)h[0];
+    v[1] = (float)h[1];
   }
-  __device__ static inline u32x4 pack(const float* v) {  // to nearest, ties to even
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float a = v[2 * i], b = v[2 * i + 1];
-      asm("" : "+v"(a), "+v"(b));  // the fp32 value is rounded, as everywhere: no fma straight into 16 bits
-      const f16x2 h = {(_Float16)a, (_Float16)b};
-      r[i] = __builtin_bit_cast(uint32_t, h);
-    }
-    return r;
+  __device__ static inline uint32_t pack(const float* v) {  // to nearest, ties to even
+    float a = v[0], b = v[1];
+    asm("" : "+v"(a), "+v"(b));  // the fp32 value is rounded, as everywhere: no fma straight into 16 bits
+    const f16x2 h = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, h);
   }
 };
 
-template <class IO>
-__device__ static inline u32x4 load16(const typename IO::elem* p) {
-  return *reinterpret_cast<const u32x4_any*>(p);
-}
-template <class IO>
-__device__ static inline void store16(typename IO::elem* p, u32x4 r) {
-  *reinterpret_cast<u32x4_any*>(p) = r;
-}
-
-// The first n (0..VEC) elements at p, the rest zero; a full vector is one load.
-template <class IO>
-__device__ static inline u32x4 load_some(const typename IO::elem* p, int n) {
-  if (n >= IO::VEC) return load16<IO>(p);
-  float v[IO::VEC];
+// N elements as a lane holds them (8 or 16 bytes).  Rows of odd strides: global memory takes any element address.
+template <class IO, int N>
+struct Lane {
+  static constexpr int W = N / IO::PER;
+  typedef uint32_t raw __attribute__((ext_vector_type(W)));
+  typedef raw raw_any __attribute__((aligned(2)));
+  typedef typename IO::elem E;
+  __device__ static inline raw fill(uint32_t w) {
+    raw r;
 #pragma unroll
-  for (int i = 0; i < IO::VEC; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
-  return IO::pack(v);
-}
+    for (int i = 0; i < W; ++i) r[i] = w;
+    return r;
+  }
+  __device__ static inline void unpack(raw r, float* v) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) IO::unpack(r[i], v + i * IO::PER);
+  }
+  __device__ static inline raw pack(const float* v) {
+    raw r;
+#pragma unroll
+    for (int i = 0; i < W; ++i) r[i] = IO::pack(v + i * IO::PER);
+    return r;
+  }
+  __device__ static inline raw load(const E* p) { return *reinterpret_cast<const raw_any*>(p); }
+  __device__ static inline void store(E* p, raw r) { *reinterpret_cast<raw_any*>(p) = r; }
+  // the first n (0..N) elements at p, the rest zero; a full vector is one load
+  __device__ static inline raw load_some(const E* p, int n) {
+    if (n >= N) return load(p);
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
+    return pack(v);
+  }
+  __device__ static inline void store_some(E* p, raw r, int n) {
+    if (n >= N) {
+      store(p, r);
+      return;
+    }
+    float v[N];
+    unpack(r, v);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) p[i] = (E)v[i];
+  }
+};
+
+// One element per lane.
 template <class IO>
-__device__ static inline void store_some(typename IO::elem* p, u32x4 r, int n) {
-  if (n >= IO::VEC) {
-    store16<IO>(p, r);
+struct Lane<IO, 1> {
+  static constexpr int W = 1;
+  typedef uint32_t raw;
+  typedef typename IO::elem E;
+  __device__ static inline raw fill(uint32_t w) { return w; }
+  __device__ static inline void unpack(raw r, float* v) {
+    float t[IO::PER];
+    IO::unpack(r, t);
+    v[0] = t[0];
+  }
+  __device__ static inline raw pack(const float* v) {
+    float t[IO::PER] = {};
+    t[0] = v[0];
+    return IO::pack(t);
+  }
+  __device__ static inline raw load(const E* p) {
+    if constexpr (IO::PER == 1)
+      return *reinterpret_cast<const uint32_t*>(p);
+    else
+      return *reinterpret_cast<const uint16_t*>(p);
+  }
+  __device__ static inline void store(E* p, raw r) {
+    if constexpr (IO::PER == 1)
+      *reinterpret_cast<uint32_t*>(p) = r;
+    else
+      *reinterpret_cast<uint16_t*>(p) = (uint16_t)r;
+  }
+};
+
+// N consecutive fp32 values (states).
+template <int N>
+__device__ static inline void load_f32(const float* p, float* v) {
+  typedef float vec __attribute__((ext_vector_type(N == 1 ? 2 : N), aligned(4)));
+  if constexpr (N == 1) {
+    v[0] = *p;
+  } else {
+    const vec r = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = r[i];
+  }
+}
+template <int N>
+__device__ static inline void store_f32(float* p, const float* v) {
+  typedef float vec __attribute__((ext_vector_type(N == 1 ? 2 : N), aligned(4)));
+  if constexpr (N == 1) {
+    *p = v[0];
+  } else {
+    vec r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = v[i];
+    *reinterpret_cast<vec*>(p) = r;
+  }
+}
+template <int N>
+__device__ static inline void store_f32_some(float* p, int n, const float* v) {
+  if (n >= N) {
+    store_f32<N>(p, v);
     return;
   }
-  float v[IO::VEC];
-  IO::unpack(r, v);
 #pragma unroll
-  for (int i = 0; i < IO::VEC; ++i)
-    if (i < n) p[i] = (typename IO::elem)v[i];
-}
-
-// VEC consecutive fp32 values (states) of which n exist.
-template <int VEC>
-__device__ static inline void load_f32(const float* p, int n, float* v) {
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) v[i] = i < n ? p[i] : 0.0f;
-}
-template <int VEC>
-__device__ static inline void store_f32(float* p, int n, const float* v) {
-#pragma unroll
-  for (int i = 0; i < VEC; ++i)
+  for (int i = 0; i < N; ++i)
     if (i < n) p[i] = v[i];
 }
 

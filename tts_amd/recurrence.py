@@ -22,9 +22,10 @@ import functools
 import torch
 
 from . import _lib
-from ._seq import DTYPES, are_tensors, lengths_on, no_graph, on_device, overlaps, rows, same_place
+from ._seq import DTYPES, are_tensors, call, lengths_on, on_device, overlaps, pointer, rows, same_place
 
-STATE_BLOCK = 64   # steps between two kept states (TTSX_STATE_BLOCK)
+STATE_BLOCK = 64             # steps between two kept states (TTSX_STATE_BLOCK)
+MAX_CHANNELS = FURTHEST = 1 << 20   # channels, and elements between two rows, of a call
 
 
 @functools.lru_cache(maxsize=512)
@@ -36,18 +37,20 @@ def _workspace_bytes(B, T, D, dtype, backward):
 
 
 def _values_and_gates(what, x, g, axes):
-    are_tensors(what, x=x, g=g)
+    are_tensors(what, ("x", x), ("g", g))
     if x.dim() != len(axes) or g.shape != x.shape:
         raise ValueError("%s: x and g must both be [%s], got %s and %s"
                          % (what, ", ".join(axes), tuple(x.shape), tuple(g.shape)))
     if x.dtype not in DTYPES or g.dtype != x.dtype:
         raise ValueError("%s: x and g must both be float32, bfloat16 or float16, got %s and %s" % (what, x.dtype, g.dtype))
+    if x.shape[-1] > MAX_CHANNELS:
+        raise ValueError("%s: at most %d channels, got %d" % (what, MAX_CHANNELS, x.shape[-1]))
 
 
 def _state(what, name, t, B, D):
     if t is None:
         return None
-    are_tensors(what, **{name: t})
+    are_tensors(what, (name, t))
     if t.shape != (B, D) or t.dtype != torch.float32:
         raise ValueError("%s: %s must be float32 [%d, %d], got %s %s" % (what, name, B, D, t.dtype, tuple(t.shape)))
     return t.contiguous()
@@ -61,29 +64,27 @@ def gated_scan(x, g, h0=None, lengths=None, reverse=False, save_states=False):
     x's type and the float32 state behind the last step; with `save_states` also the float32 states [B,ceil(T/64),D] in
     front of every 64th step, which `gated_scan_backward` starts from.
 
-    x and g may be slices of one projection (any strides; the last axis is copied if it is not contiguous)."""
+    x and g may be slices of one projection (any strides; the last axis is copied if it is not contiguous, and all of
+    it if its rows lie more than 2^20 elements apart)."""
     what = "gated_scan"
     _values_and_gates(what, x, g, "BTD")
     B, T, D = x.shape
     h0 = _state(what, "h0", h0, B, D)
-    no_graph(what, x, g, h0)
-    on_device(what, x=x, g=g, h0=h0)
-    x, g, dev = rows(x), rows(g), x.device
-    h = torch.empty(B, T, D, dtype=x.dtype, device=dev)
-    states = torch.empty(B, -(-T // STATE_BLOCK), D, dtype=torch.float32, device=dev) if save_states else None
+    dev = on_device(what, ("x", x), ("g", g), ("h0", h0))
+    lengths = lengths_on(what, lengths, B, T, dev)
+    x, g = rows(x, FURTHEST), rows(g, FURTHEST)
+    h = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+    states = torch.empty((B, -(-T // STATE_BLOCK), D), dtype=torch.float32, device=dev) if save_states else None
     if B == 0 or T == 0 or D == 0:
         h_last = torch.zeros(B, D, device=dev) if h0 is None else h0.clone()
         return (h, h_last, states) if save_states else (h, h_last)
-    h_last = torch.empty(B, D, dtype=torch.float32, device=dev)
+    h_last = torch.empty((B, D), dtype=torch.float32, device=dev)
     dtype = DTYPES[x.dtype]
     need = _workspace_bytes(B, T, D, dtype, 0)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with torch.cuda.device(dev):
-        lengths = lengths_on(what, lengths, B, T, dev)
-        _lib.check(_lib.load().ttsx_gated_scan(
-            x.data_ptr(), x.stride(0), x.stride(1), g.data_ptr(), g.stride(0), g.stride(1), _lib.ptr(h0), _lib.ptr(lengths),
-            B, T, D, dtype, 1 if reverse else 0, h.data_ptr(), h_last.data_ptr(), _lib.ptr(states), _lib.ptr(ws), need,
-            _lib.current_stream()), "ttsx_gated_scan")
+    xs, gs = x.stride(), g.stride()
+    call("ttsx_gated_scan", dev, x.data_ptr(), xs[0], xs[1], g.data_ptr(), gs[0], gs[1], pointer(h0), pointer(lengths),
+         B, T, D, dtype, 1 if reverse else 0, h.data_ptr(), h_last.data_ptr(), pointer(states), pointer(ws), need)
     return (h, h_last, states) if save_states else (h, h_last)
 
 
@@ -94,7 +95,7 @@ def gated_scan_backward(dh, x, g, states, dh_last=None, lengths=None, reverse=Fa
     dh0."""
     what = "gated_scan_backward"
     _values_and_gates(what, x, g, "BTD")
-    are_tensors(what, dh=dh, states=states)
+    are_tensors(what, ("dh", dh), ("states", states))
     B, T, D = x.shape
     if dh.shape != x.shape or dh.dtype != x.dtype:
         raise ValueError("%s: dh must be %s %s like x, got %s %s" % (what, x.dtype, tuple(x.shape), dh.dtype, tuple(dh.shape)))
@@ -103,24 +104,21 @@ def gated_scan_backward(dh, x, g, states, dh_last=None, lengths=None, reverse=Fa
         raise ValueError("%s: states must be float32 [%d, %d, %d] as gated_scan(save_states=True) returns them, got %s %s"
                          % (what, B, blocks, D, states.dtype, tuple(states.shape)))
     dh_last = _state(what, "dh_last", dh_last, B, D)
-    no_graph(what, dh, x, g, states, dh_last)
-    on_device(what, x=x, g=g, dh=dh, states=states, dh_last=dh_last)
-    dh, x, g, states, dev = rows(dh), rows(x), rows(g), states.contiguous(), x.device
-    dx = torch.empty(B, T, D, dtype=x.dtype, device=dev)
-    dg = torch.empty(B, T, D, dtype=x.dtype, device=dev)
+    dev = on_device(what, ("x", x), ("g", g), ("dh", dh), ("states", states), ("dh_last", dh_last))
+    lengths = lengths_on(what, lengths, B, T, dev)
+    dh, x, g, states = rows(dh, FURTHEST), rows(x, FURTHEST), rows(g, FURTHEST), states.contiguous()
+    dx = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+    dg = torch.empty((B, T, D), dtype=x.dtype, device=dev)
     if B == 0 or T == 0 or D == 0:
         return dx, dg, torch.zeros(B, D, device=dev) if dh_last is None else dh_last.clone()
-    dh0 = torch.empty(B, D, dtype=torch.float32, device=dev)
+    dh0 = torch.empty((B, D), dtype=torch.float32, device=dev)
     dtype = DTYPES[x.dtype]
     need = _workspace_bytes(B, T, D, dtype, 1)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with torch.cuda.device(dev):
-        lengths = lengths_on(what, lengths, B, T, dev)
-        _lib.check(_lib.load().ttsx_gated_scan_backward(
-            dh.data_ptr(), dh.stride(0), dh.stride(1), x.data_ptr(), x.stride(0), x.stride(1), g.data_ptr(), g.stride(0),
-            g.stride(1), states.data_ptr(), _lib.ptr(dh_last), _lib.ptr(lengths), B, T, D, dtype, 1 if reverse else 0,
-            dx.data_ptr(), dg.data_ptr(), dh0.data_ptr(), _lib.ptr(ws), need, _lib.current_stream()),
-            "ttsx_gated_scan_backward")
+    xs, gs, ds = x.stride(), g.stride(), dh.stride()
+    call("ttsx_gated_scan_backward", dev, dh.data_ptr(), ds[0], ds[1], x.data_ptr(), xs[0], xs[1], g.data_ptr(), gs[0],
+         gs[1], states.data_ptr(), pointer(dh_last), pointer(lengths), B, T, D, dtype, 1 if reverse else 0,
+         dx.data_ptr(), dg.data_ptr(), dh0.data_ptr(), pointer(ws), need)
     return dx, dg, dh0
 
 
@@ -130,28 +128,24 @@ def gated_step(x, g, h, out=None):
     state in place."""
     what = "gated_step"
     _values_and_gates(what, x, g, "BD")
-    are_tensors(what, h=h)
+    are_tensors(what, ("h", h))
     B, D = x.shape
     state = _state(what, "h", h, B, D)
     if out is not None:
-        are_tensors(what, out=out)
-    no_graph(what, x, g, h, out)
-    on_device(what, x=x, g=g, h=h, out=out)
-    if out is not None:
+        are_tensors(what, ("out", out))
+    dev = on_device(what, ("x", x), ("g", g), ("h", h), ("out", out))
+    if out is None:
+        out = torch.empty((B, D), dtype=torch.float32, device=dev)
+    else:
         if out.shape != (B, D) or out.dtype != torch.float32 or not out.is_contiguous():
             raise ValueError("%s: out must be contiguous float32 [%d, %d], got %s %s"
                              % (what, B, D, out.dtype, tuple(out.shape)))
         for name, t in (("x", x), ("g", g), ("h", h)):
-            if overlaps(t, out) and not (name == "h" and same_place(t, out)):
+            if overlaps(t, out) and not (t is h and same_place(h, out)):
                 raise ValueError("%s: out overlaps %s" % (what, name))
-    x, g, h = rows(x), rows(g), state
-    y = torch.empty(B, D, dtype=x.dtype, device=x.device)
-    if out is None:
-        out = torch.empty(B, D, dtype=torch.float32, device=x.device)
-    if B == 0 or D == 0:
-        return y, out
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().ttsx_gated_step(x.data_ptr(), x.stride(0), g.data_ptr(), g.stride(0), h.data_ptr(), B, D,
-                                               DTYPES[x.dtype], y.data_ptr(), out.data_ptr(), _lib.current_stream()),
-                   "ttsx_gated_step")
+    x, g = rows(x), rows(g)
+    y = torch.empty((B, D), dtype=x.dtype, device=dev)
+    if B and D:
+        call("ttsx_gated_step", dev, x.data_ptr(), x.stride(0), g.data_ptr(), g.stride(0), state.data_ptr(), B, D,
+             DTYPES[x.dtype], y.data_ptr(), out.data_ptr())
     return y, out
