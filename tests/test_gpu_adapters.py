@@ -68,6 +68,20 @@ def test_add_matches_the_formula(size, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("size", [(260, 130, 24, 40, 5, 7), (200, 190, 72, 136, 20, 3), (150, 250, 40, 65, 40, 11)], ids=str)
+def test_many_requests(size, dtype):
+    """Batches that fill the chip take their rows in larger tiles."""
+    from tts_amd.adapters import adapter_add
+    y, x, down, up, voices, scale, lengths = _inputs(*size, dtype, 7)
+    want, tol = adapter(y, x, down, up, voices, scale, lengths)
+    gy, gx, gd, gu, gv, gs, gl = _cuda(y, x, down, up, voices, scale, lengths)
+    out = adapter_add(gy, gx, gd, gu, gv, scale=gs, lengths=gl)
+    assert _excess(out, want, tol * (1 + half_step(dtype)) + _rounding(dtype, want)) <= 0
+    assert torch.equal(adapter_add(gy, gx, gd, gu, gv, scale=gs, lengths=gl, out=gy), out)
+    _check_backward(size, dtype, 8)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_single_positions(dtype):
     """[B,N] and [B,K] are the [B,1,.] call."""
     from tts_amd.adapters import adapter_add

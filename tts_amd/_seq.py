@@ -86,16 +86,19 @@ def lengths_on(what, lengths, B, T, device):
 
 
 def _span(t):
+    last = 1
+    for n, stride in zip(t.shape, t.stride()):
+        if n == 0:
+            return None
+        last += (n - 1) * stride
     first = t.data_ptr()
-    return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+    return first, first + last * t.element_size()
 
 
 def overlaps(a, b):
     """Whether the two tensors' memory ranges meet (strided tensors may interleave and still count)."""
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
+    a, b = _span(a), _span(b)
+    return a is not None and b is not None and a[0] < b[1] and b[0] < a[1]
 
 
 def same_place(a, b):

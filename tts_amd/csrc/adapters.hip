@@ -28,8 +28,10 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 template <class IO>
 using Full = Lane<IO, IO::VEC>;  // 16 bytes of a lane
 
-constexpr int ROWS = 32;  // rows of a tile: two matrix fragments
 constexpr int WAVES = 4;
+#ifndef MF4_TILES
+#define MF4_TILES 1000000000
+#endif
 
 struct AddArgs {
   const void *x, *y, *down, *up;
@@ -37,7 +39,7 @@ struct AddArgs {
   int64_t x_bs, x_ts, y_bs, y_ts, o_bs, o_ts;
   const int32_t *voices, *lengths;
   const float* scale;
-  float* keep;  // [B][RP][keep_pitch]: s u by rank, for the weights' gradients
+  float* keep;  // [B][RP][keep_pitch]: s u by rank, for the weights' gradients (keep_hidden)
   int T, K, N, R, V, tiles, splits, in_place, keep_pitch;
 };
 
@@ -81,27 +83,67 @@ __device__ static inline int voice_of(const int32_t* voices, int b, int V) {
 }
 
 // u of a tile, as the matrix operand of the second product: [ROWS][RP] fp32, or two 16-bit planes and a factor per row.
-template <class IO, int RP>
+template <class IO, int RP, int ROWS>
 struct Hidden {
   typedef typename IO::elem E;
   E hi[ROWS][RP + 8], lo[ROWS][RP + 8];
   float factor[ROWS];
 };
-template <int RP>
-struct Hidden<IoF32, RP> {
+template <int RP, int ROWS>
+struct Hidden<IoF32, RP, ROWS> {
   float u[ROWS][RP + 4];
 };
 
+// Rank of a lane's i-th row of B: 16-bit types take 8 ranks at a time (up to rank 16 the upper half of the lanes has
+// them again, for the second part of u), fp32 a quarter of them.
+template <class IO, int RP>
+__device__ static inline int rank_of(int q, int i) {
+  if (IO::VEC == 4) return q * (RP / 4) + i;
+  return RP == 16 ? 8 * (q & 1) + i : i / 8 * 32 + 8 * q + i % 8;
+}
+
+// u for the weights' gradients, where it is contracted over rows: by rank, 8 consecutive rows to a lane.  bf16 takes it
+// as two parts, written as two planes; fp16 has no range for that (a factor per row would not come out of the sum) and
+// multiplies in fp32 there.
+template <class IO>
+constexpr bool SPLIT_HIDDEN = IO::INF == IoBf16::INF;
+template <class IO, int RP>
+__device__ static inline void keep_hidden(float* keep, int64_t b, int pitch, int row, int c0, const float* u) {
+#pragma unroll
+  for (int c = 0; c < RP / 8; ++c) {
+    const int64_t at = (b * RP + c0 + c) * pitch;
+    if constexpr (SPLIT_HIDDEN<IO>) {
+      typename IO::elem* plane = reinterpret_cast<typename IO::elem*>(keep + at);
+      two_parts<IO>(u[c], plane[row], plane[pitch + row]);
+    } else {
+      keep[at + row] = u[c];
+    }
+  }
+}
+template <class IO, int RP>
+__device__ static inline void hidden_rows(const float* keep, int64_t b, int pitch, int rank, int row, u32x4* r) {
+  const float* at = keep + (b * RP + rank) * pitch;
+  if constexpr (SPLIT_HIDDEN<IO>) {
+    const typename IO::elem* plane = reinterpret_cast<const typename IO::elem*>(at);
+    r[0] = *reinterpret_cast<const u32x4*>(plane + row);
+    r[1] = *reinterpret_cast<const u32x4*>(plane + pitch + row);
+  } else {
+    r[0] = *reinterpret_cast<const u32x4*>(at + row);
+    r[1] = *reinterpret_cast<const u32x4*>(at + row + 4);
+  }
+}
+
 // ADD: out = y + z, else out = z.  EXPAND: the second product too.
-template <class IO, int RP, bool ADD, bool EXPAND>
-__global__ __launch_bounds__(WAVES * 64) void adapter_kernel(AddArgs a) {
-  constexpr int VEC = IO::VEC, NJ = RP / 16, KSTEP = VEC * 4, CB = 16 * VEC;
+template <class IO, int RP, int MF, bool ADD, bool EXPAND>
+__global__ __launch_bounds__(WAVES * 64, RP == 64 ? 2 : 3) void adapter_kernel(AddArgs a) {
+  constexpr int VEC = IO::VEC, NJ = RP / 16, KSTEP = VEC * 4, CB = 16 * VEC, ROWS = 16 * MF, U = MF + NJ <= 4 ? 4 : 2;
   constexpr bool WIDE = VEC == 4;
   typedef typename IO::elem E;
+  typedef Full<IO> Io;
   __shared__ float part[WAVES][ROWS][RP + 1];
-  __shared__ Hidden<IO, RP> hid;
+  __shared__ Hidden<IO, RP, ROWS> hid;
   const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits % a.tiles, b = blockIdx.x / a.splits / a.tiles;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
   const int row0 = tile * ROWS, rows = min(ROWS, a.T - row0);
   const int len = valid_rows(a.lengths, b, a.T), v = voice_of(a.voices, b, a.V);
   const int live = min(rows, len - row0);  // rows of the tile that count (may be negative)
@@ -111,68 +153,105 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_kernel(AddArgs a) {
 
   if (v < 0 || live <= 0) {
     if (!EXPAND || (ADD && a.in_place)) return;
-    for (int cb = split * WAVES + wave; cb < blocks; cb += a.splits * WAVES) {
-      const int c = cb * CB + l16 * VEC, n = min(max(a.N - c, 0), VEC);
-      if (n == 0) continue;
-      for (int r = q; r < rows; r += 4)
-        Full<IO>::store_some(ob + r * a.o_ts + c, ADD ? Full<IO>::load_some(yb + r * a.y_ts + c, n) : (u32x4){0, 0, 0, 0}, n);
+    // a row per wave, 64 lanes across
+    for (int r = split * WAVES + wave; r < rows; r += a.splits * WAVES) {
+      const E* from = yb + r * a.y_ts;
+      E* to = ob + r * a.o_ts;
+      constexpr int SPAN = 64 * VEC;
+      int c = lane * VEC;
+      for (; c + 3 * SPAN + VEC <= a.N; c += 4 * SPAN) {
+        u32x4 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = ADD ? Io::load(from + c + i * SPAN) : Io::fill(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) Io::store(to + c + i * SPAN, w[i]);
+      }
+      for (; c + VEC <= a.N; c += SPAN) Io::store(to + c, ADD ? Io::load(from + c) : Io::fill(0));
+      for (; c < a.N; ++c) to[c] = ADD ? from[c] : (E)0.0f;  // the one lane whose columns the row ends in
     }
     return;
   }
 
-  // u = x A^T: lane group q holds VEC consecutive k of a row, the same of x and of A
-  const E* xb = static_cast<const E*>(a.x) + b * a.x_bs + row0 * a.x_ts;
-  const E* A = static_cast<const E*>(a.down) + (int64_t)v * a.R * a.K;
-  f32x4 acc[2][NJ];
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[m][j] = (f32x4){0, 0, 0, 0};
-  for (int k0 = wave * KSTEP; k0 < a.K; k0 += WAVES * KSTEP) {
-    const int k = k0 + q * VEC, n = min(max(a.K - k, 0), VEC);
-    u32x4 xr[2], ar[NJ];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const int r = 16 * m + l16;
-      xr[m] = r < live && n > 0 ? Full<IO>::load_some(xb + r * a.x_ts + k, n) : (u32x4){0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int r = 16 * j + l16;
-      ar[j] = r < a.R && n > 0 ? Full<IO>::load_some(A + (int64_t)r * a.K + k, n) : (u32x4){0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[m][j] = mma<IO>(xr[m], ar[j], acc[m][j]);
-  }
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) part[wave][16 * m + 4 * q + i][16 * j + l16] = acc[m][j][i];
-  __syncthreads();
+  // u = x A^T: lane group q holds VEC consecutive k of a row, the same of x and of A; rows and ranks that do not exist
+  // repeat the last one and are dropped below
   {
+    const E* xb = static_cast<const E*>(a.x) + b * a.x_bs + row0 * a.x_ts;
+    const E* A = static_cast<const E*>(a.down) + (int64_t)v * a.R * a.K;
+    f32x4 acc[MF][NJ];
+    const E *xp[MF], *ap[NJ];
+#pragma unroll
+    for (int m = 0; m < MF; ++m) xp[m] = xb + min(16 * m + l16, live - 1) * a.x_ts;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) ap[j] = A + (int64_t)min(16 * j + l16, a.R - 1) * a.K;
+#pragma unroll
+    for (int m = 0; m < MF; ++m)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[m][j] = (f32x4){0, 0, 0, 0};
+    const int whole = a.K / KSTEP;
+    int step = wave;
+    for (; step + (U - 1) * WAVES < whole; step += U * WAVES) {
+      u32x4 xr[U][MF], ar[U][NJ];
+      const int k = step * KSTEP + q * VEC;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int m = 0; m < MF; ++m) xr[u][m] = Io::load(xp[m] + k + u * WAVES * KSTEP);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) ar[u][j] = Io::load(ap[j] + k + u * WAVES * KSTEP);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int m = 0; m < MF; ++m)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[m][j] = mma<IO>(xr[u][m], ar[u][j], acc[m][j]);
+    }
+    for (; step * KSTEP < a.K; step += WAVES) {
+      u32x4 xr[MF], ar[NJ];
+      const int k = step * KSTEP + q * VEC;
+      if (step < whole) {
+#pragma unroll
+        for (int m = 0; m < MF; ++m) xr[m] = Io::load(xp[m] + k);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) ar[j] = Io::load(ap[j] + k);
+      } else {
+#pragma unroll
+        for (int m = 0; m < MF; ++m) xr[m] = Io::load_end(xp[m], k, a.K);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) ar[j] = Io::load_end(ap[j], k, a.K);
+      }
+#pragma unroll
+      for (int m = 0; m < MF; ++m)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[m][j] = mma<IO>(xr[m], ar[j], acc[m][j]);
+    }
+#pragma unroll
+    for (int m = 0; m < MF; ++m)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[wave][16 * m + 4 * q + i][16 * j + l16] = acc[m][j][i];
+  }
+  __syncthreads();
+  const float s = a.scale ? a.scale[v] : 1.0f;
+#pragma unroll
+  for (int g = 0; g < ROWS && threadIdx.x < 256; g += 32) {
     // 8 threads to a row
-    const int r = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (RP / 8);
-    const float s = a.scale ? a.scale[v] : 1.0f;
+    const int r = g + (threadIdx.x >> 3), c0 = (threadIdx.x & 7) * (RP / 8);
     float u[RP / 8], top = 0.0f;
 #pragma unroll
     for (int c = 0; c < RP / 8; ++c) {
       u[c] = 0.0f;
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) u[c] += part[w][r][c0 + c];
-      u[c] *= s;
+      u[c] = r < live && c0 + c < a.R ? u[c] * s : 0.0f;
       top = fmaxf(top, fabsf(u[c]));
-      if (a.keep && split == 0) a.keep[((int64_t)b * RP + c0 + c) * a.keep_pitch + row0 + r] = u[c];
     }
-    if constexpr (!EXPAND) {
-      return;
-    } else if constexpr (WIDE) {
+    if (a.keep && split == 0 && row0 + r < a.keep_pitch) keep_hidden<IO, RP>(a.keep, (int64_t)b, a.keep_pitch, row0 + r, c0, u);
+    if constexpr (EXPAND && WIDE) {
 #pragma unroll
       for (int c = 0; c < RP / 8; ++c) hid.u[r][c0 + c] = u[c];
-    } else {
+    } else if constexpr (EXPAND) {
       float up = 1.0f;
       if constexpr (IO::INF == IoF16::INF) {
         // the row's largest magnitude to [2^13, 2^14): both parts and their products stay inside fp16 and fp32
@@ -190,93 +269,126 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_kernel(AddArgs a) {
       for (int c = 0; c < RP / 8; ++c) two_parts<IO>(u[c] * up, hid.hi[r][c0 + c], hid.lo[r][c0 + c]);
     }
   }
-  __syncthreads();
 
   if constexpr (EXPAND) {
+    __syncthreads();
     const E* Bm = static_cast<const E*>(a.up) + (int64_t)v * a.R * a.N;
     constexpr int KB = WIDE ? 1 : (RP + 31) / 32;  // blocks of 32 ranks
-    for (int cb = split * WAVES + wave; cb < blocks; cb += a.splits * WAVES) {
-      const int c = cb * CB + l16 * VEC, n = min(max(a.N - c, 0), VEC);
-      u32x4 bt[WIDE ? RP / 4 : KB * 8];
+    constexpr int NB = WIDE ? RP / 4 : KB * 8;     // ranks of a lane
+    // A piece is 16 rows of a column block.  The waves take neighbouring blocks at a time, since rows that are no
+    // multiple of 128 bytes share a line at every border and the line should be whole when it leaves the L2; the blocks
+    // that are left over are dealt out piece by piece.  A wave reads its next piece's y and B while it multiplies.
+    const int pieces = ceil_div(rows, 16), lanes = a.splits * WAVES, me = split * WAVES + wave;
+    const int rounds = blocks / lanes, left = blocks - rounds * lanes;
+    const bool dealt = left * pieces <= lanes;
+    const int all = rounds * pieces + (dealt ? (me < left * pieces ? 1 : 0) : me < left ? pieces : 0);
+    const auto block_of = [&](int k) {
+      return k < rounds * pieces ? k / pieces * lanes + me : rounds * lanes + (dealt ? me / pieces : me);
+    };
+    const auto piece_of = [&](int k) { return k >= rounds * pieces && dealt ? me % pieces : k % pieces; };
+    const auto fetch_b = [&](int cb, u32x4* br) {
+      const int c = cb * CB + l16 * VEC;
+      if (cb * CB + CB <= a.N) {  // the same for the wave
+#pragma unroll
+        for (int i = 0; i < NB; ++i) br[i] = Io::load(Bm + (int64_t)min(rank_of<IO, RP>(q, i), a.R - 1) * a.N + c);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+          br[i] = Io::load_end(Bm + (int64_t)min(rank_of<IO, RP>(q, i), a.R - 1) * a.N, c, a.N);
+      }
+    };
+    const auto fetch_y = [&](int cb, int m, u32x4* yr) {
+      const int c = cb * CB + l16 * VEC;
+      if (cb * CB + CB <= a.N) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) yr[i] = Io::load(yb + min(16 * m + 4 * q + i, rows - 1) * a.y_ts + c);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) yr[i] = Io::load_end(yb + min(16 * m + 4 * q + i, rows - 1) * a.y_ts, c, a.N);
+      }
+    };
+    u32x4 br[NB], bn[NB], yr[4], yn[4];
+    if (all > 0) {
+      fetch_b(block_of(0), bn);
+      if constexpr (ADD) fetch_y(block_of(0), piece_of(0), yn);
+    }
+    int held = -1;
+    for (int k = 0; k < all; ++k) {
+      const int cb = block_of(k), m = piece_of(k);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) yr[i] = ADD ? yn[i] : Io::fill(0);
+      if (cb != held) {
+        held = cb;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) br[i] = rank_of<IO, RP>(q, i) < a.R ? bn[i] : Io::fill(0);
+        if constexpr (!WIDE) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            u32x4 t[8];
+            transpose8(br + 8 * kb, t);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) br[8 * kb + i] = t[i];
+          }
+        }
+      }
+      if (k + 1 < all) {
+        if (block_of(k + 1) != cb) fetch_b(block_of(k + 1), bn);
+        if constexpr (ADD) fetch_y(block_of(k + 1), piece_of(k + 1), yn);
+      }
+      f32x4 z[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) z[j] = (f32x4){0, 0, 0, 0};
+      const int r = 16 * m + l16;
       if constexpr (WIDE) {
 #pragma unroll
         for (int s = 0; s < RP / 4; ++s) {
-          const int r = q * (RP / 4) + s;
-          bt[s] = r < a.R && n > 0 ? Full<IO>::load_some(Bm + (int64_t)r * a.N + c, n) : (u32x4){0, 0, 0, 0};
+          const float u = hid.u[r][q * (RP / 4) + s];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            z[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(u, __uint_as_float(br[s][j]), z[j], 0, 0, 0);
         }
+      } else if constexpr (RP == 16) {
+        const E* src = q < 2 ? &hid.hi[r][8 * q] : &hid.lo[r][8 * (q - 2)];
+        const u32x4 u = *reinterpret_cast<const u32x4*>(src);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) z[j] = mma<IO>(u, br[j], z[j]);
       } else {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-          u32x4 br[8];
+          const u32x4 uh = *reinterpret_cast<const u32x4*>(&hid.hi[r][32 * kb + 8 * q]);
+          const u32x4 ul = *reinterpret_cast<const u32x4*>(&hid.lo[r][32 * kb + 8 * q]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = RP == 16 ? 8 * (q & 1) + i : kb * 32 + 8 * q + i;
-            br[i] = r < a.R && n > 0 ? Full<IO>::load_some(Bm + (int64_t)r * a.N + c, n) : (u32x4){0, 0, 0, 0};
+          for (int j = 0; j < VEC; ++j) {
+            z[j] = mma<IO>(ul, br[8 * kb + j], z[j]);
+            z[j] = mma<IO>(uh, br[8 * kb + j], z[j]);
           }
-          transpose8(br, bt + 8 * kb);
         }
       }
+      const int c = cb * CB + l16 * VEC, n = min(max(a.N - c, 0), VEC);
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        if (16 * m >= rows) break;
-        f32x4 z[VEC];
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * m + 4 * q + i;
+        float o[VEC];
+        u32x4 w = yr[i];
+        Io::unpack(w, o);
+        float f = 1.0f;
+        if constexpr (!WIDE && IO::INF == IoF16::INF) f = hid.factor[row];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) z[j] = (f32x4){0, 0, 0, 0};
-        const int r = 16 * m + l16;
-        if constexpr (WIDE) {
-#pragma unroll
-          for (int s = 0; s < RP / 4; ++s) {
-            const float u = hid.u[r][q * (RP / 4) + s];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              z[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(u, __uint_as_float(bt[s][j]), z[j], 0, 0, 0);
-          }
-        } else if constexpr (RP == 16) {
-          const E* src = q < 2 ? &hid.hi[r][8 * q] : &hid.lo[r][8 * (q - 2)];
-          const u32x4 u = *reinterpret_cast<const u32x4*>(src);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) z[j] = mma<IO>(u, bt[j], z[j]);
-        } else {
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
-            const u32x4 uh = *reinterpret_cast<const u32x4*>(&hid.hi[r][32 * kb + 8 * q]);
-            const u32x4 ul = *reinterpret_cast<const u32x4*>(&hid.lo[r][32 * kb + 8 * q]);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              z[j] = mma<IO>(ul, bt[8 * kb + j], z[j]);
-              z[j] = mma<IO>(uh, bt[8 * kb + j], z[j]);
-            }
-          }
-        }
-        if (n == 0) continue;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = 16 * m + 4 * q + i;
-          if (row >= rows || (ADD && a.in_place && row >= live)) continue;
-          float o[VEC];
-          u32x4 yr = (u32x4){0, 0, 0, 0};
-          if constexpr (ADD) yr = Full<IO>::load_some(yb + row * a.y_ts + c, n);
-          if (row < live) {
-            Full<IO>::unpack(yr, o);
-            float k = 1.0f;
-            if constexpr (!WIDE && IO::INF == IoF16::INF) k = hid.factor[row];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) o[j] = fmaf(k, z[j][i], o[j]);
-            yr = Full<IO>::pack(o);
-          }
-          Full<IO>::store_some(ob + row * a.o_ts + c, yr, n);
-        }
+        for (int j = 0; j < VEC; ++j) o[j] = fmaf(f, z[j][i], o[j]);
+        if (row < live) w = Io::pack(o);
+        if (row < rows && !(ADD && a.in_place && row >= live)) Io::store_some(ob + row * a.o_ts + c, w, n);
       }
     }
   }
 }
 
 // Weights' gradients, one request (and slice of its rows) at a time: part[b][chunk][rank][column] = sum of u x over
-// the slice's rows, the columns of x (from du) first, those of dy (from u) behind them.  A wave owns 16 VEC columns.
+// the slice's rows, the columns of x (from du) first, those of dy (from u) behind them.  A wave owns 16 VEC columns
+// and reads 8 rows of each lane's VEC columns at once, the next ones while it multiplies.
 struct OuterArgs {
   const void *x, *dy;
   int64_t x_bs, x_ts, dy_bs, dy_ts;
-  const float *du, *u;  // [B][RP][pitch]
+  const float *du, *u;  // as keep_hidden left them
   const int32_t *voices, *lengths;
   float* part;
   int T, K, N, V, chunks, span, pitch, groups;
@@ -285,10 +397,10 @@ struct OuterArgs {
 template <class IO, int RP>
 __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
   constexpr int VEC = IO::VEC, NJ = RP / 16, CB = 16 * VEC;
-  constexpr bool SPLIT = IO::INF == IoBf16::INF;  // the others multiply in fp32: fp16 has no range for u
   typedef typename IO::elem E;
+  typedef Full<IO> Io;
   const int group = blockIdx.x % a.groups, chunk = blockIdx.x / a.groups % a.chunks, b = blockIdx.x / a.groups / a.chunks;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
   const int kblocks = ceil_div(a.K, CB), nblocks = ceil_div(a.N, CB);
   int cb = group * WAVES + wave;
   if (cb >= kblocks + nblocks) return;
@@ -299,54 +411,63 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
   if (!of_x) cb -= kblocks;
   const int width = of_x ? a.K : a.N;
   const int c = cb * CB + l16 * VEC, n = min(max(width - c, 0), VEC);
+  const bool whole = cb * CB + CB <= width;
   const int64_t ts = of_x ? a.x_ts : a.dy_ts;
-  const E* src = (of_x ? static_cast<const E*>(a.x) + b * a.x_bs : static_cast<const E*>(a.dy) + b * a.dy_bs) + c;
-  const float* ub = (of_x ? a.du : a.u) + (int64_t)b * RP * a.pitch;
+  const E* src = of_x ? static_cast<const E*>(a.x) + b * a.x_bs : static_cast<const E*>(a.dy) + b * a.dy_bs;
+  const float* ub = of_x ? a.du : a.u;
   f32x4 acc[NJ][VEC];
 #pragma unroll
   for (int j = 0; j < NJ; ++j)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[j][i] = (f32x4){0, 0, 0, 0};
-  for (int r0 = first; r0 < last; r0 += 32) {
-    u32x4 xr[8];
+  // rows first + r0 .. + 31, this lane the 8 from 8 q on; rows behind the last are zero (and so is their u)
+  const auto fetch = [&](int r0, u32x4* xr, u32x4 (*ur)[2]) {
+    if (whole) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = r0 + 8 * q + i;
-      xr[i] = r < last && n > 0 ? Full<IO>::load_some(src + r * ts, n) : (u32x4){0, 0, 0, 0};
+      for (int i = 0; i < 8; ++i) xr[i] = Io::load(src + min(r0 + 8 * q + i, last - 1) * ts + c);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) xr[i] = Io::load_end(src + min(r0 + 8 * q + i, last - 1) * ts, c, width);
     }
-    u32x4 bt[8];
-    if constexpr (SPLIT) transpose8(xr, bt);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      // rows behind the last one were kept as zeros up to the end of their tile of 32
-      const float4* up = reinterpret_cast<const float4*>(ub + (int64_t)(16 * j + l16) * a.pitch + r0 + 8 * q);
-      const float4 u0 = up[0], u1 = up[1];
-      const float u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
-      if constexpr (SPLIT) {
-        float h[8], l[8];
+    for (int j = 0; j < NJ; ++j) hidden_rows<IO, RP>(ub, (int64_t)b, a.pitch, 16 * j + l16, r0 + 8 * q, ur[j]);
+  };
+  u32x4 xr[8], ur[NJ][2];
+  fetch(first, xr, ur);
+  for (int r0 = first; r0 < last; r0 += 32) {
+    u32x4 xn[8], un[NJ][2];
+    if (r0 + 32 < last) fetch(r0 + 32, xn, un);
+    if (r0 + 32 > last) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          E hi, lo;
-          two_parts<IO>(u[i], hi, lo);
-          h[i] = (float)hi, l[i] = (float)lo;
-        }
-        const u32x4 uh = Full<IO>::pack(h), ul = Full<IO>::pack(l);
+      for (int i = 0; i < 8; ++i)
+        if (r0 + 8 * q + i >= last) xr[i] = Io::fill(0);
+    }
+    if constexpr (SPLIT_HIDDEN<IO>) {
+      u32x4 bt[8];
+      transpose8(xr, bt);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          acc[j][i] = mma<IO>(ul, bt[i], acc[j][i]);
-          acc[j][i] = mma<IO>(uh, bt[i], acc[j][i]);
+          acc[j][i] = mma<IO>(ur[j][1], bt[i], acc[j][i]);
+          acc[j][i] = mma<IO>(ur[j][0], bt[i], acc[j][i]);
         }
-      } else {
+    } else {
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          float xv[VEC];
-          Full<IO>::unpack(xr[s], xv);
+      for (int s = 0; s < 8; ++s) {
+        float xv[VEC];
+        Io::unpack(xr[s], xv);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
           for (int i = 0; i < VEC; ++i)
-            acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(u[s], xv[i], acc[j][i], 0, 0, 0);
-        }
+            acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ur[j][s / 4][s % 4]), xv[i], acc[j][i], 0, 0, 0);
       }
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) xr[i] = xn[i];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) ur[j][0] = un[j][0], ur[j][1] = un[j][1];
   }
   const int total = a.K + a.N;
   float* out = a.part + (int64_t)(b * a.chunks + chunk) * RP * total + (of_x ? 0 : a.K) + c;
@@ -361,26 +482,48 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
     }
 }
 
-// Sum over the requests of a voice, in their order.
+// Sum over the requests of a voice, in their order.  A thread takes one column; the requests of the voice are listed
+// first, so that the loads of several are in flight.
 struct GatherArgs {
   const float* part;
   const int32_t *voices, *lengths;
   void *ddown, *dup;
   int B, T, K, N, R, RP, chunks, span;
 };
+constexpr int LISTED = 256;  // threads of the gather: one looks at one slice
 template <class IO>
-__global__ __launch_bounds__(256) void gather_kernel(GatherArgs a) {
+__global__ __launch_bounds__(LISTED) void gather_kernel(GatherArgs a) {
   typedef typename IO::elem E;
-  const int total = a.K + a.N, cols = ceil_div(total, 256);
-  const int col = blockIdx.x % cols * 256 + threadIdx.x, r = blockIdx.x / cols % a.R, v = blockIdx.x / cols / a.R;
-  if (col >= total) return;
+  __shared__ int slices[LISTED], count[LISTED / 64];
+  const int total = a.K + a.N, cols = ceil_div(total, LISTED);
+  const int col = blockIdx.x % cols * LISTED + threadIdx.x, r = blockIdx.x / cols % a.R, v = blockIdx.x / cols / a.R;
+  const int64_t pitch = (int64_t)a.RP * total;
+  const float* p = a.part + (int64_t)r * total + min(col, total - 1);
   float s = 0.0f;
-  for (int b = 0; b < a.B; ++b) {
-    if (a.voices[b] != v) continue;
-    const int used = ceil_div(valid_rows(a.lengths, b, a.T), a.span);
-    const float* p = a.part + ((int64_t)b * a.chunks * a.RP + r) * total + col;
-    for (int k = 0; k < used; ++k) s += p[(int64_t)k * a.RP * total];
+  for (int from = 0; from < a.B * a.chunks; from += LISTED) {
+    // in order: a thread's slice goes where the slices in front of it leave off
+    const int k = from + threadIdx.x, b = k / a.chunks;
+    const bool mine = k < a.B * a.chunks && a.voices[b] == v && k % a.chunks * a.span < valid_rows(a.lengths, b, a.T);
+    const uint64_t wave = __ballot(mine);
+    if ((threadIdx.x & 63) == 0) count[threadIdx.x >> 6] = __popcll(wave);
+    __syncthreads();
+    int at = __popcll(wave & ((1ull << (threadIdx.x & 63)) - 1)), all = 0;
+    for (int w = 0; w < LISTED / 64; ++w) {
+      if (w < (int)(threadIdx.x >> 6)) at += count[w];
+      all += count[w];
+    }
+    if (mine) slices[at] = k;
+    __syncthreads();
+    int i = 0;
+    for (; i + 4 <= all; i += 4) {
+      const float t0 = p[slices[i] * pitch], t1 = p[slices[i + 1] * pitch], t2 = p[slices[i + 2] * pitch],
+                  t3 = p[slices[i + 3] * pitch];
+      s = (((s + t0) + t1) + t2) + t3;
+    }
+    for (; i < all; ++i) s += p[slices[i] * pitch];
+    __syncthreads();
   }
+  if (col >= total) return;
   if (col < a.K)
     static_cast<E*>(a.ddown)[((int64_t)v * a.R + r) * a.K + col] = (E)s;
   else
@@ -397,15 +540,21 @@ int column_splits(int64_t tiles, int N, int vec) {
   return (int)(want < most ? want : most);
 }
 
-template <class IO, int RP, bool ADD, bool EXPAND>
-int launch_tile(AddArgs a, int B, hipStream_t s) {
-  a.tiles = ceil_div(a.T, ROWS);
+template <class IO, int RP, int MF, bool ADD, bool EXPAND>
+int launch_tile_of(AddArgs a, int B, hipStream_t s) {
+  a.tiles = ceil_div(a.T, 16 * MF);
   const int64_t tiles = (int64_t)B * a.tiles;
   a.splits = EXPAND ? column_splits(tiles, a.N, IO::VEC) : 1;
   TTSX_ARG(tiles * a.splits <= 0x7fffffff, "ttsx_adapter: too many rows");
-  adapter_kernel<IO, RP, ADD, EXPAND><<<(unsigned)(tiles * a.splits), WAVES * 64, 0, s>>>(a);
+  adapter_kernel<IO, RP, MF, ADD, EXPAND><<<(unsigned)(tiles * a.splits), WAVES * 64, 0, s>>>(a);
   TTSX_LAUNCH_CHECK();
   return TTSX_OK;
+}
+template <class IO, int RP, bool ADD, bool EXPAND>
+int launch_tile(const AddArgs& a, int B, hipStream_t s) {
+  const int64_t large = (int64_t)B * ceil_div(a.T, 64);
+  if (large >= MF4_TILES) return launch_tile_of<IO, RP, 4, ADD, EXPAND>(a, B, s);
+  return launch_tile_of<IO, RP, 2, ADD, EXPAND>(a, B, s);
 }
 
 template <class IO>
@@ -425,10 +574,10 @@ struct BackPlan {
 BackPlan back_plan(int B, int T, int K, int N, int R, int vec) {
   BackPlan p;
   p.RP = padded_rank(R);
-  p.pitch = round_up(T, ROWS);
+  p.pitch = round_up(T, 32);
   const int64_t waves = (int64_t)B * (ceil_div(K, 16 * vec) + ceil_div(N, 16 * vec));
   const int want = waves >= 2048 ? 1 : (int)((2048 + waves - 1) / waves), most = ceil_div(T, 64);
-  p.span = round_up(ceil_div(T, want < most ? want : most), ROWS);
+  p.span = round_up(ceil_div(T, want < most ? want : most), 32);
   p.chunks = ceil_div(T, p.span);
   p.hidden = (size_t)B * p.RP * p.pitch;
   p.part = (size_t)B * p.chunks * p.RP * ((size_t)K + N);
@@ -463,9 +612,9 @@ int run_backward(const AddArgs& dx, const BackPlan& p, int B, float* ws, void* d
   GatherArgs g{};
   g.part = part, g.voices = dx.voices, g.lengths = dx.lengths, g.ddown = ddown, g.dup = dup;
   g.B = B, g.T = dx.T, g.K = o.K, g.N = o.N, g.R = dx.R, g.RP = RP, g.chunks = p.chunks, g.span = p.span;
-  const int64_t outs = (int64_t)dx.V * dx.R * ceil_div(o.K + o.N, 256);
+  const int64_t outs = (int64_t)dx.V * dx.R * ceil_div(o.K + o.N, LISTED);
   TTSX_ARG(outs <= 0x7fffffff, "ttsx_adapter_backward: too many voices");
-  gather_kernel<IO><<<(unsigned)outs, 256, 0, s>>>(g);
+  gather_kernel<IO><<<(unsigned)outs, LISTED, 0, s>>>(g);
   TTSX_LAUNCH_CHECK();
   return TTSX_OK;
 }

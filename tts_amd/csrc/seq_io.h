@@ -82,6 +82,19 @@ struct Lane {
     for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
     return pack(v);
   }
+  // Elements c..c+N-1 of a row of `width`, zero behind its end.  Nothing behind the row is read: the lane takes the last
+  // N elements of the row (or fewer, one by one, of a row that has no N) and moves them down.
+  __device__ static inline raw load_end(const E* row, int c, int width) {
+    static_assert(W == 4, "16 bytes");
+    const int n = min(max(width - c, 0), N);
+    if (width < N) return load_some(row + min(c, width - 1), n);
+    const int from = min(c, width - N), by = (c - from) * (4 / IO::PER);  // bytes
+    raw r = load(row + from);
+    if (by & 8) r = (raw){r[2], r[3], 0, 0};
+    if (by & 4) r = (raw){r[1], r[2], r[3], 0};
+    if (by & 2) r = (raw){r[0] >> 16 | r[1] << 16, r[1] >> 16 | r[2] << 16, r[2] >> 16 | r[3] << 16, r[3] >> 16};
+    return n > 0 ? r : fill(0);
+  }
   __device__ static inline void store_some(E* p, raw r, int n) {
     if (n >= N) {
       store(p, r);
