@@ -70,7 +70,8 @@ int ttsx_gated_step(const void* x, int64_t x_batch_stride, const void* g, int64_
  *   out[b,t,:] = y[b,t,:] + scale[v] (x[b,t,:] down[v]^T) up[v]        v = voices[b]
  *   y, out   [B,T,N]   out may be y itself (in place), and overlaps no other argument
  *   x        [B,T,K]
- *   down     [V,R,K], up [V,R,N], contiguous, of x's type; 1 <= R <= TTSX_ADAPTER_MAX_RANK
+ *   down     [V,R,K], up [V,R,N], contiguous, of x's type; 1 <= R <= TTSX_ADAPTER_MAX_RANK; K, N and the row strides
+ *            up to 2^20
  *   voices   [B] int32; a voice outside 0..V-1 has no adapter
  *   scale    [V] fp32 or NULL (= 1)
  * Rows without an adapter (no voice, or at positions >= length) are y's.  x down^T and the sum are fp32; out is

@@ -23,7 +23,8 @@ from . import _lib
 from ._seq import (DTYPES, are_tensors, call, columns_apart, lengths_on, on_device, overlaps, pointer, rows, same_place,
                    writable_rows)
 
-MAX_RANK = 64   # TTSX_ADAPTER_MAX_RANK
+MAX_RANK = 64                     # TTSX_ADAPTER_MAX_RANK
+MAX_WIDTH = FURTHEST = 1 << 20   # columns, and elements between two rows, of a call
 
 
 @functools.lru_cache(maxsize=512)
@@ -46,6 +47,8 @@ def _check(what, name, wide, x, down, up, scale):
     if down.dim() != 3 or up.dim() != 3 or down.shape[:2] != up.shape[:2] or down.shape[2] != K or up.shape[2] != N:
         raise ValueError("%s: down and up must be [V,R,%d] and [V,R,%d], got %s and %s"
                          % (what, K, N, tuple(down.shape), tuple(up.shape)))
+    if max(K, N) > MAX_WIDTH:
+        raise ValueError("%s: at most %d columns, got %d and %d" % (what, MAX_WIDTH, K, N))
     V, R = down.shape[:2]
     if not 1 <= R <= MAX_RANK or V < 1:
         raise ValueError("%s: the rank must lie in 1..%d, with at least one voice, got down %s"
@@ -117,8 +120,8 @@ def adapter_add(y, x, down, up, voices, scale=None, lengths=None, out=None):
                 into.copy_(y)
         else:
             if not in_place:
-                y = rows(y)
-            x = rows(x)
+                y = rows(y, FURTHEST)
+            x = rows(x, FURTHEST)
             scale = None if scale is None else scale.contiguous()
             ys, xs, os = y.stride(), x.stride(), into.stride()
             call("ttsx_adapter_add", dev, y.data_ptr(), ys[0], ys[1], x.data_ptr(), xs[0], xs[1], down.data_ptr(),
@@ -149,7 +152,7 @@ def adapter_backward(dy, x, down, up, voices, scale=None, lengths=None):
     dtype = DTYPES[x.dtype]
     need = _workspace_bytes(B, T, K, N, R, dtype)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    dy, x = rows(dy), rows(x)
+    dy, x = rows(dy, FURTHEST), rows(x, FURTHEST)
     scale = None if scale is None else scale.contiguous()
     ds, xs = dy.stride(), x.stride()
     call("ttsx_adapter_backward", dev, dy.data_ptr(), ds[0], ds[1], x.data_ptr(), xs[0], xs[1], down.data_ptr(),

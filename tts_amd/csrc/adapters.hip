@@ -28,19 +28,25 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 template <class IO>
 using Full = Lane<IO, IO::VEC>;  // 16 bytes of a lane
 
-constexpr int WAVES = 4;
-#ifndef MF4_TILES
-#define MF4_TILES 1000000000
-#endif
+constexpr int ROWS = 32;  // rows of a tile: two matrix fragments
 
+// A first product: x [.,K] of a request's rows with the voice's matrix m [R,K].
+struct Product {
+  const void *x, *m;
+  int64_t bs;  // stride of the batch in elements
+  uint32_t ts;  // of the rows, in bytes
+  int K;
+  float* keep;  // [B][tiles][RP][ROWS]: s u for the weights' gradients (keep_hidden)
+};
 struct AddArgs {
-  const void *x, *y, *down, *up;
+  Product first, second;  // the second one is only kept
+  const void *y, *up;
   void* out;
-  int64_t x_bs, x_ts, y_bs, y_ts, o_bs, o_ts;
+  int64_t y_bs, o_bs;
+  uint32_t y_ts, o_ts;
   const int32_t *voices, *lengths;
   const float* scale;
-  float* keep;  // [B][RP][keep_pitch]: s u by rank, for the weights' gradients (keep_hidden)
-  int T, K, N, R, V, tiles, splits, in_place, keep_pitch;
+  int T, N, R, V, tiles, splits, in_place;
 };
 
 template <class IO>
@@ -83,14 +89,14 @@ __device__ static inline int voice_of(const int32_t* voices, int b, int V) {
 }
 
 // u of a tile, as the matrix operand of the second product: [ROWS][RP] fp32, or two 16-bit planes and a factor per row.
-template <class IO, int RP, int ROWS>
+template <class IO, int RP>
 struct Hidden {
   typedef typename IO::elem E;
   E hi[ROWS][RP + 8], lo[ROWS][RP + 8];
   float factor[ROWS];
 };
-template <int RP, int ROWS>
-struct Hidden<IoF32, RP, ROWS> {
+template <int RP>
+struct Hidden<IoF32, RP> {
   float u[ROWS][RP + 4];
 };
 
@@ -102,61 +108,178 @@ __device__ static inline int rank_of(int q, int i) {
   return RP == 16 ? 8 * (q & 1) + i : i / 8 * 32 + 8 * q + i % 8;
 }
 
-// u for the weights' gradients, where it is contracted over rows: by rank, 8 consecutive rows to a lane.  bf16 takes it
-// as two parts, written as two planes; fp16 has no range for that (a factor per row would not come out of the sum) and
-// multiplies in fp32 there.
+// u for the weights' gradients, where it is contracted over rows: per tile of 32 rows and 16 ranks two times 1 KB in the
+// order of the matrix operand, lane 16 q + rank with rows 8 q .. 8 q + 7.  bf16 takes it as two parts, one KB each; fp16
+// has no range for that (a factor per row would not come out of the sum) and multiplies in fp32, rows 8 q .. + 3 in the
+// first KB and the other four in the second.
 template <class IO>
 constexpr bool SPLIT_HIDDEN = IO::INF == IoBf16::INF;
 template <class IO, int RP>
-__device__ static inline void keep_hidden(float* keep, int64_t b, int pitch, int row, int c0, const float* u) {
+__device__ static inline void keep_hidden(float* keep, int64_t tile, int row, int c0, const float* u) {
 #pragma unroll
   for (int c = 0; c < RP / 8; ++c) {
-    const int64_t at = (b * RP + c0 + c) * pitch;
+    const int rank = c0 + c, lane = 16 * (row >> 3) + (rank & 15);
+    float* at = keep + (tile * (RP / 16) + (rank >> 4)) * 512;
     if constexpr (SPLIT_HIDDEN<IO>) {
-      typename IO::elem* plane = reinterpret_cast<typename IO::elem*>(keep + at);
-      two_parts<IO>(u[c], plane[row], plane[pitch + row]);
+      typename IO::elem* e = reinterpret_cast<typename IO::elem*>(at) + lane * 8 + (row & 7);
+      two_parts<IO>(u[c], e[0], e[512]);
     } else {
-      keep[at + row] = u[c];
+      at[(row >> 2 & 1) * 256 + lane * 4 + (row & 3)] = u[c];
     }
   }
 }
-template <class IO, int RP>
-__device__ static inline void hidden_rows(const float* keep, int64_t b, int pitch, int rank, int row, u32x4* r) {
-  const float* at = keep + (b * RP + rank) * pitch;
-  if constexpr (SPLIT_HIDDEN<IO>) {
-    const typename IO::elem* plane = reinterpret_cast<const typename IO::elem*>(at);
-    r[0] = *reinterpret_cast<const u32x4*>(plane + row);
-    r[1] = *reinterpret_cast<const u32x4*>(plane + pitch + row);
-  } else {
-    r[0] = *reinterpret_cast<const u32x4*>(at + row);
-    r[1] = *reinterpret_cast<const u32x4*>(at + row + 4);
+template <int RP>
+__device__ static inline void hidden_rows(const float* keep, int64_t tile, int j, int lane, u32x4* r) {
+  const u32x4* at = reinterpret_cast<const u32x4*>(keep + (tile * (RP / 16) + j) * 512) + lane;
+  r[0] = at[0];
+  r[1] = at[64];
+}
+
+// A scalar base and a lane's offset in bytes.
+template <class T>
+__device__ static inline T* shifted(T* base, uint32_t bytes) {
+  typedef typename std::conditional<std::is_const<T>::value, const char, char>::type C;
+  return reinterpret_cast<T*>(reinterpret_cast<C*>(base) + bytes);
+}
+
+// A lane number the compiler takes for a new one: what follows from it is computed again instead of being held in
+// registers around a loop, which the operands need.
+__device__ static inline int anew(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+template <class T>
+__device__ static inline T* row_at(T* base, int64_t row, uint32_t stride) {
+  typedef typename std::conditional<std::is_const<T>::value, const char, char>::type C;
+  return reinterpret_cast<T*>(reinterpret_cast<C*>(base) + row * stride);
+}
+
+// Four registers of four neighbouring lanes, transposed: register j of lane i becomes register i of lane j.
+__device__ static inline void quad_transpose(u32x4* r, int lane) {
+  const bool odd = lane & 1, high = lane & 2;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t v[4] = {r[0][w], r[1][w], r[2][w], r[3][w]};
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {  // lanes 1 apart: quad_perm 1,0,3,2
+      const uint32_t a = __builtin_amdgcn_mov_dpp(v[j], 0xb1, 0xf, 0xf, true);
+      const uint32_t b = __builtin_amdgcn_mov_dpp(v[j + 1], 0xb1, 0xf, 0xf, true);
+      v[j] = odd ? b : v[j];
+      v[j + 1] = odd ? v[j + 1] : a;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {  // lanes 2 apart: quad_perm 2,3,0,1
+      const uint32_t a = __builtin_amdgcn_mov_dpp(v[j], 0x4e, 0xf, 0xf, true);
+      const uint32_t b = __builtin_amdgcn_mov_dpp(v[j + 2], 0x4e, 0xf, 0xf, true);
+      v[j] = high ? b : v[j];
+      v[j + 2] = high ? v[j + 2] : a;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j][w] = v[j];
   }
 }
 
-// ADD: out = y + z, else out = z.  EXPAND: the second product too.
-template <class IO, int RP, int MF, bool ADD, bool EXPAND>
-__global__ __launch_bounds__(WAVES * 64, RP == 64 ? 2 : 3) void adapter_kernel(AddArgs a) {
-  constexpr int VEC = IO::VEC, NJ = RP / 16, KSTEP = VEC * 4, CB = 16 * VEC, ROWS = 16 * MF, U = MF + NJ <= 4 ? 4 : 2;
+// The waves' shares of u = x A^T, 256 bytes of every row at a time.  A matrix operand wants 16 rows in 16 neighbouring
+// lanes, which as a load is 64 separate accesses (the first form of this kernel was bound by them: 50 cache accesses to
+// an instruction).  So four loads bring four rows each, 16 neighbouring lanes to a row, and the lanes' quads are
+// transposed: lane 16 q + r then holds chunks 4 q .. 4 q + 3 of 16 bytes of row r, one per register, the same of x and of
+// A.  Rows and ranks that do not exist repeat the last one and are dropped in the sum.
+template <class IO, int RP, int WV>
+__device__ static inline void first_product(const Product& p, const typename IO::elem* xb, int v, int R, int live, int wave,
+                                            int lane, float (*part)[ROWS][RP + 1]) {
+  constexpr int VEC = IO::VEC, NJ = RP / 16, STEP = VEC * 16, MF = ROWS / 16;
+  typedef typename IO::elem E;
+  typedef Full<IO> Io;
+  const E* A = static_cast<const E*>(p.m) + (int64_t)v * R * p.K;
+  f32x4 acc[MF][NJ];
+#pragma unroll
+  for (int m = 0; m < MF; ++m)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[m][j] = (f32x4){0, 0, 0, 0};
+  for (int k0 = wave * STEP; k0 < p.K; k0 += WV * STEP) {
+    u32x4 xr[MF][4], ar[NJ][4];
+    const uint32_t pitch = p.K * sizeof(E);
+    const int l = anew(lane), row = l >> 2 & 3, k = ((l >> 4) * 4 + (l & 3)) * VEC;  // of load j: row 4 row + j
+    if (k0 + STEP <= p.K) {  // the same for the wave
+#pragma unroll
+      for (int m = 0; m < MF; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          xr[m][j] = Io::load(shifted(xb + k0, min(16 * m + 4 * row + j, live - 1) * p.ts + (uint32_t)(k * sizeof(E))));
+#pragma unroll
+      for (int n = 0; n < NJ; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          ar[n][j] = Io::load(shifted(A + k0, min(16 * n + 4 * row + j, R - 1) * pitch + (uint32_t)(k * sizeof(E))));
+    } else {
+#pragma unroll
+      for (int m = 0; m < MF; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          xr[m][j] = Io::load_end(shifted(xb, min(16 * m + 4 * row + j, live - 1) * p.ts), k0 + k, p.K);
+#pragma unroll
+      for (int n = 0; n < NJ; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          ar[n][j] = Io::load_end(shifted(A, min(16 * n + 4 * row + j, R - 1) * pitch), k0 + k, p.K);
+    }
+#pragma unroll
+    for (int m = 0; m < MF; ++m) quad_transpose(xr[m], lane);
+#pragma unroll
+    for (int n = 0; n < NJ; ++n) {
+      quad_transpose(ar[n], lane);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int m = 0; m < MF; ++m) acc[m][n] = mma<IO>(xr[m][j], ar[n][j], acc[m][n]);
+    }
+  }
+  const int q = lane >> 4, l16 = lane & 15;
+#pragma unroll
+  for (int m = 0; m < MF; ++m)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[wave][16 * m + 4 * q + i][16 * j + l16] = acc[m][j][i];
+}
+
+// Ranks c0.. of row r of s u, from the waves' shares; zero where the row or the rank does not exist.
+template <int RP, int WV>
+__device__ static inline void sum_shares(float (*part)[ROWS][RP + 1], int r, int c0, int live, int R, float s, float* u) {
+#pragma unroll
+  for (int c = 0; c < RP / 8; ++c) {
+    u[c] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WV; ++w) u[c] += part[w][r][c0 + c];
+    u[c] = r < live && c0 + c < R ? u[c] * s : 0.0f;
+  }
+}
+
+// ADD: out = y + z.  Else out = z, and the hidden rows of both products are kept.
+template <class IO, int RP, int WV, bool ADD>
+__global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_kernel(AddArgs a) {
+  constexpr int VEC = IO::VEC, CB = 16 * VEC;
   constexpr bool WIDE = VEC == 4;
   typedef typename IO::elem E;
   typedef Full<IO> Io;
-  __shared__ float part[WAVES][ROWS][RP + 1];
-  __shared__ Hidden<IO, RP, ROWS> hid;
+  __shared__ float part[WV][ROWS][RP + 1];
+  __shared__ Hidden<IO, RP> hid;
   const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits % a.tiles, b = blockIdx.x / a.splits / a.tiles;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
   const int row0 = tile * ROWS, rows = min(ROWS, a.T - row0);
   const int len = valid_rows(a.lengths, b, a.T), v = voice_of(a.voices, b, a.V);
   const int live = min(rows, len - row0);  // rows of the tile that count (may be negative)
-  const E* yb = static_cast<const E*>(a.y) + b * a.y_bs + row0 * a.y_ts;
-  E* ob = static_cast<E*>(a.out) + b * a.o_bs + row0 * a.o_ts;
+  const E* yb = row_at(static_cast<const E*>(a.y) + b * a.y_bs, row0, a.y_ts);
+  E* ob = row_at(static_cast<E*>(a.out) + b * a.o_bs, row0, a.o_ts);
   const int blocks = ceil_div(a.N, CB);
 
   if (v < 0 || live <= 0) {
-    if (!EXPAND || (ADD && a.in_place)) return;
+    if (ADD && a.in_place) return;
     // a row per wave, 64 lanes across
-    for (int r = split * WAVES + wave; r < rows; r += a.splits * WAVES) {
-      const E* from = yb + r * a.y_ts;
-      E* to = ob + r * a.o_ts;
+    for (int r = split * WV + wave; r < rows; r += a.splits * WV) {
+      const E* from = shifted(yb, r * a.y_ts);
+      E* to = shifted(ob, r * a.o_ts);
       constexpr int SPAN = 64 * VEC;
       int c = lane * VEC;
       for (; c + 3 * SPAN + VEC <= a.N; c += 4 * SPAN) {
@@ -172,89 +295,83 @@ __global__ __launch_bounds__(WAVES * 64, RP == 64 ? 2 : 3) void adapter_kernel(A
     return;
   }
 
-  // u = x A^T: lane group q holds VEC consecutive k of a row, the same of x and of A; rows and ranks that do not exist
-  // repeat the last one and are dropped below
-  {
-    const E* xb = static_cast<const E*>(a.x) + b * a.x_bs + row0 * a.x_ts;
-    const E* A = static_cast<const E*>(a.down) + (int64_t)v * a.R * a.K;
-    f32x4 acc[MF][NJ];
-    const E *xp[MF], *ap[NJ];
+  // A piece is 16 rows of a column block.  The waves take neighbouring blocks at a time, since rows that are no multiple
+  // of 128 bytes share a line at every border and the line should be whole when it leaves the L2; the blocks that are
+  // left over are dealt out piece by piece.  A wave reads its next piece's y (and B, where registers allow) while it
+  // multiplies, and its first piece's y before anything else.
+  constexpr int KB = WIDE ? 1 : (RP + 31) / 32;  // blocks of 32 ranks
+  constexpr int NB = WIDE ? RP / 4 : KB * 8;     // ranks of a lane
+  constexpr bool AHEAD = WV == 4;
+  const int pieces = ceil_div(rows, 16), lanes = a.splits * WV, me = split * WV + wave;
+  const int rounds = blocks / lanes, left = blocks - rounds * lanes;
+  const bool dealt = left * pieces <= lanes;
+  const int all = rounds * pieces + (dealt ? (me < left * pieces ? 1 : 0) : me < left ? pieces : 0);
+  const auto block_of = [&](int k) {
+    return k < rounds * pieces ? k / pieces * lanes + me : rounds * lanes + (dealt ? me / pieces : me);
+  };
+  const auto piece_of = [&](int k) { return k >= rounds * pieces && dealt ? me % pieces : k % pieces; };
+  const E* Bm = static_cast<const E*>(a.up) + (int64_t)v * a.R * a.N;
+  const uint32_t b_pitch = a.N * sizeof(E);
+  const auto fetch_b = [&](int cb, u32x4* br) {
+    const int q = anew(lane >> 4), l16 = anew(lane & 15);
+    if (cb * CB + CB <= a.N) {  // the same for the wave
 #pragma unroll
-    for (int m = 0; m < MF; ++m) xp[m] = xb + min(16 * m + l16, live - 1) * a.x_ts;
+      for (int i = 0; i < NB; ++i)
+        br[i] = Io::load(shifted(Bm + cb * CB, min(rank_of<IO, RP>(q, i), a.R - 1) * b_pitch + (uint32_t)(l16 * 16)));
+    } else {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) ap[j] = A + (int64_t)min(16 * j + l16, a.R - 1) * a.K;
-#pragma unroll
-    for (int m = 0; m < MF; ++m)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[m][j] = (f32x4){0, 0, 0, 0};
-    const int whole = a.K / KSTEP;
-    int step = wave;
-    for (; step + (U - 1) * WAVES < whole; step += U * WAVES) {
-      u32x4 xr[U][MF], ar[U][NJ];
-      const int k = step * KSTEP + q * VEC;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-#pragma unroll
-        for (int m = 0; m < MF; ++m) xr[u][m] = Io::load(xp[m] + k + u * WAVES * KSTEP);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) ar[u][j] = Io::load(ap[j] + k + u * WAVES * KSTEP);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int m = 0; m < MF; ++m)
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) acc[m][j] = mma<IO>(xr[u][m], ar[u][j], acc[m][j]);
+      for (int i = 0; i < NB; ++i)
+        br[i] = Io::load_end(shifted(Bm, min(rank_of<IO, RP>(q, i), a.R - 1) * b_pitch), cb * CB + l16 * VEC, a.N);
     }
-    for (; step * KSTEP < a.K; step += WAVES) {
-      u32x4 xr[MF], ar[NJ];
-      const int k = step * KSTEP + q * VEC;
-      if (step < whole) {
+  };
+  const auto fetch_y = [&](int cb, int m, u32x4* yr) {
+    const int q = anew(lane >> 4), l16 = anew(lane & 15);
+    if (cb * CB + CB <= a.N) {
 #pragma unroll
-        for (int m = 0; m < MF; ++m) xr[m] = Io::load(xp[m] + k);
+      for (int i = 0; i < 4; ++i)
+        yr[i] = Io::load(shifted(yb + cb * CB, min(16 * m + 4 * q + i, rows - 1) * a.y_ts + (uint32_t)(l16 * 16)));
+    } else {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) ar[j] = Io::load(ap[j] + k);
-      } else {
-#pragma unroll
-        for (int m = 0; m < MF; ++m) xr[m] = Io::load_end(xp[m], k, a.K);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) ar[j] = Io::load_end(ap[j], k, a.K);
-      }
-#pragma unroll
-      for (int m = 0; m < MF; ++m)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[m][j] = mma<IO>(xr[m], ar[j], acc[m][j]);
+      for (int i = 0; i < 4; ++i)
+        yr[i] = Io::load_end(shifted(yb, min(16 * m + 4 * q + i, rows - 1) * a.y_ts), cb * CB + l16 * VEC, a.N);
     }
-#pragma unroll
-    for (int m = 0; m < MF; ++m)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part[wave][16 * m + 4 * q + i][16 * j + l16] = acc[m][j][i];
-  }
-  __syncthreads();
+  };
+  u32x4 br[NB], bn[AHEAD ? NB : 1], yr[4], yn[4];
+  if (ADD && all > 0) fetch_y(block_of(0), piece_of(0), yn);
+
   const float s = a.scale ? a.scale[v] : 1.0f;
-#pragma unroll
-  for (int g = 0; g < ROWS && threadIdx.x < 256; g += 32) {
-    // 8 threads to a row
-    const int r = g + (threadIdx.x >> 3), c0 = (threadIdx.x & 7) * (RP / 8);
-    float u[RP / 8], top = 0.0f;
-#pragma unroll
-    for (int c = 0; c < RP / 8; ++c) {
-      u[c] = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) u[c] += part[w][r][c0 + c];
-      u[c] = r < live && c0 + c < a.R ? u[c] * s : 0.0f;
-      top = fmaxf(top, fabsf(u[c]));
+  const int r = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (RP / 8);  // of the sums: 8 threads to a row
+  if constexpr (!ADD) {
+    const E* xb = row_at(static_cast<const E*>(a.second.x) + b * a.second.bs, row0, a.second.ts);
+    if (split == 0) {
+      first_product<IO, RP, WV>(a.second, xb, v, a.R, live, wave, lane, part);
+      __syncthreads();
+      if (r < ROWS) {
+        float u[RP / 8];
+        sum_shares<RP, WV>(part, r, c0, live, a.R, s, u);
+        keep_hidden<IO, RP>(a.second.keep, (int64_t)b * a.tiles + tile, r, c0, u);
+      }
+      __syncthreads();
     }
-    if (a.keep && split == 0 && row0 + r < a.keep_pitch) keep_hidden<IO, RP>(a.keep, (int64_t)b, a.keep_pitch, row0 + r, c0, u);
-    if constexpr (EXPAND && WIDE) {
+  }
+  first_product<IO, RP, WV>(a.first, row_at(static_cast<const E*>(a.first.x) + b * a.first.bs, row0, a.first.ts), v, a.R,
+                            live, wave, lane, part);
+  if (AHEAD && all > 0) fetch_b(block_of(0), bn);
+  __syncthreads();
+  if (r < ROWS) {
+    float u[RP / 8];
+    sum_shares<RP, WV>(part, r, c0, live, a.R, s, u);
+    if (!ADD && split == 0) keep_hidden<IO, RP>(a.first.keep, (int64_t)b * a.tiles + tile, r, c0, u);
+    if constexpr (WIDE) {
 #pragma unroll
       for (int c = 0; c < RP / 8; ++c) hid.u[r][c0 + c] = u[c];
-    } else if constexpr (EXPAND) {
+    } else {
       float up = 1.0f;
       if constexpr (IO::INF == IoF16::INF) {
         // the row's largest magnitude to [2^13, 2^14): both parts and their products stay inside fp16 and fp32
+        float top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < RP / 8; ++c) top = fmaxf(top, fabsf(u[c]));
         top = fmaxf(top, __shfl_xor(top, 1, 64));
         top = fmaxf(top, __shfl_xor(top, 2, 64));
         top = fmaxf(top, __shfl_xor(top, 4, 64));
@@ -269,115 +386,78 @@ __global__ __launch_bounds__(WAVES * 64, RP == 64 ? 2 : 3) void adapter_kernel(A
       for (int c = 0; c < RP / 8; ++c) two_parts<IO>(u[c] * up, hid.hi[r][c0 + c], hid.lo[r][c0 + c]);
     }
   }
+  __syncthreads();
 
-  if constexpr (EXPAND) {
-    __syncthreads();
-    const E* Bm = static_cast<const E*>(a.up) + (int64_t)v * a.R * a.N;
-    constexpr int KB = WIDE ? 1 : (RP + 31) / 32;  // blocks of 32 ranks
-    constexpr int NB = WIDE ? RP / 4 : KB * 8;     // ranks of a lane
-    // A piece is 16 rows of a column block.  The waves take neighbouring blocks at a time, since rows that are no
-    // multiple of 128 bytes share a line at every border and the line should be whole when it leaves the L2; the blocks
-    // that are left over are dealt out piece by piece.  A wave reads its next piece's y and B while it multiplies.
-    const int pieces = ceil_div(rows, 16), lanes = a.splits * WAVES, me = split * WAVES + wave;
-    const int rounds = blocks / lanes, left = blocks - rounds * lanes;
-    const bool dealt = left * pieces <= lanes;
-    const int all = rounds * pieces + (dealt ? (me < left * pieces ? 1 : 0) : me < left ? pieces : 0);
-    const auto block_of = [&](int k) {
-      return k < rounds * pieces ? k / pieces * lanes + me : rounds * lanes + (dealt ? me / pieces : me);
-    };
-    const auto piece_of = [&](int k) { return k >= rounds * pieces && dealt ? me % pieces : k % pieces; };
-    const auto fetch_b = [&](int cb, u32x4* br) {
-      const int c = cb * CB + l16 * VEC;
-      if (cb * CB + CB <= a.N) {  // the same for the wave
+  int held = -1;
+  for (int k = 0; k < all; ++k) {
+    const int cb = block_of(k), m = piece_of(k);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) br[i] = Io::load(Bm + (int64_t)min(rank_of<IO, RP>(q, i), a.R - 1) * a.N + c);
-      } else {
+    for (int i = 0; i < 4; ++i) yr[i] = ADD ? yn[i] : Io::fill(0);
+    if (cb != held) {
+      held = cb;
+      if constexpr (!AHEAD) fetch_b(cb, br);
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
-          br[i] = Io::load_end(Bm + (int64_t)min(rank_of<IO, RP>(q, i), a.R - 1) * a.N, c, a.N);
+      for (int i = 0; i < NB; ++i) {
+        if constexpr (AHEAD) br[i] = bn[i];
+        if (rank_of<IO, RP>(q, i) >= a.R) br[i] = Io::fill(0);
       }
-    };
-    const auto fetch_y = [&](int cb, int m, u32x4* yr) {
-      const int c = cb * CB + l16 * VEC;
-      if (cb * CB + CB <= a.N) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) yr[i] = Io::load(yb + min(16 * m + 4 * q + i, rows - 1) * a.y_ts + c);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) yr[i] = Io::load_end(yb + min(16 * m + 4 * q + i, rows - 1) * a.y_ts, c, a.N);
-      }
-    };
-    u32x4 br[NB], bn[NB], yr[4], yn[4];
-    if (all > 0) {
-      fetch_b(block_of(0), bn);
-      if constexpr (ADD) fetch_y(block_of(0), piece_of(0), yn);
-    }
-    int held = -1;
-    for (int k = 0; k < all; ++k) {
-      const int cb = block_of(k), m = piece_of(k);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) yr[i] = ADD ? yn[i] : Io::fill(0);
-      if (cb != held) {
-        held = cb;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) br[i] = rank_of<IO, RP>(q, i) < a.R ? bn[i] : Io::fill(0);
-        if constexpr (!WIDE) {
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
-            u32x4 t[8];
-            transpose8(br + 8 * kb, t);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) br[8 * kb + i] = t[i];
-          }
-        }
-      }
-      if (k + 1 < all) {
-        if (block_of(k + 1) != cb) fetch_b(block_of(k + 1), bn);
-        if constexpr (ADD) fetch_y(block_of(k + 1), piece_of(k + 1), yn);
-      }
-      f32x4 z[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) z[j] = (f32x4){0, 0, 0, 0};
-      const int r = 16 * m + l16;
-      if constexpr (WIDE) {
-#pragma unroll
-        for (int s = 0; s < RP / 4; ++s) {
-          const float u = hid.u[r][q * (RP / 4) + s];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            z[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(u, __uint_as_float(br[s][j]), z[j], 0, 0, 0);
-        }
-      } else if constexpr (RP == 16) {
-        const E* src = q < 2 ? &hid.hi[r][8 * q] : &hid.lo[r][8 * (q - 2)];
-        const u32x4 u = *reinterpret_cast<const u32x4*>(src);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) z[j] = mma<IO>(u, br[j], z[j]);
-      } else {
+      if constexpr (!WIDE) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-          const u32x4 uh = *reinterpret_cast<const u32x4*>(&hid.hi[r][32 * kb + 8 * q]);
-          const u32x4 ul = *reinterpret_cast<const u32x4*>(&hid.lo[r][32 * kb + 8 * q]);
+          u32x4 t[8];
+          transpose8(br + 8 * kb, t);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            z[j] = mma<IO>(ul, br[8 * kb + j], z[j]);
-            z[j] = mma<IO>(uh, br[8 * kb + j], z[j]);
-          }
+          for (int i = 0; i < 8; ++i) br[8 * kb + i] = t[i];
         }
       }
-      const int c = cb * CB + l16 * VEC, n = min(max(a.N - c, 0), VEC);
+    }
+    if (k + 1 < all) {
+      if constexpr (ADD) fetch_y(block_of(k + 1), piece_of(k + 1), yn);
+      if (AHEAD && block_of(k + 1) != cb) fetch_b(block_of(k + 1), bn);
+    }
+    f32x4 z[VEC];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * m + 4 * q + i;
-        float o[VEC];
-        u32x4 w = yr[i];
-        Io::unpack(w, o);
-        float f = 1.0f;
-        if constexpr (!WIDE && IO::INF == IoF16::INF) f = hid.factor[row];
+    for (int j = 0; j < VEC; ++j) z[j] = (f32x4){0, 0, 0, 0};
+    const int ur = 16 * m + l16;
+    if constexpr (WIDE) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = fmaf(f, z[j][i], o[j]);
-        if (row < live) w = Io::pack(o);
-        if (row < rows && !(ADD && a.in_place && row >= live)) Io::store_some(ob + row * a.o_ts + c, w, n);
+      for (int t = 0; t < RP / 4; ++t) {
+        const float u = hid.u[ur][q * (RP / 4) + t];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          z[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(u, __uint_as_float(br[t][j]), z[j], 0, 0, 0);
       }
+    } else if constexpr (RP == 16) {
+      const E* src = q < 2 ? &hid.hi[ur][8 * q] : &hid.lo[ur][8 * (q - 2)];
+      const u32x4 u = *reinterpret_cast<const u32x4*>(src);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) z[j] = mma<IO>(u, br[j], z[j]);
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const u32x4 uh = *reinterpret_cast<const u32x4*>(&hid.hi[ur][32 * kb + 8 * q]);
+        const u32x4 ul = *reinterpret_cast<const u32x4*>(&hid.lo[ur][32 * kb + 8 * q]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          z[j] = mma<IO>(ul, br[8 * kb + j], z[j]);
+          z[j] = mma<IO>(uh, br[8 * kb + j], z[j]);
+        }
+      }
+    }
+    const int sl = anew(l16), n = min(max(a.N - cb * CB - sl * VEC, 0), VEC);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * m + 4 * (lane >> 4) + i;
+      float o[VEC];
+      u32x4 w = yr[i];
+      Io::unpack(w, o);
+      float f = 1.0f;
+      if constexpr (!WIDE && IO::INF == IoF16::INF) f = hid.factor[row];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) o[j] = fmaf(f, z[j][i], o[j]);
+      if (row < live) w = Io::pack(o);
+      if (row < rows && !(ADD && a.in_place && row >= live))
+        Io::store_some(shifted(ob + cb * CB, row * a.o_ts + (uint32_t)(sl * 16)), w, n);
     }
   }
 }
@@ -387,13 +467,15 @@ __global__ __launch_bounds__(WAVES * 64, RP == 64 ? 2 : 3) void adapter_kernel(A
 // and reads 8 rows of each lane's VEC columns at once, the next ones while it multiplies.
 struct OuterArgs {
   const void *x, *dy;
-  int64_t x_bs, x_ts, dy_bs, dy_ts;
+  int64_t x_bs, dy_bs;
+  uint32_t x_ts, dy_ts;
   const float *du, *u;  // as keep_hidden left them
   const int32_t *voices, *lengths;
   float* part;
-  int T, K, N, V, chunks, span, pitch, groups;
+  int T, K, N, V, chunks, span, tiles, groups;
 };
 
+constexpr int WAVES = 4;
 template <class IO, int RP>
 __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
   constexpr int VEC = IO::VEC, NJ = RP / 16, CB = 16 * VEC;
@@ -412,7 +494,7 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
   const int width = of_x ? a.K : a.N;
   const int c = cb * CB + l16 * VEC, n = min(max(width - c, 0), VEC);
   const bool whole = cb * CB + CB <= width;
-  const int64_t ts = of_x ? a.x_ts : a.dy_ts;
+  const uint32_t ts = of_x ? a.x_ts : a.dy_ts;
   const E* src = of_x ? static_cast<const E*>(a.x) + b * a.x_bs : static_cast<const E*>(a.dy) + b * a.dy_bs;
   const float* ub = of_x ? a.du : a.u;
   f32x4 acc[NJ][VEC];
@@ -424,20 +506,22 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
   const auto fetch = [&](int r0, u32x4* xr, u32x4 (*ur)[2]) {
     if (whole) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) xr[i] = Io::load(src + min(r0 + 8 * q + i, last - 1) * ts + c);
+      for (int i = 0; i < 8; ++i)
+        xr[i] = Io::load(shifted(row_at(src + cb * CB, r0, ts), min(8 * q + i, last - 1 - r0) * ts + (uint32_t)(l16 * 16)));
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) xr[i] = Io::load_end(src + min(r0 + 8 * q + i, last - 1) * ts, c, width);
+      for (int i = 0; i < 8; ++i)
+        xr[i] = Io::load_end(shifted(row_at(src, r0, ts), min(8 * q + i, last - 1 - r0) * ts), c, width);
     }
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) hidden_rows<IO, RP>(ub, (int64_t)b, a.pitch, 16 * j + l16, r0 + 8 * q, ur[j]);
+    for (int j = 0; j < NJ; ++j) hidden_rows<RP>(ub, (int64_t)b * a.tiles + r0 / ROWS, j, lane, ur[j]);
   };
   u32x4 xr[8], ur[NJ][2];
   fetch(first, xr, ur);
-  for (int r0 = first; r0 < last; r0 += 32) {
+  for (int r0 = first; r0 < last; r0 += ROWS) {
     u32x4 xn[8], un[NJ][2];
-    if (r0 + 32 < last) fetch(r0 + 32, xn, un);
-    if (r0 + 32 > last) {
+    if (r0 + ROWS < last) fetch(r0 + ROWS, xn, un);
+    if (r0 + ROWS > last) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (r0 + 8 * q + i >= last) xr[i] = Io::fill(0);
@@ -532,87 +616,74 @@ __global__ __launch_bounds__(LISTED) void gather_kernel(GatherArgs a) {
 
 int padded_rank(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : 64; }
 
-// Workgroups share the columns of a tile of rows where the tiles alone do not fill 256 CUs twice (each then repeats the
-// first product).
-int column_splits(int64_t tiles, int N, int vec) {
-  const int most = ceil_div(ceil_div(N, 16 * vec), WAVES);
-  const int64_t want = tiles >= 512 ? 1 : (512 + tiles - 1) / tiles;
-  return (int)(want < most ? want : most);
-}
-
-template <class IO, int RP, int MF, bool ADD, bool EXPAND>
-int launch_tile_of(AddArgs a, int B, hipStream_t s) {
-  a.tiles = ceil_div(a.T, 16 * MF);
-  const int64_t tiles = (int64_t)B * a.tiles;
-  a.splits = EXPAND ? column_splits(tiles, a.N, IO::VEC) : 1;
-  TTSX_ARG(tiles * a.splits <= 0x7fffffff, "ttsx_adapter: too many rows");
-  adapter_kernel<IO, RP, MF, ADD, EXPAND><<<(unsigned)(tiles * a.splits), WAVES * 64, 0, s>>>(a);
+template <class IO, int RP, int WV, bool ADD>
+int launch_waves(AddArgs a, int64_t tiles, int splits, hipStream_t s) {
+  a.splits = splits;
+  TTSX_ARG(tiles * splits <= 0x7fffffff, "ttsx_adapter: too many rows");
+  adapter_kernel<IO, RP, WV, ADD><<<(unsigned)(tiles * splits), WV * 64, 0, s>>>(a);
   TTSX_LAUNCH_CHECK();
   return TTSX_OK;
 }
-template <class IO, int RP, bool ADD, bool EXPAND>
-int launch_tile(const AddArgs& a, int B, hipStream_t s) {
-  const int64_t large = (int64_t)B * ceil_div(a.T, 64);
-  if (large >= MF4_TILES) return launch_tile_of<IO, RP, 4, ADD, EXPAND>(a, B, s);
-  return launch_tile_of<IO, RP, 2, ADD, EXPAND>(a, B, s);
+// Four waves to a tile where the tiles fill 256 CUs twice.  Fewer tiles get a workgroup of 16 waves each (8 at rank 64,
+// whose operands need the registers) and share their columns among up to 256 workgroups; each of those repeats the
+// first product, so no more of them than N is longer than K.
+template <class IO, int RP, bool ADD>
+int launch_tiles(AddArgs a, int B, hipStream_t s) {
+  constexpr int MANY = RP == 64 ? 8 : 16;
+  a.tiles = ceil_div(a.T, ROWS);
+  const int64_t tiles = (int64_t)B * a.tiles;
+  if (tiles >= 512) return launch_waves<IO, RP, 4, ADD>(a, tiles, 1, s);
+  const int blocks = ceil_div(a.N, 16 * IO::VEC), pieces = ceil_div(min(a.T, ROWS), 16);
+  const int splits = min(min(ceil_div(blocks * pieces, MANY), max(1, (int)(256 / tiles))), max(1, a.N / a.first.K));
+  return launch_waves<IO, RP, MANY, ADD>(a, tiles, splits, s);
 }
 
 template <class IO>
 int run_add(const AddArgs& a, int B, hipStream_t s) {
   switch (padded_rank(a.R)) {
-    case 16: return launch_tile<IO, 16, true, true>(a, B, s);
-    case 32: return launch_tile<IO, 32, true, true>(a, B, s);
-    default: return launch_tile<IO, 64, true, true>(a, B, s);
+    case 16: return launch_tiles<IO, 16, true>(a, B, s);
+    case 32: return launch_tiles<IO, 32, true>(a, B, s);
+    default: return launch_tiles<IO, 64, true>(a, B, s);
   }
 }
 
 struct BackPlan {
-  int RP, pitch, chunks, span;
+  int RP, chunks, span;
   size_t hidden, part;  // floats
 };
 // Slices of a request's rows: enough waves (one per 16 VEC columns and slice) to fill the chip, 64 rows at least.
 BackPlan back_plan(int B, int T, int K, int N, int R, int vec) {
   BackPlan p;
   p.RP = padded_rank(R);
-  p.pitch = round_up(T, 32);
   const int64_t waves = (int64_t)B * (ceil_div(K, 16 * vec) + ceil_div(N, 16 * vec));
   const int want = waves >= 2048 ? 1 : (int)((2048 + waves - 1) / waves), most = ceil_div(T, 64);
-  p.span = round_up(ceil_div(T, want < most ? want : most), 32);
+  p.span = round_up(ceil_div(T, want < most ? want : most), ROWS);
   p.chunks = ceil_div(T, p.span);
-  p.hidden = (size_t)B * p.RP * p.pitch;
+  p.hidden = (size_t)B * p.RP * round_up(T, ROWS);
   p.part = (size_t)B * p.chunks * p.RP * ((size_t)K + N);
   return p;
 }
 
 template <class IO, int RP>
-int run_backward(const AddArgs& dx, const BackPlan& p, int B, float* ws, void* ddown, void* dup, hipStream_t s) {
+int run_backward(AddArgs a, const BackPlan& p, int B, float* ws, void* ddown, void* dup, hipStream_t s) {
   float *du = ws, *u = du + p.hidden, *part = u + p.hidden;
-  // dx = (s dy B^T) A, keeping s dy B^T
-  AddArgs a = dx;
-  a.keep = du, a.keep_pitch = p.pitch;
-  int rc = launch_tile<IO, RP, false, true>(a, B, s);
-  if (rc != TTSX_OK) return rc;
-  // s x A^T
-  AddArgs c = dx;
-  c.x = dx.y, c.x_bs = dx.y_bs, c.x_ts = dx.y_ts, c.K = dx.N, c.N = dx.K;
-  c.down = dx.up, c.up = nullptr, c.out = nullptr;
-  c.keep = u, c.keep_pitch = p.pitch;
-  rc = launch_tile<IO, RP, false, false>(c, B, s);
+  a.first.keep = du, a.second.keep = u;
+  const int rc = launch_tiles<IO, RP, false>(a, B, s);
   if (rc != TTSX_OK) return rc;
   OuterArgs o{};
-  o.x = dx.y, o.x_bs = dx.y_bs, o.x_ts = dx.y_ts;
-  o.dy = dx.x, o.dy_bs = dx.x_bs, o.dy_ts = dx.x_ts;
-  o.du = du, o.u = u, o.voices = dx.voices, o.lengths = dx.lengths, o.part = part;
-  o.T = dx.T, o.K = dx.N, o.N = dx.K, o.V = dx.V, o.chunks = p.chunks, o.span = p.span, o.pitch = p.pitch;
+  o.x = a.second.x, o.x_bs = a.second.bs, o.x_ts = a.second.ts;
+  o.dy = a.first.x, o.dy_bs = a.first.bs, o.dy_ts = a.first.ts;
+  o.du = du, o.u = u, o.voices = a.voices, o.lengths = a.lengths, o.part = part;
+  o.T = a.T, o.K = a.second.K, o.N = a.first.K, o.V = a.V, o.chunks = p.chunks, o.span = p.span, o.tiles = ceil_div(a.T, ROWS);
   o.groups = ceil_div(ceil_div(o.K, 16 * IO::VEC) + ceil_div(o.N, 16 * IO::VEC), WAVES);
   const int64_t grid = (int64_t)B * p.chunks * o.groups;
   TTSX_ARG(grid <= 0x7fffffff, "ttsx_adapter_backward: too many rows");
   outer_kernel<IO, RP><<<(unsigned)grid, WAVES * 64, 0, s>>>(o);
   TTSX_LAUNCH_CHECK();
   GatherArgs g{};
-  g.part = part, g.voices = dx.voices, g.lengths = dx.lengths, g.ddown = ddown, g.dup = dup;
-  g.B = B, g.T = dx.T, g.K = o.K, g.N = o.N, g.R = dx.R, g.RP = RP, g.chunks = p.chunks, g.span = p.span;
-  const int64_t outs = (int64_t)dx.V * dx.R * ceil_div(o.K + o.N, LISTED);
+  g.part = part, g.voices = a.voices, g.lengths = a.lengths, g.ddown = ddown, g.dup = dup;
+  g.B = B, g.T = a.T, g.K = o.K, g.N = o.N, g.R = a.R, g.RP = RP, g.chunks = p.chunks, g.span = p.span;
+  const int64_t outs = (int64_t)a.V * a.R * ceil_div(o.K + o.N, LISTED);
   TTSX_ARG(outs <= 0x7fffffff, "ttsx_adapter_backward: too many voices");
   gather_kernel<IO><<<(unsigned)outs, LISTED, 0, s>>>(g);
   TTSX_LAUNCH_CHECK();
@@ -628,9 +699,12 @@ int run_backward_any(const AddArgs& a, const BackPlan& p, int B, float* ws, void
   }
 }
 
+// The widest row: the offsets inside a tile, and inside an adapter, fit 32 bits.
+constexpr int64_t MAX_STRIDE = 1 << 20;
+bool stride_ok(int64_t s) { return s >= 0 && s <= MAX_STRIDE; }
 bool shape_ok(int B, int T, int K, int N, int R, int V) {
   return B >= 1 && T >= 1 && K >= 1 && N >= 1 && R >= 1 && R <= TTSX_ADAPTER_MAX_RANK && V >= 1 && T <= (1 << 30) &&
-         K <= (1 << 24) && N <= (1 << 24) && V <= (1 << 24);
+         K <= MAX_STRIDE && N <= MAX_STRIDE && V <= (1 << 24);
 }
 bool dtype_ok(int d) { return d == TTSX_F32 || d == TTSX_BF16 || d == TTSX_F16; }
 
@@ -645,12 +719,16 @@ extern "C" int ttsx_adapter_add(const void* y, int64_t y_batch_stride, int64_t y
   TTSX_ARG(shape_ok(B, T, K, N, R, V), "ttsx_adapter_add: bad shape B=%d T=%d K=%d N=%d R=%d V=%d (1 <= R <= %d)", B, T,
            K, N, R, V, TTSX_ADAPTER_MAX_RANK);
   TTSX_ARG(dtype_ok(dtype), "ttsx_adapter_add: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
+  TTSX_ARG(stride_ok(y_row_stride) && stride_ok(x_row_stride) && stride_ok(out_row_stride),
+           "ttsx_adapter_add: a row stride outside 0..%ld", (long)MAX_STRIDE);
   TTSX_ARG(out != y || (out_batch_stride == y_batch_stride && out_row_stride == y_row_stride),
            "ttsx_adapter_add: out is y with other strides");
   AddArgs a{};
-  a.x = x, a.x_bs = x_batch_stride, a.x_ts = x_row_stride, a.y = y, a.y_bs = y_batch_stride, a.y_ts = y_row_stride;
-  a.out = out, a.o_bs = out_batch_stride, a.o_ts = out_row_stride, a.down = down, a.up = up;
-  a.voices = voices, a.scale = scale, a.lengths = lengths, a.T = T, a.K = K, a.N = N, a.R = R, a.V = V;
+  const int64_t size = dtype == TTSX_F32 ? 4 : 2;
+  a.first = {x, down, x_batch_stride, (uint32_t)(x_row_stride * size), K, nullptr};
+  a.y = y, a.y_bs = y_batch_stride, a.y_ts = (uint32_t)(y_row_stride * size), a.up = up;
+  a.out = out, a.o_bs = out_batch_stride, a.o_ts = (uint32_t)(out_row_stride * size);
+  a.voices = voices, a.scale = scale, a.lengths = lengths, a.T = T, a.N = N, a.R = R, a.V = V;
   a.in_place = out == y;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return dtype == TTSX_F32 ? run_add<IoF32>(a, B, s) : dtype == TTSX_BF16 ? run_add<IoBf16>(a, B, s) : run_add<IoF16>(a, B, s);
@@ -671,14 +749,18 @@ extern "C" int ttsx_adapter_backward(const void* dy, int64_t dy_batch_stride, in
   TTSX_ARG(shape_ok(B, T, K, N, R, V), "ttsx_adapter_backward: bad shape B=%d T=%d K=%d N=%d R=%d V=%d (1 <= R <= %d)",
            B, T, K, N, R, V, TTSX_ADAPTER_MAX_RANK);
   TTSX_ARG(dtype_ok(dtype), "ttsx_adapter_backward: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
+  TTSX_ARG(stride_ok(dy_row_stride) && stride_ok(x_row_stride), "ttsx_adapter_backward: a row stride outside 0..%ld",
+           (long)MAX_STRIDE);
   const BackPlan p = back_plan(B, T, K, N, R, dtype == TTSX_F32 ? 4 : 8);
   TTSX_ARG(workspace_bytes >= sizeof(float) * (2 * p.hidden + p.part) && (uintptr_t)workspace % 16 == 0,
            "ttsx_adapter_backward: workspace too small or not aligned to 16 bytes");
-  // the forward kernel with dy for x and the matrices swapped; its y is the x of this call
+  // the forward kernel with dy for x and the matrices swapped; x A^T is only kept
   AddArgs a{};
-  a.x = dy, a.x_bs = dy_batch_stride, a.x_ts = dy_row_stride, a.y = x, a.y_bs = x_batch_stride, a.y_ts = x_row_stride;
-  a.out = dx, a.o_bs = (int64_t)T * K, a.o_ts = K, a.down = up, a.up = down;
-  a.voices = voices, a.scale = scale, a.lengths = lengths, a.T = T, a.K = N, a.N = K, a.R = R, a.V = V;
+  const int64_t size = dtype == TTSX_F32 ? 4 : 2;
+  a.first = {dy, up, dy_batch_stride, (uint32_t)(dy_row_stride * size), N, nullptr};
+  a.second = {x, down, x_batch_stride, (uint32_t)(x_row_stride * size), K, nullptr};
+  a.out = dx, a.o_bs = (int64_t)T * K, a.o_ts = (uint32_t)(K * size), a.up = down;
+  a.voices = voices, a.scale = scale, a.lengths = lengths, a.T = T, a.N = K, a.R = R, a.V = V;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   float* ws = static_cast<float*>(workspace);
   return dtype == TTSX_F32    ? run_backward_any<IoF32>(a, p, B, ws, ddown, dup, s)
