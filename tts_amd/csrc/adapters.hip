@@ -263,7 +263,7 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
   constexpr bool WIDE = VEC == 4;
   typedef typename IO::elem E;
   typedef Full<IO> Io;
-  __shared__ float part[WV][ROWS][RP + 1];
+  __shared__ float part[ADD ? 1 : 2][WV][ROWS][RP + 1];
   __shared__ Hidden<IO, RP> hid;
   const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits % a.tiles, b = blockIdx.x / a.splits / a.tiles;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
@@ -341,26 +341,23 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
 
   const float s = a.scale ? a.scale[v] : 1.0f;
   const int r = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (RP / 8);  // of the sums: 8 threads to a row
-  if constexpr (!ADD) {
-    const E* xb = row_at(static_cast<const E*>(a.second.x) + b * a.second.bs, row0, a.second.ts);
-    if (split == 0) {
-      first_product<IO, RP, WV>(a.second, xb, v, a.R, live, wave, lane, part);
-      __syncthreads();
-      if (r < ROWS) {
-        float u[RP / 8];
-        sum_shares<RP, WV>(part, r, c0, live, a.R, s, u);
-        keep_hidden<IO, RP>(a.second.keep, (int64_t)b * a.tiles + tile, r, c0, u);
-      }
-      __syncthreads();
-    }
-  }
   first_product<IO, RP, WV>(a.first, row_at(static_cast<const E*>(a.first.x) + b * a.first.bs, row0, a.first.ts), v, a.R,
-                            live, wave, lane, part);
-  if (AHEAD && all > 0) fetch_b(block_of(0), bn);
+                            live, wave, lane, part[0]);
+  if constexpr (!ADD) {
+    // its 256 bytes go to the waves the first product leaves off at
+    if (split == 0)
+      first_product<IO, RP, WV>(a.second, row_at(static_cast<const E*>(a.second.x) + b * a.second.bs, row0, a.second.ts),
+                                v, a.R, live, (wave + WV - ceil_div(a.first.K, 16 * VEC) % WV) % WV, lane, part[1]);
+  }
+  if (all > 0) fetch_b(block_of(0), AHEAD ? bn : br);
   __syncthreads();
   if (r < ROWS) {
     float u[RP / 8];
-    sum_shares<RP, WV>(part, r, c0, live, a.R, s, u);
+    if (!ADD && split == 0) {
+      sum_shares<RP, WV>(part[ADD ? 0 : 1], r, c0, live, a.R, s, u);
+      keep_hidden<IO, RP>(a.second.keep, (int64_t)b * a.tiles + tile, r, c0, u);
+    }
+    sum_shares<RP, WV>(part[0], r, c0, live, a.R, s, u);
     if (!ADD && split == 0) keep_hidden<IO, RP>(a.first.keep, (int64_t)b * a.tiles + tile, r, c0, u);
     if constexpr (WIDE) {
 #pragma unroll
@@ -395,7 +392,7 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
     for (int i = 0; i < 4; ++i) yr[i] = ADD ? yn[i] : Io::fill(0);
     if (cb != held) {
       held = cb;
-      if constexpr (!AHEAD) fetch_b(cb, br);
+      if (!AHEAD && k > 0) fetch_b(cb, br);
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         if constexpr (AHEAD) br[i] = bn[i];
@@ -463,8 +460,9 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
 }
 
 // Weights' gradients, one request (and slice of its rows) at a time: part[b][chunk][rank][column] = sum of u x over
-// the slice's rows, the columns of x (from du) first, those of dy (from u) behind them.  A wave owns 16 VEC columns
-// and reads 8 rows of each lane's VEC columns at once, the next ones while it multiplies.
+// the slice's rows, the columns of x (from du) first, those of dy (from u) behind them.  A workgroup owns 16 VEC columns,
+// its waves take every fourth 32 rows, 8 of them and VEC columns to a lane, the next ones in flight while they multiply;
+// their sums meet in LDS, the upper two waves' first.
 struct OuterArgs {
   const void *x, *dy;
   int64_t x_bs, dy_bs;
@@ -472,7 +470,7 @@ struct OuterArgs {
   const float *du, *u;  // as keep_hidden left them
   const int32_t *voices, *lengths;
   float* part;
-  int T, K, N, V, chunks, span, tiles, groups;
+  int T, K, N, V, chunks, span, tiles;
 };
 
 constexpr int WAVES = 4;
@@ -481,11 +479,11 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
   constexpr int VEC = IO::VEC, NJ = RP / 16, CB = 16 * VEC;
   typedef typename IO::elem E;
   typedef Full<IO> Io;
-  const int group = blockIdx.x % a.groups, chunk = blockIdx.x / a.groups % a.chunks, b = blockIdx.x / a.groups / a.chunks;
+  const int kblocks = ceil_div(a.K, CB), groups = kblocks + ceil_div(a.N, CB);
+  int cb = blockIdx.x % groups;
+  const int chunk = blockIdx.x / groups % a.chunks, b = blockIdx.x / groups / a.chunks;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
-  const int kblocks = ceil_div(a.K, CB), nblocks = ceil_div(a.N, CB);
-  int cb = group * WAVES + wave;
-  if (cb >= kblocks + nblocks) return;
+  __shared__ f32x4 sums[2][NJ * VEC][64];
   const int len = valid_rows(a.lengths, b, a.T);
   const int first = chunk * a.span, last = min(first + a.span, len);
   if (voice_of(a.voices, b, a.V) < 0 || first >= last) return;
@@ -517,10 +515,10 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
     for (int j = 0; j < NJ; ++j) hidden_rows<RP>(ub, (int64_t)b * a.tiles + r0 / ROWS, j, lane, ur[j]);
   };
   u32x4 xr[8], ur[NJ][2];
-  fetch(first, xr, ur);
-  for (int r0 = first; r0 < last; r0 += ROWS) {
+  if (first + wave * ROWS < last) fetch(first + wave * ROWS, xr, ur);
+  for (int r0 = first + wave * ROWS; r0 < last; r0 += WAVES * ROWS) {
     u32x4 xn[8], un[NJ][2];
-    if (r0 + ROWS < last) fetch(r0 + ROWS, xn, un);
+    if (r0 + WAVES * ROWS < last) fetch(r0 + WAVES * ROWS, xn, un);
     if (r0 + ROWS > last) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -553,6 +551,24 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) ur[j][0] = un[j][0], ur[j][1] = un[j][1];
   }
+#pragma unroll
+  for (int half = 2; half > 0; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sums[wave - half][j * VEC + i][lane] = acc[j][i];
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[j][i] += sums[wave][j * VEC + i][lane];
+    }
+    __syncthreads();
+  }
+  if (wave > 0) return;
   const int total = a.K + a.N;
   float* out = a.part + (int64_t)(b * a.chunks + chunk) * RP * total + (of_x ? 0 : a.K) + c;
 #pragma unroll
@@ -566,7 +582,7 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
     }
 }
 
-// Sum over the requests of a voice, in their order.  A thread takes one column; the requests of the voice are listed
+// Sum over the requests of a voice, in their order.  A thread takes four columns; the requests of the voice are listed
 // first, so that the loads of several are in flight.
 struct GatherArgs {
   const float* part;
@@ -579,11 +595,13 @@ template <class IO>
 __global__ __launch_bounds__(LISTED) void gather_kernel(GatherArgs a) {
   typedef typename IO::elem E;
   __shared__ int slices[LISTED], count[LISTED / 64];
-  const int total = a.K + a.N, cols = ceil_div(total, LISTED);
-  const int col = blockIdx.x % cols * LISTED + threadIdx.x, r = blockIdx.x / cols % a.R, v = blockIdx.x / cols / a.R;
+  const int total = a.K + a.N, cols = ceil_div(total, LISTED * 4);
+  const int col = (blockIdx.x % cols * LISTED + threadIdx.x) * 4, r = blockIdx.x / cols % a.R, v = blockIdx.x / cols / a.R;
   const int64_t pitch = (int64_t)a.RP * total;
-  const float* p = a.part + (int64_t)r * total + min(col, total - 1);
-  float s = 0.0f;
+  // the last thread of a row that ends inside its four columns takes the row's last four (a row has two at least)
+  const int at0 = min(col, max(total - 4, 0));
+  const float* p = a.part + (int64_t)r * total + at0;
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int from = 0; from < a.B * a.chunks; from += LISTED) {
     // in order: a thread's slice goes where the slices in front of it leave off
     const int k = from + threadIdx.x, b = k / a.chunks;
@@ -598,20 +616,40 @@ __global__ __launch_bounds__(LISTED) void gather_kernel(GatherArgs a) {
     }
     if (mine) slices[at] = k;
     __syncthreads();
+    const auto take = [&](int k, float* t) {
+      if (total >= 4)
+        load_f32<4>(p + slices[k] * pitch, t);
+      else
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = j < total ? p[slices[k] * pitch + j] : 0.0f;
+    };
     int i = 0;
     for (; i + 4 <= all; i += 4) {
-      const float t0 = p[slices[i] * pitch], t1 = p[slices[i + 1] * pitch], t2 = p[slices[i + 2] * pitch],
-                  t3 = p[slices[i + 3] * pitch];
-      s = (((s + t0) + t1) + t2) + t3;
+      float t[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) take(i + k, t[k]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] += t[k][j];
     }
-    for (; i < all; ++i) s += p[slices[i] * pitch];
+    for (; i < all; ++i) {
+      float t[4];
+      take(i, t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] += t[j];
+    }
     __syncthreads();
   }
-  if (col >= total) return;
-  if (col < a.K)
-    static_cast<E*>(a.ddown)[((int64_t)v * a.R + r) * a.K + col] = (E)s;
-  else
-    static_cast<E*>(a.dup)[((int64_t)v * a.R + r) * a.N + col - a.K] = (E)s;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = at0 + j;
+    if (c < col || c >= total) continue;
+    if (c < a.K)
+      static_cast<E*>(a.ddown)[((int64_t)v * a.R + r) * a.K + c] = (E)s[j];
+    else
+      static_cast<E*>(a.dup)[((int64_t)v * a.R + r) * a.N + c - a.K] = (E)s[j];
+  }
 }
 
 int padded_rank(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : 64; }
@@ -651,12 +689,13 @@ struct BackPlan {
   int RP, chunks, span;
   size_t hidden, part;  // floats
 };
-// Slices of a request's rows: enough waves (one per 16 VEC columns and slice) to fill the chip, 64 rows at least.
+// Slices of a request's rows: enough workgroups (one per 16 VEC columns and slice) to fill 256 CUs twice, 128 rows at
+// least; every slice more is written and read again.
 BackPlan back_plan(int B, int T, int K, int N, int R, int vec) {
   BackPlan p;
   p.RP = padded_rank(R);
-  const int64_t waves = (int64_t)B * (ceil_div(K, 16 * vec) + ceil_div(N, 16 * vec));
-  const int want = waves >= 2048 ? 1 : (int)((2048 + waves - 1) / waves), most = ceil_div(T, 64);
+  const int64_t groups = (int64_t)B * (ceil_div(K, 16 * vec) + ceil_div(N, 16 * vec));
+  const int want = groups >= 512 ? 1 : (int)((512 + groups - 1) / groups), most = ceil_div(T, WAVES * ROWS);
   p.span = round_up(ceil_div(T, want < most ? want : most), ROWS);
   p.chunks = ceil_div(T, p.span);
   p.hidden = (size_t)B * p.RP * round_up(T, ROWS);
@@ -675,15 +714,14 @@ int run_backward(AddArgs a, const BackPlan& p, int B, float* ws, void* ddown, vo
   o.dy = a.first.x, o.dy_bs = a.first.bs, o.dy_ts = a.first.ts;
   o.du = du, o.u = u, o.voices = a.voices, o.lengths = a.lengths, o.part = part;
   o.T = a.T, o.K = a.second.K, o.N = a.first.K, o.V = a.V, o.chunks = p.chunks, o.span = p.span, o.tiles = ceil_div(a.T, ROWS);
-  o.groups = ceil_div(ceil_div(o.K, 16 * IO::VEC) + ceil_div(o.N, 16 * IO::VEC), WAVES);
-  const int64_t grid = (int64_t)B * p.chunks * o.groups;
+  const int64_t grid = (int64_t)B * p.chunks * (ceil_div(o.K, 16 * IO::VEC) + ceil_div(o.N, 16 * IO::VEC));
   TTSX_ARG(grid <= 0x7fffffff, "ttsx_adapter_backward: too many rows");
   outer_kernel<IO, RP><<<(unsigned)grid, WAVES * 64, 0, s>>>(o);
   TTSX_LAUNCH_CHECK();
   GatherArgs g{};
   g.part = part, g.voices = a.voices, g.lengths = a.lengths, g.ddown = ddown, g.dup = dup;
   g.B = B, g.T = a.T, g.K = o.K, g.N = o.N, g.R = a.R, g.RP = RP, g.chunks = p.chunks, g.span = p.span;
-  const int64_t outs = (int64_t)a.V * a.R * ceil_div(o.K + o.N, LISTED);
+  const int64_t outs = (int64_t)a.V * a.R * ceil_div(o.K + o.N, LISTED * 4);
   TTSX_ARG(outs <= 0x7fffffff, "ttsx_adapter_backward: too many voices");
   gather_kernel<IO><<<(unsigned)outs, LISTED, 0, s>>>(g);
   TTSX_LAUNCH_CHECK();
