@@ -83,6 +83,15 @@ def test_scan_over_a_cut_time_axis(dtype):
     _check_scan(x, g, h0, lengths, True, dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("reverse", [False, True])
+def test_cut_time_axis_of_whole_channel_groups(dtype, reverse):
+    """The same where lanes take several channels: both passes, short requests that end chunks early."""
+    x, g, h0, lengths = _inputs(4, 4100, 16, dtype, 7, ragged=True)
+    _check_scan(x, g, h0, lengths, reverse, dtype)
+    _check_backward(x, g, h0, lengths, reverse, dtype, 9)
+
+
 def test_scan_of_strided_and_repeated_inputs():
     """Time-major activations, a channel axis that is not contiguous, and a batch that repeats one request."""
     from tts_amd.recurrence import gated_scan

@@ -461,8 +461,8 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
 
 // Weights' gradients, one request (and slice of its rows) at a time: part[b][chunk][rank][column] = sum of u x over
 // the slice's rows, the columns of x (from du) first, those of dy (from u) behind them.  A workgroup owns 16 VEC columns,
-// its waves take every fourth 32 rows, 8 of them and VEC columns to a lane, the next ones in flight while they multiply;
-// their sums meet in LDS, the upper two waves' first.
+// its waves take every fourth 32 rows, 8 of them and VEC columns to a lane; their sums meet in LDS, the upper two waves'
+// first.  Three workgroups to a CU hide the loads (fetching the next rows ahead leaves room for two and is no faster).
 struct OuterArgs {
   const void *x, *dy;
   int64_t x_bs, dy_bs;
@@ -475,7 +475,7 @@ struct OuterArgs {
 
 constexpr int WAVES = 4;
 template <class IO, int RP>
-__global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
+__global__ __launch_bounds__(WAVES * 64, 3) void outer_kernel(OuterArgs a) {
   constexpr int VEC = IO::VEC, NJ = RP / 16, CB = 16 * VEC;
   typedef typename IO::elem E;
   typedef Full<IO> Io;
@@ -514,11 +514,9 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) hidden_rows<RP>(ub, (int64_t)b * a.tiles + r0 / ROWS, j, lane, ur[j]);
   };
-  u32x4 xr[8], ur[NJ][2];
-  if (first + wave * ROWS < last) fetch(first + wave * ROWS, xr, ur);
   for (int r0 = first + wave * ROWS; r0 < last; r0 += WAVES * ROWS) {
-    u32x4 xn[8], un[NJ][2];
-    if (r0 + WAVES * ROWS < last) fetch(r0 + WAVES * ROWS, xn, un);
+    u32x4 xr[8], ur[NJ][2];
+    fetch(r0, xr, ur);
     if (r0 + ROWS > last) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -546,10 +544,6 @@ __global__ __launch_bounds__(WAVES * 64) void outer_kernel(OuterArgs a) {
             acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ur[j][s / 4][s % 4]), xv[i], acc[j][i], 0, 0, 0);
       }
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) xr[i] = xn[i];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) ur[j][0] = un[j][0], ur[j][1] = un[j][1];
   }
 #pragma unroll
   for (int half = 2; half > 0; half /= 2) {

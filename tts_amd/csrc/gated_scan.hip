@@ -45,26 +45,41 @@ struct Shape {
   static_assert(TILE % BLOCK == 0 && BLOCK % L == 0, "a tile and some lane of it start at a kept state");
 };
 
-// w = sigmoid(-g); f = 1 - w wherever f is a factor of a state.  Long memories live in w: an error d of f is one of
-// d / w in the state, so w = e / (1 + e) keeps its own digits, with e = exp(-g) from exp2 of the rounded -g log2(e) and
-// what the rounding lost put back, and the difference 1 - w adds half a unit of f.  fw = f w, the slope of f, keeps its
-// digits at both ends.  Below -87 the exponential overflows: f is below 2e-38 there, w = 1.  A NaN stays one.
-__device__ static inline void gate(float g, float& w, float& fw) {
-  const bool low = g < -87.0f;
-  g = __builtin_elementwise_minimum(g, 126.0f);
-  const float t = -1.44269502f * g;
-  const float rest = fmaf(t, 1.90465421e-9f, fmaf(t, -0.693147182f, -g));  // -g - t ln 2, ln 2 in two parts
-  const float p = __builtin_amdgcn_exp2f(t);
-  const float e = fmaf(p, rest, p);
-  const float f = __builtin_amdgcn_rcpf(1.0f + e);
-  w = e * f;
-  fw = w * f;
-  w = low ? 1.0f : w;
-  fw = low ? 0.0f : fw;
+// log2(e) cut to 16 and 13 bits, and ln(2) times what was cut off.
+constexpr float L2E_16 = 1.44268799f, L2E_16_REST = 4.88849537e-6f;
+constexpr float L2E_13 = 1.44262695f, L2E_13_REST = 4.71948406e-5f;
+
+// w = sigmoid(-g) = 1 / (1 + e^g), to a few units in its own last place over all of g; f = 1 - w wherever f is a factor of
+// a state.  Long memories live in w (an error d of f is one of d / w in the state), and the difference adds half a unit
+// of f.  e^g is exp2 of the rounded product with log2(e), with what was rounded away put back: for 16-bit logits the
+// product with a log2(e) cut to 16 (bf16) or 13 bits (fp16) is exact and the rest of the constant is the correction, fp32
+// logits take it from a fused product.  -inf gives w = 1, +inf gives 0, a NaN stays one.
+template <class IO>
+__device__ static inline float gate(float g, float& e) {
+  float w;
+  if constexpr (IO::PER == 1) {
+    const float c = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -126.0f), 88.0f);
+    const float t = 1.44269502f * c;
+    const float rest = fmaf(t, -1.90465421e-9f, fmaf(t, -0.693147182f, c));  // c - t ln 2, ln 2 in two parts
+    const float p = __builtin_amdgcn_exp2f(t);
+    e = fmaf(p, rest, p);
+    w = __builtin_amdgcn_rcpf(1.0f + e);
+    w = g > 88.0f ? 0.0f : w;
+  } else {
+    constexpr bool B = IO::INF == IoBf16::INF;
+    constexpr float C1 = B ? L2E_16 : L2E_13, C2 = B ? L2E_16_REST : L2E_13_REST;
+    const float c = __builtin_elementwise_maximum(g, -126.0f);
+    const float p = __builtin_amdgcn_exp2f(C1 * c);
+    e = fmaf(p, C2 * c, p);
+    w = __builtin_amdgcn_rcpf(1.0f + e);
+  }
+  return w;
 }
+// f w, the slope of f, with its digits at both ends.
+__device__ static inline float slope(float w, float e) { return w * (e < 1.0f ? e * w : 1.0f - w); }
 
 struct Place {
-  int b, chunk, c, across, tg, wave, lane;  // c: first channel of the lane
+  int b, chunk, c, across, tg, wave, lane;  // c: first channel of the lane; wave: a scalar
   bool on;                                  // the lane has channels
 };
 template <class S>
@@ -73,7 +88,7 @@ __device__ static inline Place place(const ScanArgs& a) {
   const int id = blockIdx.x;
   q.chunk = id / a.cols % a.chunks;
   q.b = id / a.cols / a.chunks;
-  q.wave = threadIdx.x >> 6;
+  q.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   q.lane = threadIdx.x & 63;
   q.across = q.lane & (S::GROUP - 1);
   q.tg = threadIdx.x / S::GROUP;
@@ -93,16 +108,22 @@ struct Tile {
     count = min(len - p0, S::TILE);
     base = reverse ? len - p0 - count : p0;
   }
-  __device__ inline uint32_t row(const Place& q, int i) const {
-    const int k = min(q.tg * S::L + i, count - 1);
+  __device__ inline uint32_t row(int tg, int i) const {
+    const int k = min(tg * S::L + i, count - 1);
     return reverse ? count - 1 - k : k;
   }
-  __device__ inline bool live(const Place& q, int i) const { return q.tg * S::L + i < count; }
+  __device__ inline bool live(int tg, int i) const { return tg * S::L + i < count; }
 };
 template <class T>
 __device__ static inline T* shifted(T* base, int64_t bytes, uint32_t lane) {
   typedef typename std::conditional<std::is_const<T>::value, const char, char>::type C;
   return reinterpret_cast<T*>(reinterpret_cast<C*>(base) + bytes + lane);
+}
+// A lane number the compiler takes for a new one: the rows that follow from it are computed again instead of being held
+// from the loads to the stores, which the backward pass has no registers for.
+__device__ static inline int anew(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 // Strides below 2^22 bytes and rows below 2^9: the product of two 24-bit numbers.
 __device__ static inline uint32_t offset(uint32_t row, uint32_t stride, uint32_t c) { return __umul24(row, stride) + c; }
@@ -111,22 +132,23 @@ template <class S>
 __device__ static inline void load_rows(typename S::Io::raw* r, const typename S::E* base, uint32_t stride, const Tile<S>& t,
                                         const Place& q) {
   const uint32_t c = (q.on ? q.c : 0) * sizeof(typename S::E);
+  const int tg = anew(q.tg);
 #pragma unroll
   for (int i = 0; i < S::L; ++i)
-    r[i] = S::Io::load(shifted(base, t.base * stride, offset(t.row(q, i), stride, c)));
+    r[i] = S::Io::load(shifted(base, t.base * stride, offset(t.row(tg, i), stride, c)));
 }
 template <class S>
 __device__ static inline void blank_rows(typename S::Io::raw* r, uint32_t with, const Tile<S>& t, const Place& q) {
 #pragma unroll
   for (int i = 0; i < S::L; ++i)
-    if (!t.live(q, i)) r[i] = S::Io::fill(with);
+    if (!t.live(q.tg, i)) r[i] = S::Io::fill(with);
 }
-// To [T,D] contiguous.
+// To [T,D] contiguous; `out` begins at the tile's lowest row.
 template <class S>
-__device__ static inline void store_row(typename S::E* base, uint32_t pitch, const Tile<S>& t, const Place& q, int i,
+__device__ static inline void store_row(typename S::E* out, uint32_t pitch, const Tile<S>& t, const Place& q, int i,
                                         typename S::Io::raw r) {
-  if (t.live(q, i) && q.on)
-    S::Io::store(shifted(base, t.base * pitch, offset(t.row(q, i), pitch, q.c * sizeof(typename S::E))), r);
+  const int tg = anew(q.tg);
+  if (t.live(tg, i) && q.on) S::Io::store(shifted(out, t.base * pitch, offset(t.row(tg, i), pitch, q.c * sizeof(typename S::E))), r);
 }
 // Zero in rows from..to-1 of the tile's span.
 template <class S>
@@ -218,29 +240,92 @@ __device__ static inline void apply_chunks(const float* pairs, int D, int first,
     for (int j = 0; j < N; ++j) h[j] = fmaf(tot.v[k][0][q.across][j], h[j], tot.v[k][1][q.across][j]);
 }
 
-// Forward pass.  FOLD: only the pair of a chunk (first launch of a cut time axis).
-template <class S, bool FOLD, bool SAVE>
+// The pair of every chunk of a cut time axis: forwards the map of the state, BACK the map of R from the chunk's last step to
+// its first.  A lane group takes one run of steps and folds them 8 at a time; nothing is exchanged until all are folded.
+template <class S, bool BACK>
+__global__ __launch_bounds__(WAVES * 64) void fold_kernel(ScanArgs a) {
+  constexpr int N = S::N, U = 8;
+  typedef typename S::E E;
+  typedef typename S::Io Io;
+  __shared__ Totals<S> tot;
+  const Place q = place<S>(a);
+  if (q.chunk == (BACK ? 0 : a.chunks - 1)) return;  // nothing starts behind it
+  const int len = valid_rows(a.lengths, q.b, a.T);
+  const int run = a.per * S::L, first = q.chunk * a.per * S::TILE + q.tg * run, last = min(first + run, len);
+  const E* other = static_cast<const E*>(BACK ? a.dh : a.x) + q.b * (BACK ? a.dh_bs : a.x_bs) + (q.on ? q.c : 0);
+  const E* gb = static_cast<const E*>(a.g) + q.b * a.g_bs + (q.on ? q.c : 0);
+  const int64_t os = BACK ? a.dh_ts : a.x_ts, gs = a.g_ts;
+  float A[N], B[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) A[j] = 1.0f, B[j] = 0.0f;
+  const int steps = max(last - first, 0);
+  for (int k0 = 0; k0 < steps; k0 += U) {
+    typename Io::raw gr[U], vr[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int k = min(k0 + i, steps - 1), p = BACK ? last - 1 - k : first + k;
+      const int64_t row = a.reverse ? len - 1 - p : p;
+      gr[i] = Io::load(shifted(gb, row * gs, 0));
+      vr[i] = Io::load(shifted(other, row * os, 0));
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      float gv[N], v[N];
+      Io::unpack(k0 + i < steps ? gr[i] : Io::fill(S::Type::INF), gv);
+      Io::unpack(k0 + i < steps ? vr[i] : Io::fill(0), v);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        float e;
+        const float w = gate<typename S::Type>(gv[j], e), f = 1.0f - w;
+        A[j] *= f;
+        B[j] = BACK ? f * (B[j] + v[j]) : fmaf(f, B[j], w * v[j]);
+      }
+    }
+  }
+  if constexpr (BACK)
+    wave_scan_back<S>(A, B, q.lane);
+  else
+    wave_scan<S>(A, B, q.lane);
+  if (BACK ? q.lane < S::GROUP : q.lane >= 64 - S::GROUP) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) tot.v[q.wave][0][q.across][j] = A[j], tot.v[q.wave][1][q.across][j] = B[j];
+  }
+  __syncthreads();
+  if (q.tg != 0 || !q.on) return;
+#pragma unroll
+  for (int j = 0; j < N; ++j) A[j] = 1.0f, B[j] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < WAVES; ++k)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float ta = tot.v[BACK ? WAVES - 1 - k : k][0][q.across][j];
+      B[j] = fmaf(ta, B[j], tot.v[BACK ? WAVES - 1 - k : k][1][q.across][j]);
+      A[j] *= ta;
+    }
+  float* pr = a.pairs + ((int64_t)q.b * a.chunks + q.chunk) * 2 * a.D + q.c;
+  store_f32<N>(pr, A);
+  store_f32<N>(pr + a.D, B);
+}
+
+// Forward pass.
+template <class S, bool SAVE>
 __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
   constexpr int N = S::N, L = S::L;
   typedef typename S::E E;
   typedef typename S::Io Io;
   __shared__ Totals<S> tot[2];
   const Place q = place<S>(a);
-  if (FOLD && q.chunk == a.chunks - 1) return;  // nothing starts behind the last chunk
   const int len = valid_rows(a.lengths, q.b, a.T), blocks = ceil_div(a.T, BLOCK);
   const E* xb = static_cast<const E*>(a.x) + q.b * a.x_bs;
   const E* gb = static_cast<const E*>(a.g) + q.b * a.g_bs;
   E* hb = static_cast<E*>(a.h) + (int64_t)q.b * a.T * a.D;
   const uint32_t pitch = a.D * sizeof(E);
 
-  float carry[N], prod[N];  // state in front of the tile; FOLD: the pair so far
+  float carry[N];  // state in front of the tile
 #pragma unroll
-  for (int j = 0; j < N; ++j) carry[j] = 0.0f, prod[j] = 1.0f;
-  if constexpr (!FOLD) {
-    if (a.h0 && q.on) load_f32<N>(a.h0 + (int64_t)q.b * a.D + q.c, carry);
-    if (q.chunk > 0)
-      apply_chunks<S>(a.pairs + (int64_t)q.b * a.chunks * 2 * a.D, a.D, 0, 1, q.chunk, q, tot[1], carry);
-  }
+  for (int j = 0; j < N; ++j) carry[j] = 0.0f;
+  if (a.h0 && q.on) load_f32<N>(a.h0 + (int64_t)q.b * a.D + q.c, carry);
+  if (q.chunk > 0) apply_chunks<S>(a.pairs + (int64_t)q.b * a.chunks * 2 * a.D, a.D, 0, 1, q.chunk, q, tot[1], carry);
 
   const int first = q.chunk * a.per * S::TILE, last = min(first + a.per * S::TILE, a.T);
   int flip = 0;
@@ -249,7 +334,6 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
     const bool keeps = SAVE && p % BLOCK == 0 && p < a.T && q.on;
     float* kept = SAVE ? a.states + ((int64_t)q.b * blocks + p / BLOCK) * a.D + q.c : nullptr;
     if (p0 >= len) {  // behind the end: zero rows, the state stays
-      if constexpr (FOLD) break;
       zero_rows<S>(hb, pitch, p0, len, a.T, q);
       if (keeps) store_f32<N>(kept, carry);
       continue;
@@ -261,7 +345,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
     if (t.count < S::TILE) {  // the same for the workgroup
       blank_rows<S>(gr, S::Type::INF, t, q);
       blank_rows<S>(xr, 0, t, q);
-      if constexpr (!FOLD) zero_rows<S>(hb, pitch, p0, len, a.T, q);
+      zero_rows<S>(hb, pitch, p0, len, a.T, q);
     }
     float f[L][N], v[L][N], A[N], B[N];
 #pragma unroll
@@ -273,8 +357,8 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
       Io::unpack(xr[i], xv);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        float w, fw;
-        gate(gv[j], w, fw);
+        float e;
+        const float w = gate<typename S::Type>(gv[j], e);
         f[i][j] = 1.0f - w;
         v[i][j] = w * xv[j];
         A[j] *= f[i][j];
@@ -289,48 +373,41 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
     __syncthreads();  // the other half of `tot` is written next: one barrier per tile
     float h[N];       // state in front of the wave, then of the lane
 #pragma unroll
-    for (int k = 0; k < WAVES; ++k)
+    for (int k = 0; k < WAVES; ++k) {
+      if (k == q.wave) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) h[j] = carry[j];
+      }
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float ta = tot[flip].v[k][0][q.across][j], tb = tot[flip].v[k][1][q.across][j];
-        if (k == q.wave) h[j] = carry[j];
-        carry[j] = fmaf(ta, carry[j], tb);
-        if (FOLD) prod[j] *= ta;
-      }
-    if constexpr (!FOLD) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float pa = __shfl_up(A[j], S::GROUP, 64), pb = __shfl_up(B[j], S::GROUP, 64);
-        h[j] = q.lane >= S::GROUP ? fmaf(pa, h[j], pb) : h[j];
-      }
-      if (keeps) store_f32<N>(kept, h);
-#pragma unroll
-      for (int i = 0; i < L; ++i) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) h[j] = fmaf(f[i][j], h[j], v[i][j]);
-        store_row<S>(hb, pitch, t, q, i, Io::pack(h));
+        const float ta = tot[flip].v[k][0][q.across][j];
+        carry[j] = fmaf(ta, carry[j], tot[flip].v[k][1][q.across][j]);
       }
     }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float pa = __shfl_up(A[j], S::GROUP, 64), pb = __shfl_up(B[j], S::GROUP, 64);
+      h[j] = q.lane >= S::GROUP ? fmaf(pa, h[j], pb) : h[j];
+    }
+    if (keeps) store_f32<N>(kept, h);
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) h[j] = fmaf(f[i][j], h[j], v[i][j]);
+      store_row<S>(hb, pitch, t, q, i, Io::pack(h));
+    }
   }
-  if (q.tg != 0 || !q.on) return;
-  if constexpr (FOLD) {
-    float* pr = a.pairs + ((int64_t)q.b * a.chunks + q.chunk) * 2 * a.D + q.c;
-    store_f32<N>(pr, prod);
-    store_f32<N>(pr + a.D, carry);
-  } else if (q.chunk == a.chunks - 1) {
-    store_f32<N>(a.h_last + (int64_t)q.b * a.D + q.c, carry);
-  }
+  if (q.tg == 0 && q.on && q.chunk == a.chunks - 1) store_f32<N>(a.h_last + (int64_t)q.b * a.D + q.c, carry);
 }
 
-// Backward pass.  FOLD: only the pair (product of f, folded f dh) of a chunk, from its last step to its first.
-template <class S, bool FOLD>
+// Backward pass.
+template <class S>
 __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a) {
   constexpr int N = S::N, L = S::L;
   typedef typename S::E E;
   typedef typename S::Io Io;
   __shared__ Totals<S> tot[2];
   const Place q = place<S>(a);
-  if (FOLD && q.chunk == 0) return;  // nothing lies in front of the first chunk
   const int len = valid_rows(a.lengths, q.b, a.T), blocks = ceil_div(a.T, BLOCK);
   const E* xb = static_cast<const E*>(a.x) + q.b * a.x_bs;
   const E* gb = static_cast<const E*>(a.g) + q.b * a.g_bs;
@@ -339,24 +416,20 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
   E* dgb = static_cast<E*>(a.dg) + (int64_t)q.b * a.T * a.D;
   const uint32_t pitch = a.D * sizeof(E);
 
-  float carry[N], prod[N];  // R behind the tile; FOLD: the pair so far
+  float carry[N];  // R behind the tile
 #pragma unroll
-  for (int j = 0; j < N; ++j) carry[j] = 0.0f, prod[j] = 1.0f;
-  if constexpr (!FOLD) {
-    if (a.dh_last && q.on) load_f32<N>(a.dh_last + (int64_t)q.b * a.D + q.c, carry);
-    if (q.chunk < a.chunks - 1)
-      apply_chunks<S>(a.pairs + (int64_t)q.b * a.chunks * 2 * a.D, a.D, a.chunks - 1, -1, a.chunks - 1 - q.chunk, q,
-                      tot[1], carry);
-  }
+  for (int j = 0; j < N; ++j) carry[j] = 0.0f;
+  if (a.dh_last && q.on) load_f32<N>(a.dh_last + (int64_t)q.b * a.D + q.c, carry);
+  if (q.chunk < a.chunks - 1)
+    apply_chunks<S>(a.pairs + (int64_t)q.b * a.chunks * 2 * a.D, a.D, a.chunks - 1, -1, a.chunks - 1 - q.chunk, q, tot[1],
+                    carry);
 
   const int first = q.chunk * a.per * S::TILE, last = min(first + a.per * S::TILE, a.T);
   int flip = 0;
   for (int p0 = first + (ceil_div(last - first, S::TILE) - 1) * S::TILE; p0 >= first; p0 -= S::TILE, flip ^= 1) {
     if (p0 >= len) {
-      if constexpr (!FOLD) {
-        zero_rows<S>(dxb, pitch, p0, len, a.T, q);
-        zero_rows<S>(dgb, pitch, p0, len, a.T, q);
-      }
+      zero_rows<S>(dxb, pitch, p0, len, a.T, q);
+      zero_rows<S>(dgb, pitch, p0, len, a.T, q);
       continue;
     }
     const Tile<S> t(p0, len, a.reverse);
@@ -366,18 +439,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
     for (int j = 0; j < N; ++j) h[j] = 0.0f;
     load_rows<S>(gr, gb, a.g_ts, t, q);
     load_rows<S>(dr, db, a.dh_ts, t, q);
-    if constexpr (!FOLD) {
-      load_rows<S>(xr, xb, a.x_ts, t, q);
-      if (q.on) load_f32<N>(a.states_in + ((int64_t)q.b * blocks + p0 / BLOCK) * a.D + q.c, h);
-    }
+    load_rows<S>(xr, xb, a.x_ts, t, q);
+    if (q.on) load_f32<N>(a.states_in + ((int64_t)q.b * blocks + p0 / BLOCK) * a.D + q.c, h);
     if (t.count < S::TILE) {  // the same for the workgroup
       blank_rows<S>(gr, S::Type::INF, t, q);
       blank_rows<S>(dr, 0, t, q);
-      if constexpr (!FOLD) {
-        blank_rows<S>(xr, 0, t, q);
-        zero_rows<S>(dxb, pitch, p0, len, a.T, q);
-        zero_rows<S>(dgb, pitch, p0, len, a.T, q);
-      }
+      blank_rows<S>(xr, 0, t, q);
+      zero_rows<S>(dxb, pitch, p0, len, a.T, q);
+      zero_rows<S>(dgb, pitch, p0, len, a.T, q);
     }
     // s: f w, later dg / G.  A: product of f; B: the forward fold; C: the backward fold of f dh
     float w[L][N], s[L][N], A[N], A2[N], B[N], C[N];
@@ -387,16 +456,18 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
     for (int i = 0; i < L; ++i) {
       float gv[N], xv[N];
       Io::unpack(gr[i], gv);
-      if constexpr (!FOLD) Io::unpack(xr[i], xv);
+      Io::unpack(xr[i], xv);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        gate(gv[j], w[i][j], s[i][j]);
+        float e;
+        w[i][j] = gate<typename S::Type>(gv[j], e);
+        s[i][j] = slope(w[i][j], e);
         A[j] *= 1.0f - w[i][j];
-        if constexpr (!FOLD) B[j] = fmaf(1.0f - w[i][j], B[j], w[i][j] * xv[j]);
+        B[j] = fmaf(1.0f - w[i][j], B[j], w[i][j] * xv[j]);
         forget(w[i][j]);
-        if constexpr (!FOLD) forget(s[i][j]);
+        forget(s[i][j]);
       }
-      if constexpr (!FOLD) forget<S>(xr[i]);
+      forget<S>(xr[i]);
     }
 #pragma unroll
     for (int i = L - 1; i >= 0; --i) {
@@ -404,7 +475,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
       Io::unpack(dr[i], dv);
 #pragma unroll
       for (int j = 0; j < N; ++j) C[j] = (1.0f - w[i][j]) * (C[j] + dv[j]);
-      if constexpr (!FOLD) forget<S>(dr[i]);
+      forget<S>(dr[i]);
     }
 #pragma unroll
     for (int i = 0; i < L; ++i)
@@ -413,74 +484,65 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
 #pragma unroll
     for (int j = 0; j < N; ++j) A2[j] = A[j];
     wave_scan_back<S>(A2, C, q.lane);
-    if constexpr (!FOLD) wave_scan<S>(A, B, q.lane);
+    wave_scan<S>(A, B, q.lane);
     if (q.lane < S::GROUP) {
 #pragma unroll
       for (int j = 0; j < N; ++j) tot[flip].v[q.wave][0][q.across][j] = A2[j], tot[flip].v[q.wave][2][q.across][j] = C[j];
     }
-    if (!FOLD && q.lane >= 64 - S::GROUP) {
+    if (q.lane >= 64 - S::GROUP) {
 #pragma unroll
       for (int j = 0; j < N; ++j) tot[flip].v[q.wave][1][q.across][j] = B[j];
     }
     __syncthreads();
     float R[N];  // gradient behind the wave, then behind the lane
-#pragma unroll
+#pragma unroll 1
     for (int k = WAVES - 1; k >= 0; --k)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const float ta = tot[flip].v[k][0][q.across][j];
         if (k == q.wave) R[j] = carry[j];
         carry[j] = fmaf(ta, carry[j], tot[flip].v[k][2][q.across][j]);
-        if (FOLD) prod[j] *= ta;
       }
-    if constexpr (!FOLD) {
-      for (int k = 0; k < q.wave; ++k)
+#pragma unroll 1
+    for (int k = 0; k < q.wave; ++k)
 #pragma unroll
-        for (int j = 0; j < N; ++j) h[j] = fmaf(tot[flip].v[k][0][q.across][j], h[j], tot[flip].v[k][1][q.across][j]);
+      for (int j = 0; j < N; ++j) h[j] = fmaf(tot[flip].v[k][0][q.across][j], h[j], tot[flip].v[k][1][q.across][j]);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float pa = __shfl_up(A[j], S::GROUP, 64), pb = __shfl_up(B[j], S::GROUP, 64);
+      h[j] = q.lane >= S::GROUP ? fmaf(pa, h[j], pb) : h[j];
+      pa = __shfl_down(A2[j], S::GROUP, 64), pb = __shfl_down(C[j], S::GROUP, 64);
+      R[j] = q.lane < 64 - S::GROUP ? fmaf(pa, R[j], pb) : R[j];
+    }
+    // the states of the lane's steps again
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      float xv[N];
+      Io::unpack(xr[i], xv);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        float pa = __shfl_up(A[j], S::GROUP, 64), pb = __shfl_up(B[j], S::GROUP, 64);
-        h[j] = q.lane >= S::GROUP ? fmaf(pa, h[j], pb) : h[j];
-        pa = __shfl_down(A2[j], S::GROUP, 64), pb = __shfl_down(C[j], S::GROUP, 64);
-        R[j] = q.lane < 64 - S::GROUP ? fmaf(pa, R[j], pb) : R[j];
-      }
-      // the states of the lane's steps again
-#pragma unroll
-      for (int i = 0; i < L; ++i) {
-        float xv[N];
-        Io::unpack(xr[i], xv);
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          s[i][j] *= h[j] - xv[j];
-          h[j] = fmaf(1.0f - w[i][j], h[j], w[i][j] * xv[j]);
-          forget(w[i][j]);
-          forget(s[i][j]);
-        }
-      }
-#pragma unroll
-      for (int i = L - 1; i >= 0; --i) {
-        float dv[N], gx[N], gg[N];
-        Io::unpack(dr[i], dv);
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const float G = dv[j] + R[j];
-          gx[j] = w[i][j] * G;
-          gg[j] = s[i][j] * G;
-          R[j] = (1.0f - w[i][j]) * G;
-        }
-        store_row<S>(dxb, pitch, t, q, i, Io::pack(gx));
-        store_row<S>(dgb, pitch, t, q, i, Io::pack(gg));
+        s[i][j] *= h[j] - xv[j];
+        h[j] = fmaf(1.0f - w[i][j], h[j], w[i][j] * xv[j]);
+        forget(w[i][j]);
+        forget(s[i][j]);
       }
     }
+#pragma unroll
+    for (int i = L - 1; i >= 0; --i) {
+      float dv[N], gx[N], gg[N];
+      Io::unpack(dr[i], dv);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float G = dv[j] + R[j];
+        gx[j] = w[i][j] * G;
+        gg[j] = s[i][j] * G;
+        R[j] = (1.0f - w[i][j]) * G;
+      }
+      store_row<S>(dxb, pitch, t, q, i, Io::pack(gx));
+      store_row<S>(dgb, pitch, t, q, i, Io::pack(gg));
+    }
   }
-  if (q.tg != 0 || !q.on) return;
-  if constexpr (FOLD) {
-    float* pr = a.pairs + ((int64_t)q.b * a.chunks + q.chunk) * 2 * a.D + q.c;
-    store_f32<N>(pr, prod);
-    store_f32<N>(pr + a.D, carry);
-  } else if (q.chunk == 0) {
-    store_f32<N>(a.dh0 + (int64_t)q.b * a.D + q.c, carry);
-  }
+  if (q.tg == 0 && q.on && q.chunk == 0) store_f32<N>(a.dh0 + (int64_t)q.b * a.D + q.c, carry);
 }
 
 // One step of every request: elementwise.
@@ -500,8 +562,8 @@ __global__ __launch_bounds__(256) void step_kernel(const typename IO::elem* x, i
   load_f32<N>(h + b * D + c, hv);
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    float w, fw;
-    gate(gv[j], w, fw);
+    float e;
+    const float w = gate<IO>(gv[j], e);
     hv[j] = fmaf(1.0f - w, hv[j], w * xv[j]);
   }
   Io::store(y + b * D + c, Io::pack(hv));
@@ -554,17 +616,17 @@ int launch(ScanArgs a, int B, size_t ws_bytes, bool backward, hipStream_t s) {
   const dim3 g((unsigned)grid), t(WAVES * 64);
   if (p.chunks > 1) {
     if (backward)
-      scan_backward_kernel<S, true><<<g, t, 0, s>>>(a);
+      fold_kernel<S, true><<<g, t, 0, s>>>(a);
     else
-      scan_kernel<S, true, false><<<g, t, 0, s>>>(a);
+      fold_kernel<S, false><<<g, t, 0, s>>>(a);
     TTSX_LAUNCH_CHECK();
   }
   if (backward)
-    scan_backward_kernel<S, false><<<g, t, 0, s>>>(a);
+    scan_backward_kernel<S><<<g, t, 0, s>>>(a);
   else if (a.states)
-    scan_kernel<S, false, true><<<g, t, 0, s>>>(a);
+    scan_kernel<S, true><<<g, t, 0, s>>>(a);
   else
-    scan_kernel<S, false, false><<<g, t, 0, s>>>(a);
+    scan_kernel<S, false><<<g, t, 0, s>>>(a);
   TTSX_LAUNCH_CHECK();
   return TTSX_OK;
 }
