@@ -16,7 +16,9 @@ masking, attention without location features, Graves attention
 
 Extensions the reference does not have (its `inference` is batch-1 only,
 models.py:661): `inference_batch` decodes B utterances at once with
-per-utterance stop handling and optional length masking.
+per-utterance stop handling and optional length masking; `load_voices` /
+`voice_ids` give every utterance of a batch a low-rank adapter of its own
+beside the shared encoder layer.
 """
 import ctypes
 
@@ -24,7 +26,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
-from . import _lib
+from . import _lib, adapters
 
 
 def _dev_tensor(v, device):
@@ -89,6 +91,8 @@ class Tacotron2:
         self._post_handle = None
         self._enc_handle = None
         self._lstm_handle = None
+        self._voices_src = None         # (down, up, scale) of load_voices, and the same on the device
+        self._voices = None
 
     # ---- torch.nn.Module look-alikes ------------------------------------
     def load_state_dict(self, state_dict, strict=True):
@@ -122,10 +126,39 @@ class Tacotron2:
             self._upload()
         return self
 
+    def load_voices(self, down, up, scale=None):
+        """Voices beside the shared weights (no counterpart in the reference, whose speakers differ by one added embedding,
+        models.py:838-849): V low-rank adapters down [V,R,512], up [V,R,512] of rank 1 to 64 and a factor scale [V].
+        An utterance with voice v is encoded as BiLSTM(c) + scale[v] (c down[v]^T) up[v], c the output of the conv blocks:
+        what it takes is chosen per utterance by `voice_ids` of encode / inference / inference_batch, -1 for the
+        shared weights alone.  `load_voices(None, None)` forgets them."""
+        if down is None and up is None:
+            self._voices_src = self._voices = None
+            return self
+        cpu = [torch.as_tensor(t).detach().float().contiguous() for t in (down, up)]
+        V, R = cpu[0].shape[:2] if cpu[0].dim() == 3 else (0, 0)
+        if V < 1 or not 1 <= R <= adapters.MAX_RANK or any(t.shape != (V, R, 512) for t in cpu):
+            raise ValueError("voices must be down and up [V,R,512] with a rank of 1..%d, got %s and %s"
+                             % (adapters.MAX_RANK, tuple(cpu[0].shape), tuple(cpu[1].shape)))
+        if scale is not None:
+            scale = torch.as_tensor(scale).detach().float().contiguous()
+            if scale.shape != (V,):
+                raise ValueError("scale must hold one factor for each of the %d voices, got %s" % (V, tuple(scale.shape)))
+        self._voices_src = (cpu[0], cpu[1], scale)
+        self._voices = None
+        if self.device.type == "cuda":
+            self._upload_voices()
+        return self
+
+    def _upload_voices(self):
+        if self._voices_src is not None:
+            self._voices = tuple(None if t is None else t.to(self.device) for t in self._voices_src)
+
     def cuda(self, device=None):
         self.device = torch.device("cuda", torch.cuda.current_device() if device is None else device)
         if getattr(self, "_sd_src", None) is not None:
             self._upload()
+        self._upload_voices()
         return self
 
     def to(self, device):
@@ -251,16 +284,19 @@ class Tacotron2:
 
     # ---- forward pieces ----------------------------------------------------
     @torch.no_grad()
-    def encode(self, text, text_lengths=None, speaker_ids=None, rnn_state=None):
+    def encode(self, text, text_lengths=None, speaker_ids=None, rnn_state=None, voice_ids=None):
         """Embedding + Encoder.inference (Tacotron2/TTS/models.py:803-804, 449-454).  The three
         conv blocks (position-major, so the embedding output is consumed as it is) and the BiLSTM
         run in HIP kernels; the embedding lookup is a stock op.  With `text_lengths` every
         utterance is encoded as its unpadded batch-1 run would be.  `speaker_ids` adds the
         speaker embedding (_add_speaker_embedding, :838-849); `rnn_state` = (h, c), each
         [2,B,256], is the BiLSTM state to start from and is overwritten with the final one
-        (Encoder.inference_truncated, :456-464)."""
+        (Encoder.inference_truncated, :456-464).  `voice_ids` names the adapter of `load_voices`
+        each utterance has (-1: none)."""
         lib = _lib.load()
         sd = self._sd
+        if voice_ids is not None and self._voices is None:
+            raise RuntimeError("voice_ids given but no voices are loaded (load_voices)")
         x = F.embedding(text, sd["embedding.weight"]).contiguous()          # [B,T,512]
         B, T, _ = x.shape
         y = torch.empty_like(x)
@@ -279,6 +315,9 @@ class Tacotron2:
                                                               _lib.ptr(out), _lib.ptr(rnn_state[0]),
                                                               _lib.ptr(rnn_state[1]), _lib.current_stream()),
                            "ttsx_encoder_lstm_run_stateful")
+            if voice_ids is not None:
+                down, up, scale = self._voices
+                adapters.adapter_add(out, y, down, up, voice_ids, scale=scale, lengths=lens, out=out)
             if self.num_speakers > 1:
                 if speaker_ids is None:
                     raise RuntimeError(" [!] Model has speaker embedding layer but speaker_id is not provided")
@@ -369,12 +408,12 @@ class Tacotron2:
 
     # ---- public API ----------------------------------------------------------
     @torch.no_grad()
-    def inference(self, text, speaker_ids=None):
+    def inference(self, text, speaker_ids=None, voice_ids=None):
         """Same contract as the reference `Tacotron2.inference`
         (Tacotron2/TTS/models.py:802-813): text LongTensor [B,T] ->
         (decoder_output [B,F,80], postnet_output [B,F,80], alignments [B,T_dec,T],
         stop_tokens [B,T_dec,1])."""
-        out = self.inference_batch(text, speaker_ids=speaker_ids)
+        out = self.inference_batch(text, speaker_ids=speaker_ids, voice_ids=voice_ids)
         return out["decoder_output"], out["postnet_output"], out["alignments"], out["stop_tokens"]
 
     @torch.no_grad()
@@ -412,14 +451,15 @@ class Tacotron2:
         self._memory_truncated = None
 
     @torch.no_grad()
-    def inference_batch(self, text, text_lengths=None, fixed_steps=None, speaker_ids=None):
+    def inference_batch(self, text, text_lengths=None, fixed_steps=None, speaker_ids=None, voice_ids=None):
         """Batched decode.  Each utterance's rows up to n_steps[b] equal what a
-        batch-1 `inference` of that utterance returns; later rows are padding."""
+        batch-1 `inference` of that utterance returns; later rows are padding.  `voice_ids` [B]: the
+        adapter of `load_voices` each utterance has, -1 for none."""
         self._require_device()
         text = torch.as_tensor(text).to(self.device).long()
         if text.dim() != 2:
             raise ValueError("text must be [B, T]")
-        enc = self.encode(text, text_lengths, speaker_ids)
+        enc = self.encode(text, text_lengths, speaker_ids, voice_ids=voice_ids)
         mel, align, stop, n_steps, steps = self.decode(enc, text_lengths, fixed_steps)
         if not fixed_steps and steps == self.decoder.max_decoder_steps and \
                 bool((stop[:, -1] <= self.decoder.stop_threshold).any()):
