@@ -104,12 +104,17 @@ def test_python_refusals_of_the_recurrence():
 
 
 def test_lengths_are_checked_on_the_host():
-    from tts_amd._seq import lengths_on
-    assert lengths_on("f", None, 2, 5, torch.device("cpu")) is None
-    assert lengths_on("f", [0, 5], 2, 5, torch.device("cpu")).dtype == torch.int32
+    from tts_amd._seq import lengths_on, voices_on
+    like = torch.zeros(1)
+    assert lengths_on("f", None, 2, 5, like) is None
+    assert lengths_on("f", [0, 5], 2, 5, like).dtype == torch.int32
     for bad in ([6, 1], [-1, 1], [1], [0.5, 1.0]):
         with pytest.raises(ValueError):
-            lengths_on("f", bad, 2, 5, torch.device("cpu"))
+            lengths_on("f", bad, 2, 5, like)
+    assert voices_on("f", [-1, 4], 2, 5, like).tolist() == [-1, 4]
+    for bad in ([5, 0], [-2, 0]):
+        with pytest.raises(IndexError):
+            voices_on("f", bad, 2, 5, like)
 
 
 def _add(lib, y=ONE, x=ONE, down=ONE, up=ONE, voices=ONE, B=2, T=8, K=16, N=24, R=4, V=3, dtype=0, out=ONE, out_rows=24):

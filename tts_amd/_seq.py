@@ -6,19 +6,19 @@ from . import _lib
 DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
-# What torch.cuda.current_stream() and torch.cuda.device() wrap: a call of the smallest size is bound by the host.
+# What torch.cuda.current_stream() and torch.cuda.current_device() wrap: a call of the smallest size is bound by the host.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _functions = {}
 
 
-def call(name, device, *args):
-    """The entry point `name` with `args` and the current stream of `device`, run on that device."""
+def call(name, index, *args):
+    """The entry point `name` with `args` and the current stream of device `index`, run on that device."""
     fn = _functions.get(name)
     if fn is None:
         fn = _functions[name] = getattr(_lib.load(), name)
-    index = device.index
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -34,23 +34,27 @@ def are_tensors(what, *named):
 
 
 def on_device(what, *named):
-    """All on one GPU, none part of an autograd graph (None stands for an argument left out)."""
-    if torch.is_grad_enabled():
-        for _, t in named:
-            if t is not None and t.requires_grad:
-                raise ValueError("%s records no autograd graph: call it under torch.no_grad(); gradients are a call of "
-                                 "their own" % what)
-    dev = None
+    """The index of the one GPU they are all on; none may be part of an autograd graph (None stands for an argument left
+    out)."""
+    grad, index = torch.is_grad_enabled(), None
     for name, t in named:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise _lib.TtsxError("%s runs on the GPU only: %s is on %s (there is no CPU path)" % (what, name, t.device))
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError("%s: %s is on %s, the others are on %s" % (what, name, t.device, dev))
-    return dev
+        if grad and t.requires_grad:
+            raise ValueError("%s records no autograd graph: call it under torch.no_grad(); gradients are a call of "
+                             "their own" % what)
+        i = t.get_device() if t.is_cuda else -1
+        if index is None:
+            index = i
+        elif i != index:
+            where = [str(t.device) for _, t in named if t is not None]
+            if -1 in (i, index):
+                raise _lib.TtsxError("%s runs on the GPU only: its tensors are on %s (there is no CPU path)"
+                                     % (what, ", ".join(where)))
+            raise ValueError("%s: its tensors are on %s" % (what, ", ".join(where)))
+    if index < 0:
+        raise _lib.TtsxError("%s runs on the GPU only: its tensors are on the CPU (there is no CPU path)" % what)
+    return index
 
 
 def pointer(t):
@@ -65,24 +69,31 @@ def rows(t, furthest=None):
     return t
 
 
-def lengths_on(what, lengths, B, T, device):
-    """Lengths as int32 on the device.  On the device already, they are clamped there by the kernels; on the host they
-    are checked here."""
-    if lengths is None:
-        return None
-    if not isinstance(lengths, torch.Tensor):
-        lengths = torch.as_tensor(lengths)
-    if lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64):
-        raise ValueError("%s: lengths must be int32 or int64 [%d], got %s %s"
-                         % (what, B, lengths.dtype, tuple(lengths.shape)))
-    if not lengths.is_cuda:
-        if B and (int(lengths.min()) < 0 or int(lengths.max()) > T):
-            raise ValueError("%s: lengths must lie in 0..%d" % (what, T))
-    elif lengths.device != device:
-        raise ValueError("%s: lengths is on %s, the others are on %s" % (what, lengths.device, device))
-    elif lengths.dtype == torch.int32 and lengths.is_contiguous():
-        return lengths
-    return lengths.clamp(0, T).to(device=device, dtype=torch.int32).contiguous()
+def _index_tensor(what, name, t, B, like, lowest, highest, error):
+    """[B] int32 on the device of `like`.  On the device already, any number is fine there; on the host they are checked."""
+    if not isinstance(t, torch.Tensor):
+        t = torch.as_tensor(t)
+    if t.dim() != 1 or t.shape[0] != B or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError("%s: %s must be int32 or int64 [%d], got %s %s" % (what, name, B, t.dtype, tuple(t.shape)))
+    if not t.is_cuda:
+        if B and (int(t.min()) < lowest or int(t.max()) > highest):
+            raise error("%s: %s must lie in %d..%d" % (what, name, lowest, highest))
+    elif t.get_device() != like.get_device():
+        raise ValueError("%s: %s is on %s, the others are on %s" % (what, name, t.device, like.device))
+    elif t.dtype == torch.int32 and t.is_contiguous():
+        return t
+    # one beyond either end stands for all numbers there
+    return t.clamp(lowest - 1, highest + 1).to(device=like.device, dtype=torch.int32).contiguous()
+
+
+def lengths_on(what, lengths, B, T, like):
+    """Lengths of a ragged batch: 0..T, clamped to that by the kernels."""
+    return None if lengths is None else _index_tensor(what, "lengths", lengths, B, like, 0, T, ValueError)
+
+
+def voices_on(what, voices, B, V, like):
+    """Voices of a batch: 0..V-1, or -1 (any other number on the device) for none."""
+    return _index_tensor(what, "voices", voices, B, like, -1, V - 1, IndexError)
 
 
 def _span(t):
@@ -97,8 +108,18 @@ def _span(t):
 
 def overlaps(a, b):
     """Whether the two tensors' memory ranges meet (strided tensors may interleave and still count)."""
-    a, b = _span(a), _span(b)
-    return a is not None and b is not None and a[0] < b[1] and b[0] < a[1]
+    return overlapping(a, (b,)) is not None
+
+
+def overlapping(a, others):
+    """The index of the first of `others` whose memory range meets a's, or None."""
+    span = _span(a)
+    if span is not None:
+        for i, t in enumerate(others):
+            s = _span(t)
+            if s is not None and span[0] < s[1] and s[0] < span[1]:
+                return i
+    return None
 
 
 def same_place(a, b):

@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from ._seq import (DTYPES, are_tensors, call, columns_apart, lengths_on, on_device, overlaps, pointer, rows, same_place,
-                   writable_rows)
+                   voices_on, writable_rows)
 
 MAX_RANK = 64                     # TTSX_ADAPTER_MAX_RANK
 MAX_WIDTH = FURTHEST = 1 << 20   # columns, and elements between two rows, of a call
@@ -63,21 +63,6 @@ def _check(what, name, wide, x, down, up, scale):
     return on_device(what, (name, wide), ("x", x), ("down", down), ("up", up), ("scale", scale))
 
 
-def _voices_on(what, voices, B, V, device):
-    if not isinstance(voices, torch.Tensor):
-        voices = torch.as_tensor(voices)
-    if voices.shape != (B,) or voices.dtype not in (torch.int32, torch.int64):
-        raise ValueError("%s: voices must be int32 or int64 [%d], got %s %s" % (what, B, voices.dtype, tuple(voices.shape)))
-    if not voices.is_cuda:
-        if B and (int(voices.min()) < -1 or int(voices.max()) >= V):
-            raise IndexError("%s: voices must lie in -1..%d" % (what, V - 1))
-    elif voices.device != device:
-        raise ValueError("%s: voices is on %s, the others are on %s" % (what, voices.device, device))
-    elif voices.dtype == torch.int32 and voices.is_contiguous():
-        return voices
-    return voices.clamp(-1, V).to(device=device, dtype=torch.int32).contiguous()
-
-
 def adapter_add(y, x, down, up, voices, scale=None, lengths=None, out=None):
     """y [B,T,N] plus each request's adapter applied to x [B,T,K]; y [B,N] and x [B,K] are one position per request.
 
@@ -110,10 +95,10 @@ def adapter_add(y, x, down, up, voices, scale=None, lengths=None, out=None):
             raise ValueError("%s: out overlaps x" % what)
         if overlaps(into, down) or overlaps(into, up):
             raise ValueError("%s: out overlaps an adapter" % what)
-    voices = _voices_on(what, voices, B, V, dev)
-    lengths = lengths_on(what, lengths, B, T, dev)
+    voices = voices_on(what, voices, B, V, x)
+    lengths = lengths_on(what, lengths, B, T, x)
     if into is None:
-        into = torch.empty((B, T, N), dtype=y.dtype, device=dev)
+        into = y.new_empty((B, T, N))
     if B and T and N:
         if K == 0:
             if not in_place:
@@ -142,16 +127,16 @@ def adapter_backward(dy, x, down, up, voices, scale=None, lengths=None):
         dy, x = dy.unsqueeze(1), x.unsqueeze(1)
     B, T, N = dy.shape
     K, (V, R) = x.shape[2], down.shape[:2]
-    voices = _voices_on(what, voices, B, V, dev)
-    lengths = lengths_on(what, lengths, B, T, dev)
-    dx = torch.empty((B, T, K), dtype=x.dtype, device=dev)
+    voices = voices_on(what, voices, B, V, x)
+    lengths = lengths_on(what, lengths, B, T, x)
+    dx = x.new_empty((B, T, K))
     if not (B and T and K and N):
         dx.zero_()
         return dx.squeeze(1) if single else dx, torch.zeros_like(down), torch.zeros_like(up)
     ddown, dup = torch.empty_like(down), torch.empty_like(up)
     dtype = DTYPES[x.dtype]
     need = _workspace_bytes(B, T, K, N, R, dtype)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = x.new_empty((need,), dtype=torch.uint8)
     dy, x = rows(dy, FURTHEST), rows(x, FURTHEST)
     scale = None if scale is None else scale.contiguous()
     ds, xs = dy.stride(), x.stride()

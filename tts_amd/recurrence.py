@@ -22,7 +22,7 @@ import functools
 import torch
 
 from . import _lib
-from ._seq import DTYPES, are_tensors, call, lengths_on, on_device, overlaps, pointer, rows, same_place
+from ._seq import DTYPES, are_tensors, call, lengths_on, on_device, overlapping, pointer, rows, same_place
 
 STATE_BLOCK = 64             # steps between two kept states (TTSX_STATE_BLOCK)
 MAX_CHANNELS = FURTHEST = 1 << 20   # channels, and elements between two rows, of a call
@@ -71,17 +71,17 @@ def gated_scan(x, g, h0=None, lengths=None, reverse=False, save_states=False):
     B, T, D = x.shape
     h0 = _state(what, "h0", h0, B, D)
     dev = on_device(what, ("x", x), ("g", g), ("h0", h0))
-    lengths = lengths_on(what, lengths, B, T, dev)
+    lengths = lengths_on(what, lengths, B, T, x)
     x, g = rows(x, FURTHEST), rows(g, FURTHEST)
-    h = torch.empty((B, T, D), dtype=x.dtype, device=dev)
-    states = torch.empty((B, -(-T // STATE_BLOCK), D), dtype=torch.float32, device=dev) if save_states else None
+    h = x.new_empty((B, T, D))
+    states = x.new_empty((B, -(-T // STATE_BLOCK), D), dtype=torch.float32) if save_states else None
     if B == 0 or T == 0 or D == 0:
-        h_last = torch.zeros(B, D, device=dev) if h0 is None else h0.clone()
+        h_last = x.new_zeros((B, D), dtype=torch.float32) if h0 is None else h0.clone()
         return (h, h_last, states) if save_states else (h, h_last)
-    h_last = torch.empty((B, D), dtype=torch.float32, device=dev)
+    h_last = x.new_empty((B, D), dtype=torch.float32) if h0 is None else torch.empty_like(h0)
     dtype = DTYPES[x.dtype]
     need = _workspace_bytes(B, T, D, dtype, 0)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = x.new_empty((need,), dtype=torch.uint8) if need else None
     xs, gs = x.stride(), g.stride()
     call("ttsx_gated_scan", dev, x.data_ptr(), xs[0], xs[1], g.data_ptr(), gs[0], gs[1], pointer(h0), pointer(lengths),
          B, T, D, dtype, 1 if reverse else 0, h.data_ptr(), h_last.data_ptr(), pointer(states), pointer(ws), need)
@@ -105,16 +105,15 @@ def gated_scan_backward(dh, x, g, states, dh_last=None, lengths=None, reverse=Fa
                          % (what, B, blocks, D, states.dtype, tuple(states.shape)))
     dh_last = _state(what, "dh_last", dh_last, B, D)
     dev = on_device(what, ("x", x), ("g", g), ("dh", dh), ("states", states), ("dh_last", dh_last))
-    lengths = lengths_on(what, lengths, B, T, dev)
+    lengths = lengths_on(what, lengths, B, T, x)
     dh, x, g, states = rows(dh, FURTHEST), rows(x, FURTHEST), rows(g, FURTHEST), states.contiguous()
-    dx = torch.empty((B, T, D), dtype=x.dtype, device=dev)
-    dg = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+    dx, dg = x.new_empty((B, T, D)), x.new_empty((B, T, D))
     if B == 0 or T == 0 or D == 0:
-        return dx, dg, torch.zeros(B, D, device=dev) if dh_last is None else dh_last.clone()
-    dh0 = torch.empty((B, D), dtype=torch.float32, device=dev)
+        return dx, dg, x.new_zeros((B, D), dtype=torch.float32) if dh_last is None else dh_last.clone()
+    dh0 = x.new_empty((B, D), dtype=torch.float32)
     dtype = DTYPES[x.dtype]
     need = _workspace_bytes(B, T, D, dtype, 1)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = x.new_empty((need,), dtype=torch.uint8) if need else None
     xs, gs, ds = x.stride(), g.stride(), dh.stride()
     call("ttsx_gated_scan_backward", dev, dh.data_ptr(), ds[0], ds[1], x.data_ptr(), xs[0], xs[1], g.data_ptr(), gs[0],
          gs[1], states.data_ptr(), pointer(dh_last), pointer(lengths), B, T, D, dtype, 1 if reverse else 0,
@@ -135,16 +134,17 @@ def gated_step(x, g, h, out=None):
         are_tensors(what, ("out", out))
     dev = on_device(what, ("x", x), ("g", g), ("h", h), ("out", out))
     if out is None:
-        out = torch.empty((B, D), dtype=torch.float32, device=dev)
+        out = torch.empty_like(state)
     else:
         if out.shape != (B, D) or out.dtype != torch.float32 or not out.is_contiguous():
             raise ValueError("%s: out must be contiguous float32 [%d, %d], got %s %s"
                              % (what, B, D, out.dtype, tuple(out.shape)))
-        for name, t in (("x", x), ("g", g), ("h", h)):
-            if overlaps(t, out) and not (t is h and same_place(h, out)):
-                raise ValueError("%s: out overlaps %s" % (what, name))
+        others = (x, g) if out is h or same_place(h, out) else (x, g, h)
+        i = overlapping(out, others)
+        if i is not None:
+            raise ValueError("%s: out overlaps %s" % (what, "xgh"[i]))
     x, g = rows(x), rows(g)
-    y = torch.empty((B, D), dtype=x.dtype, device=dev)
+    y = x.new_empty((B, D))
     if B and D:
         call("ttsx_gated_step", dev, x.data_ptr(), x.stride(0), g.data_ptr(), g.stride(0), state.data_ptr(), B, D,
              DTYPES[x.dtype], y.data_ptr(), out.data_ptr())
