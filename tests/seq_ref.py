@@ -57,9 +57,9 @@ def scan_backward(dh, x, g, h0=None, dh_last=None, lengths=None, reverse=False):
 
 
 def scan_error(x, g, h0, T, lengths=None):
-    """Bound on the error of a state kept in fp32.  Per step f carries 3 F32 (the sum 1 + e, the reciprocal's 2) and w
-    (|g| + 6) F32 (the exponent's argument, the exponential, the product), the update 2 more; as w |g| <= 0.28 that is
-    below 8 F32 of the largest magnitude m of x and h0, which bounds h too.  Composing pairs instead of steps
+    """Bound on the error of a state kept in fp32.  Per step w = 1 / (1 + e^g) carries at most (|g| + 6) F32 of itself
+    (the exponent's argument, the exponential, the sum, the reciprocal's 2) and f = 1 - w that and half a unit, the update
+    2 more; as w |g| <= 0.28 that is below 8 F32 of the largest magnitude m of x and h0, which bounds h too.  Composing pairs instead of steps
     rounds each factor at most twice: 16.  The errors of n steps add up while the memory 1 / w lasts."""
     x, g = x.double(), g.double()
     if lengths is not None:

@@ -189,3 +189,45 @@ def test_columns_of_one_buffer():
     for bad in (buf[:1].expand(3, -1, -1), buf.transpose(1, 2), torch.zeros(60).as_strided((2, 3, 8), (24, 4, 1))):
         with pytest.raises(ValueError):
             writable_rows("f", "out", bad)
+
+
+def test_sizes_beyond_the_entry_points_are_refused():
+    """Counts are 32-bit integers at the entry points: a larger one is refused, not cut."""
+    from tts_amd.adapters import adapter_add, adapter_backward
+    from tts_amd.recurrence import gated_scan, gated_step
+    one = torch.zeros(1, 1, 1)
+    for shape, why in (((2 ** 32 + 1, 1, 1), "requests and steps"), ((1, 2 ** 32 + 1, 1), "requests and steps"),
+                       ((1, 1, 2 ** 20 + 1), "channels")):
+        with pytest.raises(ValueError, match=why):
+            gated_scan(one.expand(shape), one.expand(shape))
+    with pytest.raises(ValueError, match="requests and steps"):
+        gated_step(one[0].expand(2 ** 32 + 1, 1), one[0].expand(2 ** 32 + 1, 1), one[0])
+    v = torch.zeros(1, dtype=torch.int32)
+    for call in (adapter_add, adapter_backward):
+        for shape in ((2 ** 32 + 1, 1, 1), (1, 2 ** 32 + 1, 1)):
+            with pytest.raises(ValueError, match="requests and positions"):
+                call(one.expand(shape), one.expand(shape), one, one, v)
+        with pytest.raises(ValueError, match="voices"):
+            call(one, one, one.expand(2 ** 32 + 1, 1, 1), one.expand(2 ** 32 + 1, 1, 1), v)
+        with pytest.raises(ValueError, match="columns"):
+            call(one, one.expand(1, 1, 2 ** 20 + 1), one.expand(1, 1, 2 ** 20 + 1), one, v)
+
+
+@pytest.mark.parametrize("call,bad", [
+    (_scan, dict(B=2 ** 31 - 1, D=64)),              # more threads than a launch counts
+    (_step, dict(B=2 ** 31 - 1, D=64)),
+    (_add, dict(B=2 ** 31 - 1)), (_add_backward, dict(B=2 ** 27, n=1 << 62)),
+])
+def test_launches_beyond_32_bits_are_refused(call, bad):
+    from tts_amd import _lib
+    lib = _lib.load()
+    assert call(lib, **bad) == _lib.ERR_ARG
+    assert "too many" in lib.ttsx_last_error_string().decode()
+
+
+def test_an_empty_batch_takes_empty_lists():
+    from tts_amd._seq import lengths_on, voices_on
+    like = torch.zeros(1)
+    assert lengths_on("f", [], 0, 5, like).shape == voices_on("f", [], 0, 5, like).shape == (0,)
+    with pytest.raises(ValueError):
+        lengths_on("f", 3, 1, 5, like)

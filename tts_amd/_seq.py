@@ -73,6 +73,7 @@ def _index_tensor(what, name, t, B, like, lowest, highest, error):
     """[B] int32 on the device of `like`.  On the device already, any number is fine there; on the host they are checked."""
     if not isinstance(t, torch.Tensor):
         t = torch.as_tensor(t)
+        t = t if t.numel() else t.int()         # an empty list has no type of its own
     if t.dim() != 1 or t.shape[0] != B or t.dtype not in (torch.int32, torch.int64):
         raise ValueError("%s: %s must be int32 or int64 [%d], got %s %s" % (what, name, B, t.dtype, tuple(t.shape)))
     if not t.is_cuda:

@@ -25,6 +25,8 @@ from ._seq import (DTYPES, are_tensors, call, columns_apart, lengths_on, on_devi
 
 MAX_RANK = 64                     # TTSX_ADAPTER_MAX_RANK
 MAX_WIDTH = FURTHEST = 1 << 20   # columns, and elements between two rows, of a call
+MAX_ROWS = 1 << 30                # positions, and requests
+MAX_VOICES = 1 << 24
 
 
 @functools.lru_cache(maxsize=512)
@@ -49,7 +51,11 @@ def _check(what, name, wide, x, down, up, scale):
                          % (what, K, N, tuple(down.shape), tuple(up.shape)))
     if max(K, N) > MAX_WIDTH:
         raise ValueError("%s: at most %d columns, got %d and %d" % (what, MAX_WIDTH, K, N))
+    if x.shape[0] > MAX_ROWS or x.shape[-2] > MAX_ROWS:
+        raise ValueError("%s: at most %d requests and positions, got %s" % (what, MAX_ROWS, tuple(x.shape)))
     V, R = down.shape[:2]
+    if V > MAX_VOICES:
+        raise ValueError("%s: at most %d voices, got %d" % (what, MAX_VOICES, V))
     if not 1 <= R <= MAX_RANK or V < 1:
         raise ValueError("%s: the rank must lie in 1..%d, with at least one voice, got down %s"
                          % (what, MAX_RANK, tuple(down.shape)))
@@ -93,7 +99,7 @@ def adapter_add(y, x, down, up, voices, scale=None, lengths=None, out=None):
             raise ValueError("%s: out overlaps y" % what)
         if overlaps(into, x) and not columns_apart(into, x):
             raise ValueError("%s: out overlaps x" % what)
-        if overlaps(into, down) or overlaps(into, up):
+        if overlaps(into, down) or overlaps(into, up) or (scale is not None and overlaps(into, scale)):
             raise ValueError("%s: out overlaps an adapter" % what)
     voices = voices_on(what, voices, B, V, x)
     lengths = lengths_on(what, lengths, B, T, x)

@@ -651,7 +651,7 @@ int padded_rank(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : 64; }
 template <class IO, int RP, int WV, bool ADD>
 int launch_waves(AddArgs a, int64_t tiles, int splits, hipStream_t s) {
   a.splits = splits;
-  TTSX_ARG(tiles * splits <= 0x7fffffff, "ttsx_adapter: too many rows");
+  TTSX_ARG(tiles * splits <= most_workgroups(WV * 64), "ttsx_adapter: too many rows");
   adapter_kernel<IO, RP, WV, ADD><<<(unsigned)(tiles * splits), WV * 64, 0, s>>>(a);
   TTSX_LAUNCH_CHECK();
   return TTSX_OK;
@@ -709,14 +709,14 @@ int run_backward(AddArgs a, const BackPlan& p, int B, float* ws, void* ddown, vo
   o.du = du, o.u = u, o.voices = a.voices, o.lengths = a.lengths, o.part = part;
   o.T = a.T, o.K = a.second.K, o.N = a.first.K, o.V = a.V, o.chunks = p.chunks, o.span = p.span, o.tiles = ceil_div(a.T, ROWS);
   const int64_t grid = (int64_t)B * p.chunks * (ceil_div(o.K, 16 * IO::VEC) + ceil_div(o.N, 16 * IO::VEC));
-  TTSX_ARG(grid <= 0x7fffffff, "ttsx_adapter_backward: too many rows");
+  TTSX_ARG(grid <= most_workgroups(WAVES * 64), "ttsx_adapter_backward: too many rows");
   outer_kernel<IO, RP><<<(unsigned)grid, WAVES * 64, 0, s>>>(o);
   TTSX_LAUNCH_CHECK();
   GatherArgs g{};
   g.part = part, g.voices = a.voices, g.lengths = a.lengths, g.ddown = ddown, g.dup = dup;
   g.B = B, g.T = a.T, g.K = o.K, g.N = o.N, g.R = a.R, g.RP = RP, g.chunks = p.chunks, g.span = p.span;
   const int64_t outs = (int64_t)a.V * a.R * ceil_div(o.K + o.N, LISTED * 4);
-  TTSX_ARG(outs <= 0x7fffffff, "ttsx_adapter_backward: too many voices");
+  TTSX_ARG(outs <= most_workgroups(LISTED), "ttsx_adapter_backward: too many voices");
   gather_kernel<IO><<<(unsigned)outs, LISTED, 0, s>>>(g);
   TTSX_LAUNCH_CHECK();
   return TTSX_OK;

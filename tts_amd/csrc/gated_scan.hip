@@ -612,7 +612,7 @@ int launch(ScanArgs a, int B, size_t ws_bytes, bool backward, hipStream_t s) {
   a.cols = p.cols, a.chunks = p.chunks, a.per = p.per;
   TTSX_ARG(p.chunks == 1 || (a.pairs && ws_bytes >= pairs_bytes<S>(B, a.T, a.D)), "%s: workspace too small", name);
   const int64_t grid = (int64_t)B * p.cols * p.chunks;
-  TTSX_ARG(grid <= 0x7fffffff, "%s: too many channels", name);
+  TTSX_ARG(grid <= most_workgroups(WAVES * 64), "%s: too many requests of so many channels", name);
   const dim3 g((unsigned)grid), t(WAVES * 64);
   if (p.chunks > 1) {
     if (backward)
@@ -655,7 +655,7 @@ int launch_step(const void* x, int64_t x_bs, const void* g, int64_t g_bs, const 
                 float* h_out, hipStream_t s) {
   typedef typename IO::elem E;
   const int64_t grid = ((int64_t)B * (D / N) + 255) / 256;
-  TTSX_ARG(grid <= 0x7fffffff, "ttsx_gated_step: too many channels");
+  TTSX_ARG(grid <= most_workgroups(256), "ttsx_gated_step: too many requests of so many channels");
   step_kernel<IO, N><<<(unsigned)grid, 256, 0, s>>>(static_cast<const E*>(x), x_bs, static_cast<const E*>(g), g_bs, h, B,
                                                     D, static_cast<E*>(y), h_out);
   TTSX_LAUNCH_CHECK();

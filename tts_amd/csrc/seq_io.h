@@ -174,6 +174,9 @@ __device__ static inline void store_f32_some(float* p, int n, const float* v) {
     if (i < n) p[i] = v[i];
 }
 
+// The widest grid of workgroups of that many threads: a launch counts its threads in 32 bits.
+constexpr int64_t most_workgroups(int threads) { return 0xffffffffLL / threads; }
+
 // A row of a ragged batch is valid below this.
 __device__ static inline int valid_rows(const int32_t* lengths, int b, int T) {
   return lengths ? min(max(lengths[b], 0), T) : T;

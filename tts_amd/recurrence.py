@@ -26,6 +26,7 @@ from ._seq import DTYPES, are_tensors, call, lengths_on, on_device, overlapping,
 
 STATE_BLOCK = 64             # steps between two kept states (TTSX_STATE_BLOCK)
 MAX_CHANNELS = FURTHEST = 1 << 20   # channels, and elements between two rows, of a call
+MAX_STEPS = 1 << 30          # steps, and requests
 
 
 @functools.lru_cache(maxsize=512)
@@ -45,6 +46,8 @@ def _values_and_gates(what, x, g, axes):
         raise ValueError("%s: x and g must both be float32, bfloat16 or float16, got %s and %s" % (what, x.dtype, g.dtype))
     if x.shape[-1] > MAX_CHANNELS:
         raise ValueError("%s: at most %d channels, got %d" % (what, MAX_CHANNELS, x.shape[-1]))
+    if x.shape[0] > MAX_STEPS or x.shape[-2] > MAX_STEPS:
+        raise ValueError("%s: at most %d requests and steps, got %s" % (what, MAX_STEPS, tuple(x.shape)))
 
 
 def _state(what, name, t, B, D):

@@ -27,6 +27,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib, adapters
+from ._seq import voices_on
 
 
 def _dev_tensor(v, device):
@@ -130,7 +131,7 @@ class Tacotron2:
         """Voices beside the shared weights (no counterpart in the reference, whose speakers differ by one added embedding,
         models.py:838-849): V low-rank adapters down [V,R,512], up [V,R,512] of rank 1 to 64 and a factor scale [V].
         An utterance with voice v is encoded as BiLSTM(c) + scale[v] (c down[v]^T) up[v], c the output of the conv blocks:
-        what it takes is chosen per utterance by `voice_ids` of encode / inference / inference_batch, -1 for the
+        what it takes is chosen per utterance by `voice_ids` of encode and the inference calls, -1 for the
         shared weights alone.  `load_voices(None, None)` forgets them."""
         if down is None and up is None:
             self._voices_src = self._voices = None
@@ -299,6 +300,8 @@ class Tacotron2:
             raise RuntimeError("voice_ids given but no voices are loaded (load_voices)")
         x = F.embedding(text, sd["embedding.weight"]).contiguous()          # [B,T,512]
         B, T, _ = x.shape
+        if voice_ids is not None:       # refused before anything runs: rnn_state is updated on the way
+            voice_ids = voices_on("encode", voice_ids, B, self._voices[0].shape[0], x)
         y = torch.empty_like(x)
         lens = None
         if text_lengths is not None:
@@ -417,7 +420,7 @@ class Tacotron2:
         return out["decoder_output"], out["postnet_output"], out["alignments"], out["stop_tokens"]
 
     @torch.no_grad()
-    def inference_truncated(self, text, speaker_ids=None):
+    def inference_truncated(self, text, speaker_ids=None, voice_ids=None):
         """Same contract as the reference `Tacotron2.inference_truncated`
         (Tacotron2/TTS/models.py:815-829): the encoder BiLSTM state (:456-464), the decoder's
         LSTM states and context (:675-686) and the fed-back frame survive from call to call;
@@ -435,7 +438,7 @@ class Tacotron2:
         if first:
             self._rnn_state = (torch.zeros(2, 1, 256, device=self.device), torch.zeros(2, 1, 256, device=self.device))
             self._memory_truncated = torch.zeros(1, 80, device=self.device)
-        enc = self.encode(text, None, speaker_ids, self._rnn_state)
+        enc = self.encode(text, None, speaker_ids, self._rnn_state, voice_ids)
         mel, align, stop, n_steps, steps = self.decode(enc, None, None, keep_states=not first,
                                                        memory=self._memory_truncated)
         if steps == self.decoder.max_decoder_steps and float(stop[0, -1]) <= self.decoder.stop_threshold:
