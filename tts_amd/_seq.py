@@ -29,7 +29,7 @@ def call(name, index, *args):
 
 def are_tensors(what, *named):
     for name, t in named:
-        if not isinstance(t, torch.Tensor):
+        if type(t) is not torch.Tensor and not isinstance(t, torch.Tensor):
             raise ValueError("%s: %s must be a tensor, got %s" % (what, name, type(t).__name__))
 
 
@@ -98,6 +98,9 @@ def voices_on(what, voices, B, V, like):
 
 
 def _span(t):
+    if t.is_contiguous():
+        n, first = t.numel(), t.data_ptr()
+        return (first, first + n * t.element_size()) if n else None
     last = 1
     for n, stride in zip(t.shape, t.stride()):
         if n == 0:
@@ -124,25 +127,27 @@ def overlapping(a, others):
 
 
 def same_place(a, b):
-    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
+    return a is b or a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
 
 
 def columns_apart(a, b):
-    """Whether two [B,T,n] tensors are different columns of the same rows (slices of one buffer)."""
-    if a.stride()[:2] != b.stride()[:2] or a.shape[:2] != b.shape[:2] or a.element_size() != b.element_size():
+    """Whether two [...,n] tensors are different columns of the same rows (slices of one buffer)."""
+    if a.stride()[:-1] != b.stride()[:-1] or a.shape[:-1] != b.shape[:-1] or a.element_size() != b.element_size():
         return False
     d = (b.data_ptr() - a.data_ptr()) // a.element_size()
-    first, second = (a.shape[2], b.shape[2]) if d >= 0 else (b.shape[2], a.shape[2])
-    pitch = min([s for s, n in zip(a.stride()[:2], a.shape[:2]) if n > 1] or [abs(d) + second])
+    first, second = (a.shape[-1], b.shape[-1]) if d >= 0 else (b.shape[-1], a.shape[-1])
+    pitch = min([s for s, n in zip(a.stride()[:-1], a.shape[:-1]) if n > 1] or [abs(d) + second])
     return first <= abs(d) and abs(d) + second <= pitch
 
 
 def writable_rows(what, name, t):
-    """Refuses an output [B,T,n] whose rows are not contiguous or share memory."""
-    if t.stride(2) != 1 and t.shape[2] > 1:
+    """Refuses an output [...,n] whose rows are not contiguous or share memory."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError("%s: the last axis of %s must be contiguous" % (what, name))
-    need = t.shape[2]
-    for stride, n in sorted((s, n) for s, n in zip(t.stride()[:2], t.shape[:2]) if n > 1):
+    if t.is_contiguous():
+        return
+    need = t.shape[-1]
+    for stride, n in sorted((s, n) for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
         if stride < need:
             raise ValueError("%s: rows of %s share memory" % (what, name))
         need = stride * (n - 1) + need

@@ -20,7 +20,7 @@ import functools
 import torch
 
 from . import _lib
-from ._seq import (DTYPES, are_tensors, call, columns_apart, lengths_on, on_device, overlaps, pointer, rows, same_place,
+from ._seq import (DTYPES, are_tensors, call, columns_apart, lengths_on, on_device, overlapping, overlaps, pointer, rows, same_place,
                    voices_on, writable_rows)
 
 MAX_RANK = 64                     # TTSX_ADAPTER_MAX_RANK
@@ -42,31 +42,44 @@ def _check(what, name, wide, x, down, up, scale):
     are_tensors(what, (name, wide), ("x", x), ("down", down), ("up", up))
     if scale is not None:
         are_tensors(what, ("scale", scale))
-    if wide.dim() not in (2, 3) or x.shape[:-1] != wide.shape[:-1]:
+    shape, x_shape, d_shape, u_shape = wide.shape, x.shape, down.shape, up.shape
+    if len(shape) not in (2, 3) or len(x_shape) != len(shape) or x_shape[0] != shape[0] or x_shape[-2] != shape[-2]:
         raise ValueError("%s: %s [B,T,N] and x [B,T,K] (or [B,N] and [B,K]) must agree, got %s and %s"
                          % (what, name, tuple(wide.shape), tuple(x.shape)))
-    K, N = x.shape[-1], wide.shape[-1]
-    if down.dim() != 3 or up.dim() != 3 or down.shape[:2] != up.shape[:2] or down.shape[2] != K or up.shape[2] != N:
+    K, N = x_shape[-1], shape[-1]
+    if (len(d_shape) != 3 or len(u_shape) != 3 or d_shape[0] != u_shape[0] or d_shape[1] != u_shape[1]
+            or d_shape[2] != K or u_shape[2] != N):
         raise ValueError("%s: down and up must be [V,R,%d] and [V,R,%d], got %s and %s"
                          % (what, K, N, tuple(down.shape), tuple(up.shape)))
     if max(K, N) > MAX_WIDTH:
         raise ValueError("%s: at most %d columns, got %d and %d" % (what, MAX_WIDTH, K, N))
-    if x.shape[0] > MAX_ROWS or x.shape[-2] > MAX_ROWS:
-        raise ValueError("%s: at most %d requests and positions, got %s" % (what, MAX_ROWS, tuple(x.shape)))
-    V, R = down.shape[:2]
+    if shape[0] > MAX_ROWS or shape[-2] > MAX_ROWS:
+        raise ValueError("%s: at most %d requests and positions, got %s" % (what, MAX_ROWS, tuple(shape)))
+    V, R, _ = d_shape
     if V > MAX_VOICES:
         raise ValueError("%s: at most %d voices, got %d" % (what, MAX_VOICES, V))
     if not 1 <= R <= MAX_RANK or V < 1:
         raise ValueError("%s: the rank must lie in 1..%d, with at least one voice, got down %s"
                          % (what, MAX_RANK, tuple(down.shape)))
-    if x.dtype not in DTYPES or not x.dtype == wide.dtype == down.dtype == up.dtype:
+    dtype = x.dtype
+    if dtype not in DTYPES or not dtype == wide.dtype == down.dtype == up.dtype:
         raise ValueError("%s: %s, x, down and up must all be float32, bfloat16 or float16, got %s, %s, %s and %s"
                          % (what, name, wide.dtype, x.dtype, down.dtype, up.dtype))
     if not down.is_contiguous() or not up.is_contiguous():
         raise ValueError("%s: down and up must be contiguous" % what)
     if scale is not None and (scale.shape != (V,) or scale.dtype != torch.float32):
         raise ValueError("%s: scale must be float32 [%d], got %s %s" % (what, V, scale.dtype, tuple(scale.shape)))
-    return on_device(what, (name, wide), ("x", x), ("down", down), ("up", up), ("scale", scale))
+    dev = on_device(what, (name, wide), ("x", x), ("down", down), ("up", up), ("scale", scale))
+    return dev, shape[0], shape[1] if len(shape) == 3 else 1, K, N, R, V
+
+
+def _placed(t, keep=False):
+    """t as an entry point takes it, with its batch and row strides (a single position has one row); `keep`: where it is."""
+    single = t.dim() == 2
+    if not keep:
+        t = rows(t, None if single else FURTHEST)
+    strides = t.stride()
+    return t, strides[0], 0 if single else strides[1]
 
 
 def adapter_add(y, x, down, up, voices, scale=None, lengths=None, out=None):
@@ -77,48 +90,37 @@ def adapter_add(y, x, down, up, voices, scale=None, lengths=None, out=None):
     lengths[b] stay y's and x is not read there.  `out` takes the result; out=y works in place and leaves rows without
     an adapter untouched.  The result has y's type, rounded once."""
     what = "adapter_add"
-    dev = _check(what, "y", y, x, down, up, scale)
-    single = y.dim() == 2
-    into = None
+    dev, B, T, K, N, R, V = _check(what, "y", y, x, down, up, scale)
+    in_place = False
     if out is not None:
         are_tensors(what, ("out", out))
         on_device(what, ("y", y), ("out", out))
         if out.shape != y.shape or out.dtype != y.dtype:
             raise ValueError("%s: out must be %s %s like y, got %s %s"
                              % (what, y.dtype, tuple(y.shape), out.dtype, tuple(out.shape)))
-        into = out.unsqueeze(1) if single else out
-    if single:
-        y, x = y.unsqueeze(1), x.unsqueeze(1)
-    B, T, N = y.shape
-    K, (V, R) = x.shape[2], down.shape[:2]
-    in_place = False
-    if into is not None:
-        writable_rows(what, "out", into)
-        in_place = same_place(into, y)
-        if not in_place and overlaps(into, y) and not columns_apart(into, y):
+        writable_rows(what, "out", out)
+        in_place = same_place(out, y)
+        if not in_place and overlaps(out, y) and not columns_apart(out, y):
             raise ValueError("%s: out overlaps y" % what)
-        if overlaps(into, x) and not columns_apart(into, x):
+        if overlaps(out, x) and not columns_apart(out, x):
             raise ValueError("%s: out overlaps x" % what)
-        if overlaps(into, down) or overlaps(into, up) or (scale is not None and overlaps(into, scale)):
+        if overlapping(out, (down, up) if scale is None else (down, up, scale)) is not None:
             raise ValueError("%s: out overlaps an adapter" % what)
     voices = voices_on(what, voices, B, V, x)
     lengths = lengths_on(what, lengths, B, T, x)
-    if into is None:
-        into = y.new_empty((B, T, N))
+    if out is None:
+        out = y.new_empty(y.shape)
     if B and T and N:
         if K == 0:
             if not in_place:
-                into.copy_(y)
+                out.copy_(y)
         else:
-            if not in_place:
-                y = rows(y, FURTHEST)
-            x = rows(x, FURTHEST)
+            (y, yb, yt), (x, xb, xt), (_, ob, ot) = _placed(y, in_place), _placed(x), _placed(out, True)
             scale = None if scale is None else scale.contiguous()
-            ys, xs, os = y.stride(), x.stride(), into.stride()
-            call("ttsx_adapter_add", dev, y.data_ptr(), ys[0], ys[1], x.data_ptr(), xs[0], xs[1], down.data_ptr(),
-                 up.data_ptr(), voices.data_ptr(), pointer(scale), pointer(lengths), B, T, K, N, R, V, DTYPES[y.dtype],
-                 into.data_ptr(), os[0], os[1])
-    return out if out is not None else into.squeeze(1) if single else into
+            call("ttsx_adapter_add", dev, y.data_ptr(), yb, yt, x.data_ptr(), xb, xt, down.data_ptr(), up.data_ptr(),
+                 voices.data_ptr(), pointer(scale), pointer(lengths), B, T, K, N, R, V, DTYPES[y.dtype], out.data_ptr(), ob,
+                 ot)
+    return out
 
 
 def adapter_backward(dy, x, down, up, voices, scale=None, lengths=None):
@@ -127,26 +129,19 @@ def adapter_backward(dy, x, down, up, voices, scale=None, lengths=None):
     [V,R,K] and dup [V,R,N] of their inputs' type: sums over all rows of a voice, kept in float32 and in a fixed order,
     so that two runs agree to the bit.  `scale` is a constant."""
     what = "adapter_backward"
-    dev = _check(what, "dy", dy, x, down, up, scale)
-    single = dy.dim() == 2
-    if single:
-        dy, x = dy.unsqueeze(1), x.unsqueeze(1)
-    B, T, N = dy.shape
-    K, (V, R) = x.shape[2], down.shape[:2]
+    dev, B, T, K, N, R, V = _check(what, "dy", dy, x, down, up, scale)
     voices = voices_on(what, voices, B, V, x)
     lengths = lengths_on(what, lengths, B, T, x)
-    dx = x.new_empty((B, T, K))
+    dx = x.new_empty(x.shape)
     if not (B and T and K and N):
-        dx.zero_()
-        return dx.squeeze(1) if single else dx, torch.zeros_like(down), torch.zeros_like(up)
+        return dx.zero_(), torch.zeros_like(down), torch.zeros_like(up)
     ddown, dup = torch.empty_like(down), torch.empty_like(up)
     dtype = DTYPES[x.dtype]
     need = _workspace_bytes(B, T, K, N, R, dtype)
     ws = x.new_empty((need,), dtype=torch.uint8)
-    dy, x = rows(dy, FURTHEST), rows(x, FURTHEST)
+    (dy, db, dt), (x, xb, xt) = _placed(dy), _placed(x)
     scale = None if scale is None else scale.contiguous()
-    ds, xs = dy.stride(), x.stride()
-    call("ttsx_adapter_backward", dev, dy.data_ptr(), ds[0], ds[1], x.data_ptr(), xs[0], xs[1], down.data_ptr(),
+    call("ttsx_adapter_backward", dev, dy.data_ptr(), db, dt, x.data_ptr(), xb, xt, down.data_ptr(),
          up.data_ptr(), voices.data_ptr(), pointer(scale), pointer(lengths), B, T, K, N, R, V, dtype, dx.data_ptr(),
          ddown.data_ptr(), dup.data_ptr(), ws.data_ptr(), need)
-    return dx.squeeze(1) if single else dx, ddown, dup
+    return dx, ddown, dup

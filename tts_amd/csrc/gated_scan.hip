@@ -587,14 +587,19 @@ bool wide(int D) {
 struct Plan {
   int cols, chunks, per;
 };
-// How the time axis is cut: enough workgroups to fill 256 CUs four times over, one tile at least to each.
+// How the time axis is cut: enough workgroups to fill 256 CUs four times over, one tile at least to each.  It is not cut
+// where that loses: from one workgroup per CU on, since the fold reads everything once more (requests of 800 x 512 fp32,
+// us uncut / cut: 16 of them 21 / 25, 24 26 / 34, 32 33 / 46; below, 8 requests 17 / 16, 4 17 / 12; the backward pass 34 / 35,
+// 41 / 47, 50 / 59; 27 / 20, 26 / 16), and up to three tiles, since a second launch costs the host 4 us (1 x 300 x 512 fp32
+// 10.1 / 14.1 us a call, backwards 13.1 / 17.3).
+constexpr int ENOUGH = 256, FEW_TILES = 3, FULL = 1024;
 template <class S>
 Plan plan(int B, int T, int D) {
   Plan p;
   const int tiles = ceil_div(T, S::TILE);
   p.cols = ceil_div(D, S::GROUP * S::N);
   const int64_t rows = (int64_t)B * p.cols;
-  const int want = (int)(rows >= 1024 ? 1 : 1024 / rows);
+  const int want = (int)(rows >= ENOUGH || tiles <= FEW_TILES ? 1 : FULL / rows);
   p.per = ceil_div(tiles, want < tiles ? want : tiles);
   p.chunks = ceil_div(tiles, p.per);
   return p;
