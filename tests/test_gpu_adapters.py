@@ -344,3 +344,15 @@ def test_an_adapted_projection_in_front_of_the_recurrence():
     for g, (w, bound) in zip((dx, ddown, dup), adapter_backward(d, x, down, up, voices, lengths=lengths)):
         # d itself is off by `tol` of its largest value; `bound` holds the sums of magnitudes in units of about K F32
         assert _excess(g, w, tol * float(d.abs().max()) * (1 + bound / (4 * F32))) <= 0
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("size", [(40, 130, 80, 260, 12, 3), (30, 200, 264, 90, 30, 4), (50, 100, 96, 140, 64, 2)], ids=str)
+def test_middling_batches(size, dtype):
+    """Between few tiles, which are cut into halves, and many, which get four waves each."""
+    from tts_amd.adapters import adapter_add
+    y, x, down, up, voices, scale, lengths = _inputs(*size, dtype, 9)
+    want, tol = adapter(y, x, down, up, voices, scale, lengths)
+    out = adapter_add(*_cuda(y, x, down, up, voices), scale=scale.cuda(), lengths=lengths.cuda())
+    assert _excess(out, want, tol * (1 + half_step(dtype)) + _rounding(dtype, want)) <= 0
+    _check_backward(size, dtype, 10)

@@ -7,7 +7,7 @@
 // A and B both have their long axis contiguous, so "contract the long axis" and "expand from R" are one kernel each way:
 // dx is the same call as the forward pass with dy in the place of x and the two matrices swapped.
 //
-// One launch does both products of a tile of 32 rows of one request: the four waves share the long axis of the first
+// One launch does both products of a tile of 32 (or 16) rows of one request: the four waves share the long axis of the first
 // (each streams x and A from memory straight into matrix operands), the partial sums meet in LDS, and then the waves
 // take blocks of 16 VEC output columns each, read B once per block, and add to y as they write.  u = x A^T never
 // leaves the chip, and y is read and written once: the launch is bound by x, y and out.
@@ -28,7 +28,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 template <class IO>
 using Full = Lane<IO, IO::VEC>;  // 16 bytes of a lane
 
-constexpr int ROWS = 32;  // rows of a tile: two matrix fragments
+constexpr int ROWS = 32;  // rows of a tile of kept hidden values; the first kernel takes them in one piece or in halves
 
 // A first product: x [.,K] of a request's rows with the voice's matrix m [R,K].
 struct Product {
@@ -88,16 +88,16 @@ __device__ static inline int voice_of(const int32_t* voices, int b, int V) {
   return v >= 0 && v < V ? v : -1;
 }
 
-// u of a tile, as the matrix operand of the second product: [ROWS][RP] fp32, or two 16-bit planes and a factor per row.
-template <class IO, int RP>
+// u of a tile, as the matrix operand of the second product: [H][RP] fp32, or two 16-bit planes and a factor per row.
+template <class IO, int RP, int H>
 struct Hidden {
   typedef typename IO::elem E;
-  E hi[ROWS][RP + 8], lo[ROWS][RP + 8];
-  float factor[ROWS];
+  E hi[H][RP + 8], lo[H][RP + 8];
+  float factor[H];
 };
-template <int RP>
-struct Hidden<IoF32, RP> {
-  float u[ROWS][RP + 4];
+template <int RP, int H>
+struct Hidden<IoF32, RP, H> {
+  float u[H][RP + 4];
 };
 
 // Rank of a lane's i-th row of B: 16-bit types take 8 ranks at a time (up to rank 16 the upper half of the lanes has
@@ -127,6 +127,11 @@ __device__ static inline void keep_hidden(float* keep, int64_t tile, int row, in
       at[(row >> 2 & 1) * 256 + lane * 4 + (row & 3)] = u[c];
     }
   }
+}
+// Rows 16 .. 31 of a tile whose request ends in front of them: zero.
+template <int RP>
+__device__ static inline void keep_no_upper(float* keep, int64_t tile, int thread, int threads) {
+  for (int i = thread; i < RP * 16; i += threads) keep[tile * RP * 32 + i / 128 * 256 + 128 + i % 128] = 0.0f;
 }
 template <int RP>
 __device__ static inline void hidden_rows(const float* keep, int64_t tile, int j, int lane, u32x4* r) {
@@ -185,10 +190,10 @@ __device__ static inline void quad_transpose(u32x4* r, int lane) {
 // an instruction).  So four loads bring four rows each, 16 neighbouring lanes to a row, and the lanes' quads are
 // transposed: lane 16 q + r then holds chunks 4 q .. 4 q + 3 of 16 bytes of row r, one per register, the same of x and of
 // A.  Rows and ranks that do not exist repeat the last one and are dropped in the sum.
-template <class IO, int RP, int WV>
+template <class IO, int RP, int WV, int MF>
 __device__ static inline void first_product(const Product& p, const typename IO::elem* xb, int v, int R, int live, int wave,
-                                            int lane, float (*part)[ROWS][RP + 1]) {
-  constexpr int VEC = IO::VEC, NJ = RP / 16, STEP = VEC * 16, MF = ROWS / 16;
+                                            int lane, float (*part)[16 * MF][RP + 1]) {
+  constexpr int VEC = IO::VEC, NJ = RP / 16, STEP = VEC * 16;
   typedef typename IO::elem E;
   typedef Full<IO> Io;
   const E* A = static_cast<const E*>(p.m) + (int64_t)v * R * p.K;
@@ -245,8 +250,8 @@ __device__ static inline void first_product(const Product& p, const typename IO:
 }
 
 // Ranks c0.. of row r of s u, from the waves' shares; zero where the row or the rank does not exist.
-template <int RP, int WV>
-__device__ static inline void sum_shares(float (*part)[ROWS][RP + 1], int r, int c0, int live, int R, float s, float* u) {
+template <int RP, int WV, int H>
+__device__ static inline void sum_shares(float (*part)[H][RP + 1], int r, int c0, int live, int R, float s, float* u) {
 #pragma unroll
   for (int c = 0; c < RP / 8; ++c) {
     u[c] = 0.0f;
@@ -257,25 +262,30 @@ __device__ static inline void sum_shares(float (*part)[ROWS][RP + 1], int r, int
 }
 
 // ADD: out = y + z.  Else out = z, and the hidden rows of both products are kept.
-template <class IO, int RP, int WV, bool ADD>
+template <class IO, int RP, int WV, int MF, bool ADD>
 __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_kernel(AddArgs a) {
-  constexpr int VEC = IO::VEC, CB = 16 * VEC;
+  constexpr int VEC = IO::VEC, CB = 16 * VEC, H = 16 * MF;  // H: rows of a tile
   constexpr bool WIDE = VEC == 4;
   typedef typename IO::elem E;
   typedef Full<IO> Io;
-  __shared__ float part[ADD ? 1 : 2][WV][ROWS][RP + 1];
-  __shared__ Hidden<IO, RP> hid;
+  __shared__ float part[ADD ? 1 : 2][WV][H][RP + 1];
+  __shared__ Hidden<IO, RP, H> hid;
   const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits % a.tiles, b = blockIdx.x / a.splits / a.tiles;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
-  const int row0 = tile * ROWS, rows = min(ROWS, a.T - row0);
+  const int row0 = tile * H, rows = min(H, a.T - row0);
   const int len = valid_rows(a.lengths, b, a.T), v = voice_of(a.voices, b, a.V);
   const int live = min(rows, len - row0);  // rows of the tile that count (may be negative)
+  const int64_t kept = (int64_t)b * ceil_div(a.T, ROWS) + row0 / ROWS;
   const E* yb = row_at(static_cast<const E*>(a.y) + b * a.y_bs, row0, a.y_ts);
   E* ob = row_at(static_cast<E*>(a.out) + b * a.o_bs, row0, a.o_ts);
   const int blocks = ceil_div(a.N, CB);
 
   if (v < 0 || live <= 0) {
     if (ADD && a.in_place) return;
+    if (!ADD && v >= 0 && split == 0 && row0 % ROWS > 0 && len > row0 - H) {
+      keep_no_upper<RP>(a.first.keep, kept, threadIdx.x, WV * 64);
+      keep_no_upper<RP>(a.second.keep, kept, threadIdx.x, WV * 64);
+    }
     // a row per wave, 64 lanes across
     for (int r = split * WV + wave; r < rows; r += a.splits * WV) {
       const E* from = shifted(yb, r * a.y_ts);
@@ -341,24 +351,24 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
 
   const float s = a.scale ? a.scale[v] : 1.0f;
   const int r = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (RP / 8);  // of the sums: 8 threads to a row
-  first_product<IO, RP, WV>(a.first, row_at(static_cast<const E*>(a.first.x) + b * a.first.bs, row0, a.first.ts), v, a.R,
+  first_product<IO, RP, WV, MF>(a.first, row_at(static_cast<const E*>(a.first.x) + b * a.first.bs, row0, a.first.ts), v, a.R,
                             live, wave, lane, part[0]);
   if constexpr (!ADD) {
     // its 256 bytes go to the waves the first product leaves off at
     if (split == 0)
-      first_product<IO, RP, WV>(a.second, row_at(static_cast<const E*>(a.second.x) + b * a.second.bs, row0, a.second.ts),
+      first_product<IO, RP, WV, MF>(a.second, row_at(static_cast<const E*>(a.second.x) + b * a.second.bs, row0, a.second.ts),
                                 v, a.R, live, (wave + WV - ceil_div(a.first.K, 16 * VEC) % WV) % WV, lane, part[1]);
   }
   if (all > 0) fetch_b(block_of(0), AHEAD ? bn : br);
   __syncthreads();
-  if (r < ROWS) {
+  if (r < H) {
     float u[RP / 8];
     if (!ADD && split == 0) {
-      sum_shares<RP, WV>(part[ADD ? 0 : 1], r, c0, live, a.R, s, u);
-      keep_hidden<IO, RP>(a.second.keep, (int64_t)b * a.tiles + tile, r, c0, u);
+      sum_shares<RP, WV, H>(part[ADD ? 0 : 1], r, c0, live, a.R, s, u);
+      keep_hidden<IO, RP>(a.second.keep, kept, row0 % ROWS + r, c0, u);
     }
-    sum_shares<RP, WV>(part[0], r, c0, live, a.R, s, u);
-    if (!ADD && split == 0) keep_hidden<IO, RP>(a.first.keep, (int64_t)b * a.tiles + tile, r, c0, u);
+    sum_shares<RP, WV, H>(part[0], r, c0, live, a.R, s, u);
+    if (!ADD && split == 0) keep_hidden<IO, RP>(a.first.keep, kept, row0 % ROWS + r, c0, u);
     if constexpr (WIDE) {
 #pragma unroll
       for (int c = 0; c < RP / 8; ++c) hid.u[r][c0 + c] = u[c];
@@ -648,26 +658,35 @@ __global__ __launch_bounds__(LISTED) void gather_kernel(GatherArgs a) {
 
 int padded_rank(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : 64; }
 
-template <class IO, int RP, int WV, bool ADD>
+template <class IO, int RP, int WV, int MF, bool ADD>
 int launch_waves(AddArgs a, int64_t tiles, int splits, hipStream_t s) {
   a.splits = splits;
   TTSX_ARG(tiles * splits <= most_workgroups(WV * 64), "ttsx_adapter: too many rows");
-  adapter_kernel<IO, RP, WV, ADD><<<(unsigned)(tiles * splits), WV * 64, 0, s>>>(a);
+  adapter_kernel<IO, RP, WV, MF, ADD><<<(unsigned)(tiles * splits), WV * 64, 0, s>>>(a);
   TTSX_LAUNCH_CHECK();
   return TTSX_OK;
 }
 // Four waves to a tile where the tiles fill 256 CUs twice.  Fewer tiles get a workgroup of 16 waves each (8 at rank 64,
 // whose operands need the registers) and share their columns among up to 256 workgroups; each of those repeats the
-// first product, so no more of them than N is longer than K.
+// first product, so no more of them than N is longer than K.  Up to 128 tiles are cut into halves of 16 rows, a CU to each:
+// the chain of one tile is what is waited for then (32 x 128 x 512 -> 2048 rank 16 bf16 13.7 -> 10.9 us, its backward pass
+// in fp32 36 -> 31; at 256 tiles, 64 x 128 rank 32, A read twice as often costs more: bf16 21.0 -> 25.7, fp32 35.4 -> 39.3).
+constexpr int64_t HALVES = 128;
 template <class IO, int RP, bool ADD>
 int launch_tiles(AddArgs a, int B, hipStream_t s) {
   constexpr int MANY = RP == 64 ? 8 : 16;
   a.tiles = ceil_div(a.T, ROWS);
-  const int64_t tiles = (int64_t)B * a.tiles;
-  if (tiles >= 512) return launch_waves<IO, RP, 4, ADD>(a, tiles, 1, s);
-  const int blocks = ceil_div(a.N, 16 * IO::VEC), pieces = ceil_div(min(a.T, ROWS), 16);
+  int64_t tiles = (int64_t)B * a.tiles;
+  if (tiles >= 512) return launch_waves<IO, RP, 4, 2, ADD>(a, tiles, 1, s);
+  const int blocks = ceil_div(a.N, 16 * IO::VEC);
+  const bool halves = tiles <= HALVES;
+  if (halves) {
+    a.tiles = ADD ? ceil_div(a.T, ROWS / 2) : 2 * a.tiles;  // both halves of a tile of kept values are written
+    tiles = (int64_t)B * a.tiles;
+  }
+  const int pieces = ceil_div(min(a.T, halves ? ROWS / 2 : ROWS), 16);
   const int splits = min(min(ceil_div(blocks * pieces, MANY), max(1, (int)(256 / tiles))), max(1, a.N / a.first.K));
-  return launch_waves<IO, RP, MANY, ADD>(a, tiles, splits, s);
+  return halves ? launch_waves<IO, RP, MANY, 1, ADD>(a, tiles, splits, s) : launch_waves<IO, RP, MANY, 2, ADD>(a, tiles, splits, s);
 }
 
 template <class IO>
