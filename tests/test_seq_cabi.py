@@ -231,3 +231,24 @@ def test_an_empty_batch_takes_empty_lists():
     assert lengths_on("f", [], 0, 5, like).shape == voices_on("f", [], 0, 5, like).shape == (0,)
     with pytest.raises(ValueError):
         lengths_on("f", 3, 1, 5, like)
+
+
+def test_the_native_way_takes_ordinary_calls_only():
+    """Anything else comes back as None, to be checked in Python; nothing of these reaches a GPU."""
+    from tts_amd import _seq, _seqcalls
+    _seq._bind()
+    assert _seq.ways.ordinary is _seqcalls
+    t, s = torch.zeros(2, 5, 8), torch.zeros(2, 8)
+    v = torch.zeros(2, dtype=torch.int32)
+    for args in ((t[:, 0], t[:, 0], s, None), (1, 2, 3, None), (None,) * 4):
+        assert _seqcalls.step(*args) is None
+    assert _seqcalls.scan(t, t, None, None, False, True) is None and _seqcalls.scan(t, t, s, [1, 2], False, True) is None
+    assert _seqcalls.scan_backward(t, t, t, t, None, None, False) is None
+    assert _seqcalls.adapter_add(t, t, t, t, v, None, None, None) is None
+    assert _seqcalls.adapter_backward(t, t, t, t, [0, 1], None, None) is None
+    for call, n in ((_seqcalls.step, 4), (_seqcalls.scan, 6), (_seqcalls.scan_backward, 7), (_seqcalls.adapter_add, 8),
+                    (_seqcalls.adapter_backward, 7), (_seqcalls.bind, 7)):
+        with pytest.raises(TypeError):
+            call(*[None] * (n + 1))
+    with pytest.raises(TypeError):
+        _seqcalls.bind(*["x"] * 7)

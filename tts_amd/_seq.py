@@ -1,4 +1,11 @@
-"""Argument checks shared by the sequence operators (`recurrence`, `adapters`)."""
+"""Argument checks shared by the sequence operators (`recurrence`, `adapters`).
+
+A call has two ways in.  `ordinary` (csrc/seq_calls.cpp) makes the whole call from native code where every argument is as
+the entry point takes it, and returns None without doing anything where one is not; that call is checked, converted or
+refused here in Python."""
+import ctypes
+import types
+
 import torch
 
 from . import _lib
@@ -13,10 +20,33 @@ _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.curre
 _functions = {}
 
 
+class _Unbound:
+    """Before the library is loaded, and in place of `ordinary` to have every call checked in Python."""
+    step = scan = scan_backward = adapter_add = adapter_backward = staticmethod(lambda *args: None)
+
+
+ways = types.SimpleNamespace(ordinary=_Unbound)
+
+
+def _bind():
+    """Loads both libraries; from here on ordinary calls are made natively."""
+    lib = _lib.load()
+    try:
+        from . import _seqcalls
+    except ImportError as e:
+        raise _lib.TtsxError("tts_amd/_seqcalls.so cannot be loaded (%s): build it with `make -C tts_amd/csrc`" % e)
+    _seqcalls.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+        "ttsx_gated_step", "ttsx_gated_scan", "ttsx_gated_scan_backward", "ttsx_gated_scan_workspace", "ttsx_adapter_add",
+        "ttsx_adapter_backward", "ttsx_adapter_backward_workspace")))
+    ways.ordinary = _seqcalls
+
+
 def call(name, index, *args):
     """The entry point `name` with `args` and the current stream of device `index`, run on that device."""
     fn = _functions.get(name)
     if fn is None:
+        if not _functions:
+            _bind()
         fn = _functions[name] = getattr(_lib.load(), name)
     if _current_device() == index:
         rc = fn(*args, _raw_stream(index))

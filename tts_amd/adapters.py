@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from ._seq import (DTYPES, are_tensors, call, columns_apart, lengths_on, on_device, overlapping, overlaps, pointer, rows, same_place,
-                   voices_on, writable_rows)
+                   voices_on, ways, writable_rows)
 
 MAX_RANK = 64                     # TTSX_ADAPTER_MAX_RANK
 MAX_WIDTH = FURTHEST = 1 << 20   # columns, and elements between two rows, of a call
@@ -89,6 +89,9 @@ def adapter_add(y, x, down, up, voices, scale=None, lengths=None, out=None):
     device any number outside 0..V-1 is none); scale [V] float32: a factor per voice; lengths [B]: rows at positions >=
     lengths[b] stay y's and x is not read there.  `out` takes the result; out=y works in place and leaves rows without
     an adapter untouched.  The result has y's type, rounded once."""
+    done = ways.ordinary.adapter_add(y, x, down, up, voices, scale, lengths, out)
+    if done is not None:
+        return done
     what = "adapter_add"
     dev, B, T, K, N, R, V = _check(what, "y", y, x, down, up, scale)
     in_place = False
@@ -128,6 +131,9 @@ def adapter_backward(dy, x, down, up, voices, scale=None, lengths=None):
     Returns dx [B,T,K] (zero in rows without an adapter; not summed over axes that x was broadcast along), ddown
     [V,R,K] and dup [V,R,N] of their inputs' type: sums over all rows of a voice, kept in float32 and in a fixed order,
     so that two runs agree to the bit.  `scale` is a constant."""
+    done = ways.ordinary.adapter_backward(dy, x, down, up, voices, scale, lengths)
+    if done is not None:
+        return done
     what = "adapter_backward"
     dev, B, T, K, N, R, V = _check(what, "dy", dy, x, down, up, scale)
     voices = voices_on(what, voices, B, V, x)

@@ -22,7 +22,7 @@ import functools
 import torch
 
 from . import _lib
-from ._seq import DTYPES, are_tensors, call, lengths_on, on_device, overlapping, pointer, rows, same_place
+from ._seq import DTYPES, are_tensors, call, lengths_on, on_device, overlapping, pointer, rows, same_place, ways
 
 STATE_BLOCK = 64             # steps between two kept states (TTSX_STATE_BLOCK)
 MAX_CHANNELS = FURTHEST = 1 << 20   # channels, and elements between two rows, of a call
@@ -69,6 +69,9 @@ def gated_scan(x, g, h0=None, lengths=None, reverse=False, save_states=False):
 
     x and g may be slices of one projection (any strides; the last axis is copied if it is not contiguous, and all of
     it if its rows lie more than 2^20 elements apart)."""
+    done = ways.ordinary.scan(x, g, h0, lengths, reverse, save_states)
+    if done is not None:
+        return done
     what = "gated_scan"
     _values_and_gates(what, x, g, "BTD")
     B, T, D = x.shape
@@ -96,6 +99,9 @@ def gated_scan_backward(dh, x, g, states, dh_last=None, lengths=None, reverse=Fa
     last state.  `states` is what the forward call with the same x, g, h0, lengths and reverse kept.  Returns dx and dg
     of x's type (zero behind a request's end; not summed over axes that x or g were broadcast along) and the float32
     dh0."""
+    done = ways.ordinary.scan_backward(dh, x, g, states, dh_last, lengths, reverse)
+    if done is not None:
+        return done
     what = "gated_scan_backward"
     _values_and_gates(what, x, g, "BTD")
     are_tensors(what, ("dh", dh), ("states", states))
@@ -128,6 +134,9 @@ def gated_step(x, g, h, out=None):
     """The next step of B streams: x, g [B,D], float32 state h [B,D].  Returns (y, h'): the new state in x's type for
     the layer above, and in float32 for the next step.  `out` takes h' (a contiguous float32 [B,D]); out=h updates the
     state in place."""
+    done = ways.ordinary.step(x, g, h, out)
+    if done is not None:
+        return done
     what = "gated_step"
     _values_and_gates(what, x, g, "BD")
     are_tensors(what, ("h", h))
