@@ -590,32 +590,33 @@ struct Plan {
 // How the time axis is cut: enough workgroups to fill 256 CUs four times over, one tile at least to each.  It is not cut
 // where that loses: from one workgroup per CU on, since the fold reads everything once more (requests of 800 x 512 fp32,
 // us uncut / cut: 16 of them 21 / 25, 24 26 / 34, 32 33 / 46; below, 8 requests 17 / 16, 4 17 / 12; the backward pass 34 / 35,
-// 41 / 47, 50 / 59; 27 / 20, 26 / 16), and up to three tiles, since a second launch costs the host 4 us (1 x 300 x 512 fp32
-// 10.1 / 14.1 us a call, backwards 13.1 / 17.3).
-constexpr int ENOUGH = 256, FEW_TILES = 3, FULL = 1024;
+// 41 / 47, 50 / 59; 27 / 20, 26 / 16), and up to three tiles forwards and two backwards, where the second launch costs more
+// than the tiles in a row (300 x 512 fp32 7.1 / 8.4 us, 180 x 33 7.8 / 8.9; backwards 200 x 512 bf16 10.6 / 11.1, but its
+// three tiles of 300 x 512 15.0 / 11.3).
+constexpr int ENOUGH = 256, FULL = 1024;
 template <class S>
-Plan plan(int B, int T, int D) {
+Plan plan(int B, int T, int D, bool backward) {
   Plan p;
   const int tiles = ceil_div(T, S::TILE);
   p.cols = ceil_div(D, S::GROUP * S::N);
   const int64_t rows = (int64_t)B * p.cols;
-  const int want = (int)(rows >= ENOUGH || tiles <= FEW_TILES ? 1 : FULL / rows);
+  const int want = (int)(rows >= ENOUGH || tiles <= (backward ? 2 : 3) ? 1 : FULL / rows);
   p.per = ceil_div(tiles, want < tiles ? want : tiles);
   p.chunks = ceil_div(tiles, p.per);
   return p;
 }
 template <class S>
-size_t pairs_bytes(int B, int T, int D) {
-  const Plan p = plan<S>(B, T, D);
+size_t pairs_bytes(int B, int T, int D, bool backward) {
+  const Plan p = plan<S>(B, T, D, backward);
   return p.chunks == 1 ? 0 : sizeof(float) * 2 * (size_t)B * p.chunks * D;
 }
 
 template <class S>
 int launch(ScanArgs a, int B, size_t ws_bytes, bool backward, hipStream_t s) {
   const char* name = backward ? "ttsx_gated_scan_backward" : "ttsx_gated_scan";
-  const Plan p = plan<S>(B, a.T, a.D);
+  const Plan p = plan<S>(B, a.T, a.D, backward);
   a.cols = p.cols, a.chunks = p.chunks, a.per = p.per;
-  TTSX_ARG(p.chunks == 1 || (a.pairs && ws_bytes >= pairs_bytes<S>(B, a.T, a.D)), "%s: workspace too small", name);
+  TTSX_ARG(p.chunks == 1 || (a.pairs && ws_bytes >= pairs_bytes<S>(B, a.T, a.D, backward)), "%s: workspace too small", name);
   const int64_t grid = (int64_t)B * p.cols * p.chunks;
   TTSX_ARG(grid <= most_workgroups(WAVES * 64), "%s: too many requests of so many channels", name);
   const dim3 g((unsigned)grid), t(WAVES * 64);
@@ -650,9 +651,9 @@ int run_scan(ScanArgs a, int64_t x_ts, int64_t g_ts, int64_t dh_ts, int B, size_
 }
 
 template <class IO>
-size_t workspace(int B, int T, int D, int backward) {
-  if (!wide<IO>(D)) return pairs_bytes<Narrow<IO>>(B, T, D);
-  return backward ? pairs_bytes<WideBwd<IO>>(B, T, D) : pairs_bytes<WideFwd<IO>>(B, T, D);
+size_t workspace(int B, int T, int D, bool backward) {
+  if (!wide<IO>(D)) return pairs_bytes<Narrow<IO>>(B, T, D, backward);
+  return backward ? pairs_bytes<WideBwd<IO>>(B, T, D, true) : pairs_bytes<WideFwd<IO>>(B, T, D, false);
 }
 
 template <class IO, int N>
@@ -680,9 +681,9 @@ bool dtype_ok(int d) { return d == TTSX_F32 || d == TTSX_BF16 || d == TTSX_F16; 
 
 extern "C" long ttsx_gated_scan_workspace(int B, int T, int D, int dtype, int backward) {
   TTSX_ARG(shape_ok(B, T, D) && dtype_ok(dtype), "ttsx_gated_scan_workspace: bad shape or type");
-  return (long)(dtype == TTSX_F32    ? workspace<IoF32>(B, T, D, backward)
-                : dtype == TTSX_BF16 ? workspace<IoBf16>(B, T, D, backward)
-                                     : workspace<IoF16>(B, T, D, backward));
+  return (long)(dtype == TTSX_F32    ? workspace<IoF32>(B, T, D, backward != 0)
+                : dtype == TTSX_BF16 ? workspace<IoBf16>(B, T, D, backward != 0)
+                                     : workspace<IoF16>(B, T, D, backward != 0));
 }
 
 extern "C" int ttsx_gated_scan(const void* x, int64_t x_batch_stride, int64_t x_row_stride, const void* g,
