@@ -309,7 +309,7 @@ __global__ __launch_bounds__(WAVES * 64) void fold_kernel(ScanArgs a) {
 }
 
 // Forward pass.  Bound by memory: 64 x 800 x 512 fp32 with ragged ends (250 MB) in 57 us, 4.4 TB/s, where a copy of that size
-// reaches 5.3; a short text is one chain of load, scan and store, 4.3 us.
+// reaches 5.3; a short text is one chain of load, scan and store, 4.1 us.
 template <class S, bool SAVE>
 __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
   constexpr int N = S::N, L = S::L;
@@ -574,10 +574,11 @@ __global__ __launch_bounds__(256) void step_kernel(const typename IO::elem* x, i
 }
 
 // Lanes take 8 bytes of a row where D is a whole number of them, else one channel.  A tile costs its scans once, and few
-// channels over many steps make that small: 16 channel-steps per lane forwards (32 are no faster: 60 against 58 us at
-// 64 x 800 x 512 fp32; 16-byte lanes neither), 32 backwards (108 us at 64 x 800 x 1024 bf16; 16: 120, 16-byte lanes: 158).
+// channels over many steps make that small: forwards 8 steps a lane (fp32: 16 are no faster, 60 against 58 us at 64 x 800 x 512;
+// bf16: 4 take 142 us at 16 x 4000 x 1024 where 8 take 114, 35.8 and 33.3 at 48 x 800 x 512; 16-byte lanes neither), backwards
+// 32 channel-steps (108 us at 64 x 800 x 1024 bf16; 16: 120, 16-byte lanes: 158).
 template <class IO>
-using WideFwd = Shape<IO, 2 * IO::PER, 16, 8 / IO::PER>;
+using WideFwd = Shape<IO, 2 * IO::PER, 16, 8>;
 template <class IO>
 using WideBwd = Shape<IO, 2 * IO::PER, 16, 16 / IO::PER>;
 template <class IO>
