@@ -140,3 +140,55 @@ def test_a_refused_voice_leaves_the_carried_state():
     two = m.inference_truncated(ids, voice_ids=[1])[0]
     n = min(one.shape[1], two.shape[1])
     assert torch.isfinite(two).all() and not torch.equal(one[:, :n], two[:, :n])
+
+
+def test_very_many_short_requests():
+    """70 000 requests of three steps: the same as the same requests in two calls."""
+    from tts_amd.adapters import adapter_add, adapter_backward
+    from tts_amd.recurrence import gated_scan, gated_scan_backward, gated_step
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    B, T, D, V = 70000, 3, 4, 2
+    x, g, dh = (torch.randn(B, T, D, device="cuda", generator=gen) for _ in range(3))
+    lengths = torch.randint(0, T + 1, (B,), device="cuda", generator=gen, dtype=torch.int32)
+    halves = [slice(0, B // 2), slice(B // 2, B)]
+    h, last, states = gated_scan(x, g, lengths=lengths, save_states=True)
+    grads = gated_scan_backward(dh, x, g, states, lengths=lengths)
+    for s in halves:
+        a, b, c = gated_scan(x[s], g[s], lengths=lengths[s].clone(), save_states=True)
+        assert torch.equal(a, h[s]) and torch.equal(b, last[s])
+        for p, q in zip(gated_scan_backward(dh[s], x[s], g[s], c, lengths=lengths[s].clone()), grads):
+            assert torch.equal(p, q[s])
+    y, _ = gated_step(x[:, 0], g[:, 0], last)
+    assert torch.equal(y[-5:], gated_step(x[-5:, 0], g[-5:, 0], last[-5:])[0])
+    m = torch.randn(V, 3, D, device="cuda", generator=gen)
+    voices = torch.randint(-1, V, (B,), device="cuda", generator=gen, dtype=torch.int32)
+    out = adapter_add(x, g, m, m, voices, lengths=lengths)
+    dx, ddown, dup = adapter_backward(x, g, m, m, voices, lengths=lengths)
+    parts = [adapter_backward(x[s], g[s], m, m, voices[s].clone(), lengths=lengths[s].clone()) for s in halves]
+    for s, p in zip(halves, parts):
+        assert torch.equal(adapter_add(x[s], g[s], m, m, voices[s].clone(), lengths=lengths[s].clone()), out[s])
+        assert torch.equal(p[0], dx[s])
+    # whole numbers, whose sums stay below 2^24: the weights' gradients are exact
+    x, g = (torch.randint(-2, 3, (B, T, D), device="cuda", generator=gen).float() for _ in range(2))
+    m = torch.randint(-1, 2, (V, 3, D), device="cuda", generator=gen).float()
+    _, ddown, dup = adapter_backward(x, g, m, m, voices, lengths=lengths)
+    live = (torch.arange(T, device="cuda")[None] < lengths[:, None]).double()[..., None]
+    for v in range(V):
+        d, i = x[voices == v].double(), g[voices == v].double()
+        d, i = (d * live[voices == v]).reshape(-1, D), (i * live[voices == v]).reshape(-1, D)
+        assert torch.equal(ddown[v].double(), (d @ m[v].double().t()).t().contiguous() @ i)
+        assert torch.equal(dup[v].double(), (i @ m[v].double().t()).t().contiguous() @ d)
+
+
+def test_no_columns():
+    """A projection without inputs adds nothing; one without outputs has nothing to add to."""
+    from tts_amd.adapters import adapter_add, adapter_backward
+    y, v = torch.randn(2, 5, 6, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    none, up = torch.empty(2, 5, 0, device="cuda"), torch.randn(1, 3, 6, device="cuda")
+    out = adapter_add(y, none, torch.empty(1, 3, 0, device="cuda"), up, v)
+    assert torch.equal(out, y) and out.data_ptr() != y.data_ptr()
+    assert adapter_add(y, none, torch.empty(1, 3, 0, device="cuda"), up, v, out=y) is y
+    dx, ddown, dup = adapter_backward(y, none, torch.empty(1, 3, 0, device="cuda"), up, v)
+    assert dx.shape == none.shape and ddown.shape == (1, 3, 0) and not dup.any()
+    assert adapter_add(none, y, up, torch.empty(1, 3, 0, device="cuda"), v).shape == (2, 5, 0)
+    assert not adapter_backward(none, y, up, torch.empty(1, 3, 0, device="cuda"), v)[0].any()
