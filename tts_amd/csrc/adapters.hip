@@ -523,14 +523,20 @@ struct OuterArgs {
 };
 
 constexpr int WAVES = 4;
+// Above rank 32 the 16-bit types' sums (VEC to a lane and rank) leave room for one workgroup a CU: two take half of the ranks
+// each (32 x 128 x (512 + 2048) rank 64 bf16: the whole backward pass 45.7 -> 36.1 us; fp32, half as many, loses 0 to 2 %).
+template <class IO, int RP>
+constexpr int RANK_PARTS = RP > 32 && IO::VEC == 8 ? RP / 32 : 1;
 template <class IO, int RP>
 __global__ __launch_bounds__(WAVES * 64, 3) void outer_kernel(OuterArgs a) {
-  constexpr int VEC = IO::VEC, NJ = RP / 16, CB = 16 * VEC;
+  constexpr int VEC = IO::VEC, PARTS = RANK_PARTS<IO, RP>, NJ = RP / 16 / PARTS, CB = 16 * VEC;
   typedef typename IO::elem E;
   typedef Full<IO> Io;
+  const int j0 = blockIdx.x % PARTS * NJ;  // first sixteen of ranks
   const int kblocks = ceil_div(a.K, CB), groups = kblocks + ceil_div(a.N, CB);
-  int cb = blockIdx.x % groups;
-  const int chunk = blockIdx.x / groups % a.chunks, b = blockIdx.x / groups / a.chunks;
+  const int id = blockIdx.x / PARTS;
+  int cb = id % groups;
+  const int chunk = id / groups % a.chunks, b = id / groups / a.chunks;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
   __shared__ f32x4 sums[2][NJ * VEC][64];
   const int len = valid_rows(a.lengths, b, a.T);
@@ -561,7 +567,7 @@ __global__ __launch_bounds__(WAVES * 64, 3) void outer_kernel(OuterArgs a) {
         xr[i] = Io::load_end(shifted(row_at(src, r0, ts), min(8 * q + i, last - 1 - r0) * ts), c, width);
     }
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) hidden_rows<RP>(ub, (int64_t)b * a.tiles + r0 / ROWS, j, lane, ur[j]);
+    for (int j = 0; j < NJ; ++j) hidden_rows<RP>(ub, (int64_t)b * a.tiles + r0 / ROWS, j0 + j, lane, ur[j]);
   };
   for (int r0 = first + wave * ROWS; r0 < last; r0 += WAVES * ROWS) {
     u32x4 xr[8], ur[NJ][2];
@@ -621,7 +627,7 @@ __global__ __launch_bounds__(WAVES * 64, 3) void outer_kernel(OuterArgs a) {
       float o[VEC];
 #pragma unroll
       for (int k = 0; k < VEC; ++k) o[k] = acc[j][k][i];
-      store_f32_some<VEC>(out + (int64_t)(16 * j + 4 * q + i) * total, n, o);
+      store_f32_some<VEC>(out + (int64_t)(16 * (j0 + j) + 4 * q + i) * total, n, o);
     }
 }
 
@@ -766,7 +772,7 @@ int run_backward(AddArgs a, const BackPlan& p, int B, float* ws, void* ddown, vo
   o.dy = a.first.x, o.dy_bs = a.first.bs, o.dy_ts = a.first.ts;
   o.du = du, o.u = u, o.voices = a.voices, o.lengths = a.lengths, o.part = part;
   o.T = a.T, o.K = a.second.K, o.N = a.first.K, o.V = a.V, o.chunks = p.chunks, o.span = p.span, o.tiles = ceil_div(a.T, ROWS);
-  const int64_t grid = (int64_t)B * p.chunks * (ceil_div(o.K, 16 * IO::VEC) + ceil_div(o.N, 16 * IO::VEC));
+  const int64_t grid = (int64_t)B * p.chunks * (ceil_div(o.K, 16 * IO::VEC) + ceil_div(o.N, 16 * IO::VEC)) * RANK_PARTS<IO, RP>;
   TTSX_ARG(grid <= most_workgroups(WAVES * 64), "ttsx_adapter_backward: too many rows");
   outer_kernel<IO, RP><<<(unsigned)grid, WAVES * 64, 0, s>>>(o);
   TTSX_LAUNCH_CHECK();
