@@ -330,8 +330,8 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
   if (q.chunk > 0) apply_chunks<S>(a.pairs + (int64_t)q.b * a.chunks * 2 * a.D, a.D, 0, 1, q.chunk, q, tot[1], carry);
 
   const int first = q.chunk * a.per * S::TILE, last = min(first + a.per * S::TILE, a.T);
-  int flip = 0;
-  for (int p0 = first; p0 < last; p0 += S::TILE, flip ^= 1) {
+  int half = 1;  // of `tot`; the first tile that has rows takes the one that apply_chunks left alone
+  for (int p0 = first; p0 < last; p0 += S::TILE) {
     const int p = p0 + q.tg * L;
     const bool keeps = SAVE && p % BLOCK == 0 && p < a.T && q.on;
     float* kept = SAVE ? a.states + ((int64_t)q.b * blocks + p / BLOCK) * a.D + q.c : nullptr;
@@ -340,6 +340,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
       if (keeps) store_f32<N>(kept, carry);
       continue;
     }
+    half ^= 1;
     const Tile<S> t(p0, len, a.reverse);
     typename Io::raw xr[L], gr[L];
     load_rows<S>(gr, gb, a.g_ts, t, q);
@@ -370,7 +371,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
     wave_scan<S>(A, B, q.lane);
     if (q.lane >= 64 - S::GROUP) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) tot[flip].v[q.wave][0][q.across][j] = A[j], tot[flip].v[q.wave][1][q.across][j] = B[j];
+      for (int j = 0; j < N; ++j) tot[half].v[q.wave][0][q.across][j] = A[j], tot[half].v[q.wave][1][q.across][j] = B[j];
     }
     __syncthreads();  // the other half of `tot` is written next: one barrier per tile
     float h[N];       // state in front of the wave, then of the lane
@@ -382,8 +383,8 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float ta = tot[flip].v[k][0][q.across][j];
-        carry[j] = fmaf(ta, carry[j], tot[flip].v[k][1][q.across][j]);
+        const float ta = tot[half].v[k][0][q.across][j];
+        carry[j] = fmaf(ta, carry[j], tot[half].v[k][1][q.across][j]);
       }
     }
 #pragma unroll
@@ -428,13 +429,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
                     carry);
 
   const int first = q.chunk * a.per * S::TILE, last = min(first + a.per * S::TILE, a.T);
-  int flip = 0;
-  for (int p0 = first + (ceil_div(last - first, S::TILE) - 1) * S::TILE; p0 >= first; p0 -= S::TILE, flip ^= 1) {
+  int half = 1;  // as in scan_kernel; tiles behind the end come first here and have no barrier, so they leave it as it is
+  for (int p0 = first + (ceil_div(last - first, S::TILE) - 1) * S::TILE; p0 >= first; p0 -= S::TILE) {
     if (p0 >= len) {
       zero_rows<S>(dxb, pitch, p0, len, a.T, q);
       zero_rows<S>(dgb, pitch, p0, len, a.T, q);
       continue;
     }
+    half ^= 1;
     const Tile<S> t(p0, len, a.reverse);
     typename Io::raw xr[L], gr[L], dr[L];
     float h[N];  // state in front of the tile
@@ -490,11 +492,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
     wave_scan<S>(A, B, q.lane);
     if (q.lane < S::GROUP) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) tot[flip].v[q.wave][0][q.across][j] = A2[j], tot[flip].v[q.wave][2][q.across][j] = C[j];
+      for (int j = 0; j < N; ++j) tot[half].v[q.wave][0][q.across][j] = A2[j], tot[half].v[q.wave][2][q.across][j] = C[j];
     }
     if (q.lane >= 64 - S::GROUP) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) tot[flip].v[q.wave][1][q.across][j] = B[j];
+      for (int j = 0; j < N; ++j) tot[half].v[q.wave][1][q.across][j] = B[j];
     }
     __syncthreads();
     float R[N];  // gradient behind the wave, then behind the lane
@@ -502,14 +504,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
     for (int k = WAVES - 1; k >= 0; --k)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float ta = tot[flip].v[k][0][q.across][j];
+        const float ta = tot[half].v[k][0][q.across][j];
         if (k == q.wave) R[j] = carry[j];
-        carry[j] = fmaf(ta, carry[j], tot[flip].v[k][2][q.across][j]);
+        carry[j] = fmaf(ta, carry[j], tot[half].v[k][2][q.across][j]);
       }
 #pragma unroll 1
     for (int k = 0; k < q.wave; ++k)
 #pragma unroll
-      for (int j = 0; j < N; ++j) h[j] = fmaf(tot[flip].v[k][0][q.across][j], h[j], tot[flip].v[k][1][q.across][j]);
+      for (int j = 0; j < N; ++j) h[j] = fmaf(tot[half].v[k][0][q.across][j], h[j], tot[half].v[k][1][q.across][j]);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       float pa = __shfl_up(A[j], S::GROUP, 64), pb = __shfl_up(B[j], S::GROUP, 64);
