@@ -60,7 +60,7 @@ __device__ static inline float gate(float g, float& e) {
   if constexpr (IO::PER == 1) {
     const float c = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -126.0f), 88.0f);
     const float t = 1.44269502f * c;
-    const float rest = fmaf(t, -1.90465421e-9f, fmaf(t, -0.693147182f, c));  // c - t ln 2, ln 2 in two parts
+    const float rest = fmaf(t, 1.90465421e-9f, fmaf(t, -0.693147182f, c));  // c - t ln 2, ln 2 = 0.693147182 - 1.9e-9
     const float p = __builtin_amdgcn_exp2f(t);
     e = fmaf(p, rest, p);
     w = __builtin_amdgcn_rcpf(1.0f + e);
