@@ -2,8 +2,8 @@
 
 Bounds in units F32 = 2^-24 of the value (half a unit in the last place).  The hardware's exponential and reciprocal are
 off by one unit in the last place, 2 F32 each.  fp32: e = e^g is the exponential, one fused product (1), and a remainder
-that is exact to second order: 3.  16-bit logits: 2 + 1, and the second order of the correction, (88 x 4.89e-6)^2 / 2 = 1.6
-F32 at the farthest logits here: 5.  w = 1 / (1 + e): e's error, the sum's 1, the reciprocal's 2: 6 and 8."""
+that is exact to second order: 3.  16-bit logits: 2 + 1, and what the correction leaves out, the second order of bf16's, (85 x
+4.89e-6)^2 / 2 = 1.5 F32 at the farthest logits here, or the third of fp16's, (85 x 4.72e-5)^3 / 6 = 0.2: 5.  w = 1 / (1 + e): e's error, the sum's 1, the reciprocal's 2: 6 and 8."""
 import pytest
 import torch
 
@@ -11,8 +11,8 @@ from seq_ref import F32
 
 pytestmark = pytest.mark.gpu
 
-TYPES = [torch.float32, torch.bfloat16]
-W_UNITS = {torch.float32: 6, torch.bfloat16: 8}
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+W_UNITS = {torch.float32: 6, torch.bfloat16: 8, torch.float16: 8}
 
 
 def _logits(dtype, low=-85.0, high=85.0):
