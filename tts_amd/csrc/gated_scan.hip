@@ -49,14 +49,15 @@ struct Shape {
 constexpr float L2E_16 = 1.44268799f, L2E_16_REST = 4.88849537e-6f;
 constexpr float L2E_13 = 1.44262695f, L2E_13_REST = 4.71948406e-5f;
 
-// w = sigmoid(-g) = 1 / (1 + e^g), to a few units in its own last place over all of g; f = 1 - w wherever f is a factor of
-// a state.  Long memories live in w (an error d of f is one of d / w in the state), and the difference adds half a unit
-// of f.  e^g is exp2 of the rounded product with log2(e), with what was rounded away put back: for 16-bit logits the
+// w = sigmoid(-g) = 1 / (1 + e^g) and f = sigmoid(g), each to a few units in its own last place wherever it is a normal number.
+// Long memories live in w (an error d of f is one of d / w in the state), and what is left of a state behind a closed gate
+// in f: below a half f is e^g w, since 1 - w has lost the digits that count (a third of f at g = -16, all of it from -17.4
+// on); above it 1 - w adds half a unit.  e^g is exp2 of the rounded product with log2(e), with what was rounded away put back: for 16-bit logits the
 // product with a log2(e) cut to 16 (bf16) or 13 bits (fp16) is exact and the rest of the constant is the correction, fp32
 // logits take it from a fused product.  -inf gives w = 1, +inf gives 0, a NaN stays one.
 template <class IO>
-__device__ static inline float gate(float g, float& e) {
-  float w;
+__device__ static inline float gate(float g, float& f) {
+  float w, e;
   if constexpr (IO::PER == 1) {
     const float c = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -126.0f), 88.0f);
     const float t = 1.44269502f * c;
@@ -74,10 +75,9 @@ __device__ static inline float gate(float g, float& e) {
     e = fmaf(p, B ? d : fmaf(0.5f * d, d, d), p);  // fp16: d is up to 4e-3 where w is no zero, its square counts
     w = __builtin_amdgcn_rcpf(1.0f + e);
   }
+  f = e < 1.0f ? e * w : 1.0f - w;
   return w;
 }
-// f w, the slope of f, with its digits at both ends.
-__device__ static inline float slope(float w, float e) { return w * (e < 1.0f ? e * w : 1.0f - w); }
 
 struct Place {
   int b, chunk, c, across, tg, wave, lane;  // c: first channel of the lane; wave: a scalar
@@ -277,8 +277,8 @@ __global__ __launch_bounds__(WAVES * 64) void fold_kernel(ScanArgs a) {
       Io::unpack(k0 + i < steps ? vr[i] : Io::fill(0), v);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        float e;
-        const float w = gate<typename S::Type>(gv[j], e), f = 1.0f - w;
+        float f;
+        const float w = gate<typename S::Type>(gv[j], f);
         A[j] *= f;
         B[j] = BACK ? f * (B[j] + v[j]) : fmaf(f, B[j], w * v[j]);
       }
@@ -361,9 +361,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
       Io::unpack(xr[i], xv);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        float e;
-        const float w = gate<typename S::Type>(gv[j], e);
-        f[i][j] = 1.0f - w;
+        const float w = gate<typename S::Type>(gv[j], f[i][j]);
         v[i][j] = w * xv[j];
         A[j] *= f[i][j];
         B[j] = fmaf(f[i][j], B[j], v[i][j]);
@@ -454,8 +452,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
       zero_rows<S>(dxb, pitch, p0, len, a.T, q);
       zero_rows<S>(dgb, pitch, p0, len, a.T, q);
     }
-    // s: f w, later dg / G.  A: product of f; B: the forward fold; C: the backward fold of f dh
-    float w[L][N], s[L][N], A[N], A2[N], B[N], C[N];
+    // A: product of f; B: the forward fold; C: the backward fold of f dh
+    float f[L][N], w[L][N], A[N], A2[N], B[N], C[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) A[j] = 1.0f, B[j] = C[j] = 0.0f;
 #pragma unroll
@@ -465,13 +463,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
       Io::unpack(xr[i], xv);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        float e;
-        w[i][j] = gate<typename S::Type>(gv[j], e);
-        s[i][j] = slope(w[i][j], e);
-        A[j] *= 1.0f - w[i][j];
-        B[j] = fmaf(1.0f - w[i][j], B[j], w[i][j] * xv[j]);
+        w[i][j] = gate<typename S::Type>(gv[j], f[i][j]);
         forget(w[i][j]);
-        forget(s[i][j]);
+        forget(f[i][j]);
+        A[j] *= f[i][j];
+        B[j] = fmaf(f[i][j], B[j], w[i][j] * xv[j]);
       }
       forget<S>(xr[i]);
     }
@@ -480,13 +476,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
       float dv[N];
       Io::unpack(dr[i], dv);
 #pragma unroll
-      for (int j = 0; j < N; ++j) C[j] = (1.0f - w[i][j]) * (C[j] + dv[j]);
+      for (int j = 0; j < N; ++j) C[j] = f[i][j] * (C[j] + dv[j]);
       forget<S>(dr[i]);
     }
-#pragma unroll
-    for (int i = 0; i < L; ++i)
-#pragma unroll
-      for (int j = 0; j < N; ++j) forget(w[i][j]);
 #pragma unroll
     for (int j = 0; j < N; ++j) A2[j] = A[j];
     wave_scan_back<S>(A2, C, q.lane);
@@ -520,17 +512,16 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
       pa = __shfl_down(A2[j], S::GROUP, 64), pb = __shfl_down(C[j], S::GROUP, 64);
       R[j] = q.lane < 64 - S::GROUP ? fmaf(pa, R[j], pb) : R[j];
     }
-    // the states of the lane's steps again
+    // the states of the lane's steps again; s: dg / G
+    float s[L][N];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       float xv[N];
       Io::unpack(xr[i], xv);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        s[i][j] *= h[j] - xv[j];
-        h[j] = fmaf(1.0f - w[i][j], h[j], w[i][j] * xv[j]);
-        forget(w[i][j]);
-        forget(s[i][j]);
+        s[i][j] = f[i][j] * w[i][j] * (h[j] - xv[j]);
+        h[j] = fmaf(f[i][j], h[j], w[i][j] * xv[j]);
       }
     }
 #pragma unroll
@@ -542,7 +533,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a
         const float G = dv[j] + R[j];
         gx[j] = w[i][j] * G;
         gg[j] = s[i][j] * G;
-        R[j] = (1.0f - w[i][j]) * G;
+        R[j] = f[i][j] * G;
       }
       store_row<S>(dxb, pitch, t, q, i, Io::pack(gx));
       store_row<S>(dgb, pitch, t, q, i, Io::pack(gg));
@@ -568,9 +559,9 @@ __global__ __launch_bounds__(256) void step_kernel(const typename IO::elem* x, i
   load_f32<N>(h + b * D + c, hv);
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    float e;
-    const float w = gate<IO>(gv[j], e);
-    hv[j] = fmaf(1.0f - w, hv[j], w * xv[j]);
+    float f;
+    const float w = gate<IO>(gv[j], f);
+    hv[j] = fmaf(f, hv[j], w * xv[j]);
   }
   Io::store(y + b * D + c, Io::pack(hv));
   store_f32<N>(h_out + b * D + c, hv);
