@@ -12,9 +12,10 @@
 // take blocks of 16 VEC output columns each, read B once per block, and add to y as they write.  u = x A^T never
 // leaves the chip, and y is read and written once: the launch is bound by x, y and out.
 //
-// 16-bit types: the first product is exact up to its fp32 sums.  u is fp32 and is handed to the second product as the
-// sum of two 16-bit numbers (16 or more bits of it), at no cost up to rank 16, where both halves fill one matrix
-// instruction.  fp16 has no range for that, so its rows of u are scaled by a power of two first.
+// 16-bit types: the first product is exact up to its fp32 sums.  u is fp32 and is handed on as a sum of 16-bit numbers that
+// holds all of it: three of bf16's 8 bits, or two of fp16's 11 (24 bits leave a remainder below 2^12 units behind the first,
+// which the second holds to one unit: a rounding of u to 2^-23).  fp16 has no range for that, so its rows of u are scaled by a
+// power of two first.
 // Where a column block's lanes read 16 bytes of B from 8 ranks, the 8 x 8 block is transposed in registers; lane
 // l & 15 then owns VEC neighbouring columns, so y and out move 16 bytes per lane.
 #include "../../include/ttsx_seq.h"
@@ -75,12 +76,20 @@ __device__ static inline void transpose8(const u32x4* r, u32x4* t) {
     }
 }
 
-// v as the sum of two numbers of the 16-bit type (the second is zero where the first is not finite).
+// Two fp32 values as sums of numbers of the 16-bit type, a word of pairs each, the largest first (all others are zero where it is
+// not finite).
 template <class IO>
-__device__ static inline void two_parts(float v, typename IO::elem& hi, typename IO::elem& lo) {
-  hi = (typename IO::elem)v;
-  const float h = (float)hi;
-  lo = (typename IO::elem)(fabsf(h) < INFINITY ? v - h : 0.0f);
+constexpr int PARTS = IO::INF == IoBf16::INF ? 3 : 2;
+template <class IO>
+__device__ static inline void parts_of(float v0, float v1, uint32_t* p) {
+  float v[2] = {v0, v1}, h[2];
+#pragma unroll
+  for (int k = 0; k < PARTS<IO>; ++k) {
+    p[k] = IO::pack(v);
+    IO::unpack(p[k], h);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) v[i] = fabsf(h[i]) < INFINITY ? v[i] - h[i] : 0.0f;
+  }
 }
 
 __device__ static inline int voice_of(const int32_t* voices, int b, int V) {
@@ -88,11 +97,10 @@ __device__ static inline int voice_of(const int32_t* voices, int b, int V) {
   return v >= 0 && v < V ? v : -1;
 }
 
-// u of a tile, as the matrix operand of the second product: [H][RP] fp32, or two 16-bit planes and a factor per row.
+// u of a tile, as the matrix operand of the second product: [H][RP] fp32, or its parts in 16-bit planes and a factor per row.
 template <class IO, int RP, int H>
-struct Hidden {
-  typedef typename IO::elem E;
-  E hi[H][RP + 8], lo[H][RP + 8];
+struct alignas(16) Hidden {
+  typename IO::elem part[PARTS<IO>][H][RP + 8];
   float factor[H];
 };
 template <int RP, int H>
@@ -108,24 +116,15 @@ __device__ static inline int rank_of(int q, int i) {
   return RP == 16 ? 8 * (q & 1) + i : i / 8 * 32 + 8 * q + i % 8;
 }
 
-// u for the weights' gradients, where it is contracted over rows: per tile of 32 rows and 16 ranks two times 1 KB in the
-// order of the matrix operand, lane 16 q + rank with rows 8 q .. 8 q + 7.  bf16 takes it as two parts, one KB each; fp16
-// has no range for that (a factor per row would not come out of the sum) and multiplies in fp32, rows 8 q .. + 3 in the
-// first KB and the other four in the second.
-template <class IO>
-constexpr bool SPLIT_HIDDEN = IO::INF == IoBf16::INF;
-template <class IO, int RP>
+// u for the weights' gradients, where it is contracted over rows: per tile of 32 rows and 16 ranks two times 1 KB of fp32 in the
+// order of the matrix operand, lane 16 q + rank with rows 8 q .. 8 q + 7, the first four in the first KB.
+template <int RP>
 __device__ static inline void keep_hidden(float* keep, int64_t tile, int row, int c0, const float* u) {
 #pragma unroll
   for (int c = 0; c < RP / 8; ++c) {
     const int rank = c0 + c, lane = 16 * (row >> 3) + (rank & 15);
     float* at = keep + (tile * (RP / 16) + (rank >> 4)) * 512;
-    if constexpr (SPLIT_HIDDEN<IO>) {
-      typename IO::elem* e = reinterpret_cast<typename IO::elem*>(at) + lane * 8 + (row & 7);
-      two_parts<IO>(u[c], e[0], e[512]);
-    } else {
-      at[(row >> 2 & 1) * 256 + lane * 4 + (row & 3)] = u[c];
-    }
+    at[(row >> 2 & 1) * 256 + lane * 4 + (row & 3)] = u[c];
   }
 }
 // Rows 16 .. 31 of a tile whose request ends in front of them: zero.
@@ -383,10 +382,10 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
     float u[RP / 8];
     if (!ADD && split == 0) {
       sum_shares<RP, WV, H>(part[ADD ? 0 : 1], r, c0, live, a.R, s, u);
-      keep_hidden<IO, RP>(a.second.keep, kept, row0 % ROWS + r, c0, u);
+      keep_hidden<RP>(a.second.keep, kept, row0 % ROWS + r, c0, u);
     }
     sum_shares<RP, WV, H>(part[0], r, c0, live, a.R, s, u);
-    if (!ADD && split == 0) keep_hidden<IO, RP>(a.first.keep, kept, row0 % ROWS + r, c0, u);
+    if (!ADD && split == 0) keep_hidden<RP>(a.first.keep, kept, row0 % ROWS + r, c0, u);
     if (owns_rest) {
       float sum = 0.0f, y;
 #pragma unroll
@@ -428,7 +427,12 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
         if ((threadIdx.x & 7) == 0) hid.factor[r] = 1.0f / up;
       }
 #pragma unroll
-      for (int c = 0; c < RP / 8; ++c) two_parts<IO>(u[c] * up, hid.hi[r][c0 + c], hid.lo[r][c0 + c]);
+      for (int c = 0; c < RP / 8; c += 2) {
+        uint32_t p[PARTS<IO>];
+        parts_of<IO>(u[c] * up, u[c + 1] * up, p);
+#pragma unroll
+        for (int k = 0; k < PARTS<IO>; ++k) *reinterpret_cast<uint32_t*>(&hid.part[k][r][c0 + c]) = p[k];
+      }
     }
   }
   __syncthreads();
@@ -473,19 +477,22 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
           z[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(u, __uint_as_float(br[t][j]), z[j], 0, 0, 0);
       }
     } else if constexpr (RP == 16) {
-      const E* src = q < 2 ? &hid.hi[ur][8 * q] : &hid.lo[ur][8 * (q - 2)];
-      const u32x4 u = *reinterpret_cast<const u32x4*>(src);
+      // both halves of the lanes have these ranks of B: two parts of u to an instruction
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) z[j] = mma<IO>(u, br[j], z[j]);
+      for (int k = (PARTS<IO> - 1) / 2 * 2; k >= 0; k -= 2) {
+        u32x4 u = Io::fill(0);
+        if (k + 1 < PARTS<IO> || q < 2) u = *reinterpret_cast<const u32x4*>(&hid.part[k + q / 2][ur][8 * (q & 1)]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) z[j] = mma<IO>(u, br[j], z[j]);
+      }
     } else {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        const u32x4 uh = *reinterpret_cast<const u32x4*>(&hid.hi[ur][32 * kb + 8 * q]);
-        const u32x4 ul = *reinterpret_cast<const u32x4*>(&hid.lo[ur][32 * kb + 8 * q]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          z[j] = mma<IO>(ul, br[8 * kb + j], z[j]);
-          z[j] = mma<IO>(uh, br[8 * kb + j], z[j]);
+        for (int k = PARTS<IO> - 1; k >= 0; --k) {
+          const u32x4 u = *reinterpret_cast<const u32x4*>(&hid.part[k][ur][32 * kb + 8 * q]);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) z[j] = mma<IO>(u, br[8 * kb + j], z[j]);
         }
       }
     }
@@ -529,12 +536,12 @@ template <class IO, int RP>
 constexpr int RANK_PARTS = RP > 32 && IO::VEC == 8 ? RP / 32 : 1;
 template <class IO, int RP>
 __global__ __launch_bounds__(WAVES * 64, 3) void outer_kernel(OuterArgs a) {
-  constexpr int VEC = IO::VEC, PARTS = RANK_PARTS<IO, RP>, NJ = RP / 16 / PARTS, CB = 16 * VEC;
+  constexpr int VEC = IO::VEC, SHARES = RANK_PARTS<IO, RP>, NJ = RP / 16 / SHARES, CB = 16 * VEC;
   typedef typename IO::elem E;
   typedef Full<IO> Io;
-  const int j0 = blockIdx.x % PARTS * NJ;  // first sixteen of ranks
+  const int j0 = blockIdx.x % SHARES * NJ;  // first sixteen of ranks
   const int kblocks = ceil_div(a.K, CB), groups = kblocks + ceil_div(a.N, CB);
-  const int id = blockIdx.x / PARTS;
+  const int id = blockIdx.x / SHARES;
   int cb = id % groups;
   const int chunk = id / groups % a.chunks, b = id / groups / a.chunks;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
@@ -577,17 +584,26 @@ __global__ __launch_bounds__(WAVES * 64, 3) void outer_kernel(OuterArgs a) {
       for (int i = 0; i < 8; ++i)
         if (r0 + 8 * q + i >= last) xr[i] = Io::fill(0);
     }
-    if constexpr (SPLIT_HIDDEN<IO>) {
+    if constexpr (IO::INF == IoBf16::INF) {
       u32x4 bt[8];
       transpose8(xr, bt);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
+      for (int j = 0; j < NJ; ++j) {
+        u32x4 part[PARTS<IO>];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          acc[j][i] = mma<IO>(ur[j][1], bt[i], acc[j][i]);
-          acc[j][i] = mma<IO>(ur[j][0], bt[i], acc[j][i]);
+        for (int m = 0; m < 4; ++m) {
+          uint32_t p[PARTS<IO>];
+          const u32x4 r = ur[j][m / 2];
+          parts_of<IO>(__uint_as_float(r[m % 2 * 2]), __uint_as_float(r[m % 2 * 2 + 1]), p);
+#pragma unroll
+          for (int k = 0; k < PARTS<IO>; ++k) part[k][m] = p[k];
         }
-    } else {
+#pragma unroll
+        for (int k = PARTS<IO> - 1; k >= 0; --k)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) acc[j][i] = mma<IO>(part[k], bt[i], acc[j][i]);
+      }
+    } else {  // fp16 has no range for parts here: a factor per row would not come out of the sum
 #pragma unroll
       for (int s = 0; s < 8; ++s) {
         float xv[VEC];
