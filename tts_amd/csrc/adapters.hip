@@ -76,8 +76,7 @@ __device__ static inline void transpose8(const u32x4* r, u32x4* t) {
     }
 }
 
-// Two fp32 values as sums of numbers of the 16-bit type, a word of pairs each, the largest first (all others are zero where it is
-// not finite).
+// Two fp32 values as sums of numbers of the 16-bit type, a word of pairs each, the largest first.
 template <class IO>
 constexpr int PARTS = IO::INF == IoBf16::INF ? 3 : 2;
 template <class IO>
@@ -88,13 +87,40 @@ __device__ static inline void parts_of(float v0, float v1, uint32_t* p) {
     p[k] = IO::pack(v);
     IO::unpack(p[k], h);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) v[i] = fabsf(h[i]) < INFINITY ? v[i] - h[i] : 0.0f;
+    for (int i = 0; i < 2; ++i) v[i] -= h[i];
   }
+}
+// A sum over parts is no number where a factor is infinite: the other parts of u may be zero or of the other sign, those of an
+// infinite u are none.  The first parts alone give the infinity (or NaN) of the sum (a multiple of it does too); where they
+// give a number the sum stands.  `unsure`: whether the wave has such a sum.
+template <int N>
+__device__ static inline bool unsure(const f32x4* z) {
+  float t = 0.0f;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t = fmaf(z[j][i], 0.0f, t);
+  return __any(t != 0.0f);
+}
+__device__ static inline void settle(f32x4& z, f32x4 first) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) z[i] = fabsf(z[i]) < INFINITY || fabsf(first[i]) < INFINITY ? z[i] : first[i];
 }
 
 __device__ static inline int voice_of(const int32_t* voices, int b, int V) {
   const int v = voices[b];
   return v >= 0 && v < V ? v : -1;
+}
+
+// Zero in the place of infinities and NaN.
+__device__ static inline u32x4 finite_bf16(u32x4 r) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w = r[i];
+    w = (w & 0x7f80u) == 0x7f80u ? w & 0xffff0000u : w;
+    r[i] = (w & 0x7f800000u) == 0x7f800000u ? w & 0xffffu : w;
+  }
+  return r;
 }
 
 // u of a tile, as the matrix operand of the second product: [H][RP] fp32, or its parts in 16-bit planes and a factor per row.
@@ -496,6 +522,20 @@ __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_k
         }
       }
     }
+    if constexpr (!WIDE) {
+      if (unsure<VEC>(z)) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          f32x4 first = (f32x4){0, 0, 0, 0};
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {  // up to rank 16 in both halves of the lanes: twice the sum
+            const u32x4 u = *reinterpret_cast<const u32x4*>(&hid.part[0][ur][32 * kb + 8 * (RP > 16 ? q : q & 1)]);
+            first = mma<IO>(u, br[8 * kb + j], first);
+          }
+          settle(z[j], first);
+        }
+      }
+    }
     const int sl = anew(l16), n = min(max(a.N - cb * CB - sl * VEC, 0), VEC);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -558,10 +598,6 @@ __global__ __launch_bounds__(WAVES * 64, 3) void outer_kernel(OuterArgs a) {
   const E* src = of_x ? static_cast<const E*>(a.x) + b * a.x_bs : static_cast<const E*>(a.dy) + b * a.dy_bs;
   const float* ub = of_x ? a.du : a.u;
   f32x4 acc[NJ][VEC];
-#pragma unroll
-  for (int j = 0; j < NJ; ++j)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[j][i] = (f32x4){0, 0, 0, 0};
   // rows first + r0 .. + 31, this lane the 8 from 8 q on; rows behind the last are zero (and so is their u)
   const auto fetch = [&](int r0, u32x4* xr, u32x4 (*ur)[2]) {
     if (whole) {
@@ -576,46 +612,70 @@ __global__ __launch_bounds__(WAVES * 64, 3) void outer_kernel(OuterArgs a) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) hidden_rows<RP>(ub, (int64_t)b * a.tiles + r0 / ROWS, j0 + j, lane, ur[j]);
   };
-  for (int r0 = first + wave * ROWS; r0 < last; r0 += WAVES * ROWS) {
-    u32x4 xr[8], ur[NJ][2];
-    fetch(r0, xr, ur);
-    if (r0 + ROWS > last) {
+  // A sum over parts is no number where a factor is infinite (see `unsure`).  The wave then takes its rows once more with zero in the
+  // place of what is not finite wherever other parts than the first are multiplied.
+  constexpr bool SPLIT = IO::INF == IoBf16::INF;
+  bool again = false;
+  do {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (r0 + 8 * q + i >= last) xr[i] = Io::fill(0);
-    }
-    if constexpr (IO::INF == IoBf16::INF) {
-      u32x4 bt[8];
-      transpose8(xr, bt);
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        u32x4 part[PARTS<IO>];
+      for (int i = 0; i < VEC; ++i) acc[j][i] = (f32x4){0, 0, 0, 0};
+    for (int r0 = first + wave * ROWS; r0 < last; r0 += WAVES * ROWS) {
+      u32x4 xr[8], ur[NJ][2];
+      fetch(r0, xr, ur);
+      if (r0 + ROWS > last) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          uint32_t p[PARTS<IO>];
-          const u32x4 r = ur[j][m / 2];
-          parts_of<IO>(__uint_as_float(r[m % 2 * 2]), __uint_as_float(r[m % 2 * 2 + 1]), p);
-#pragma unroll
-          for (int k = 0; k < PARTS<IO>; ++k) part[k][m] = p[k];
-        }
-#pragma unroll
-        for (int k = PARTS<IO> - 1; k >= 0; --k)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) acc[j][i] = mma<IO>(part[k], bt[i], acc[j][i]);
+        for (int i = 0; i < 8; ++i)
+          if (r0 + 8 * q + i >= last) xr[i] = Io::fill(0);
       }
-    } else {  // fp16 has no range for parts here: a factor per row would not come out of the sum
+      if constexpr (SPLIT) {
+        u32x4 bt[8], part[NJ][PARTS<IO>];
+        transpose8(xr, bt);
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        float xv[VEC];
-        Io::unpack(xr[s], xv);
+        for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            uint32_t p[PARTS<IO>];
+            const u32x4 r = ur[j][m / 2];
+            parts_of<IO>(__uint_as_float(r[m % 2 * 2]), __uint_as_float(r[m % 2 * 2 + 1]), p);
+#pragma unroll
+            for (int k = 0; k < PARTS<IO>; ++k) part[j][k][m] = p[k];
+          }
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) acc[j][i] = mma<IO>(part[j][0], bt[i], acc[j][i]);
+        }
+        if (again) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) bt[i] = finite_bf16(bt[i]);
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int k = 1; k < PARTS<IO>; ++k) part[j][k] = finite_bf16(part[j][k]);
+        }
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ur[j][s / 4][s % 4]), xv[i], acc[j][i], 0, 0, 0);
+          for (int k = 1; k < PARTS<IO>; ++k)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[j][i] = mma<IO>(part[j][k], bt[i], acc[j][i]);
+      } else {  // fp16 has no range for parts here: a factor per row would not come out of the sum
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          float xv[VEC];
+          Io::unpack(xr[s], xv);
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+              acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ur[j][s / 4][s % 4]), xv[i], acc[j][i], 0, 0, 0);
+        }
       }
     }
-  }
+    if (again) break;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) again |= SPLIT && unsure<VEC>(acc[j]);
+  } while (again);
 #pragma unroll
   for (int half = 2; half > 0; half /= 2) {
     if (wave >= half && wave < 2 * half) {
