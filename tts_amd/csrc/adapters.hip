@@ -782,10 +782,9 @@ int padded_rank(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : 64; }
 template <class IO, int RP, int WV, int MF, bool ADD>
 int launch_waves(AddArgs a, int64_t tiles, int splits, hipStream_t s) {
   a.splits = splits;
-  TTSX_ARG(tiles * splits <= most_workgroups(WV * 64), "ttsx_adapter: too many rows");
-  adapter_kernel<IO, RP, WV, MF, ADD><<<(unsigned)(tiles * splits), WV * 64, 0, s>>>(a);
-  TTSX_LAUNCH_CHECK();
-  return TTSX_OK;
+  const char* name = ADD ? "ttsx_adapter_add" : "ttsx_adapter_backward";
+  TTSX_ARG(tiles * splits <= most_workgroups(WV * 64), "%s: too many rows", name);
+  return launch_kernel(name, adapter_kernel<IO, RP, WV, MF, ADD>, tiles * splits, WV * 64, s, a);
 }
 // Four waves to a tile where the tiles fill 256 CUs twice.  Fewer tiles get a workgroup of 16 waves each (8 at rank 64,
 // whose operands need the registers) and share their columns among up to 256 workgroups; each of those repeats the
@@ -841,25 +840,24 @@ template <class IO, int RP>
 int run_backward(AddArgs a, const BackPlan& p, int B, float* ws, void* ddown, void* dup, hipStream_t s) {
   float *du = ws, *u = du + p.hidden, *part = u + p.hidden;
   a.first.keep = du, a.second.keep = u;
-  const int rc = launch_tiles<IO, RP, false>(a, B, s);
-  if (rc != TTSX_OK) return rc;
   OuterArgs o{};
   o.x = a.second.x, o.x_bs = a.second.bs, o.x_ts = a.second.ts;
   o.dy = a.first.x, o.dy_bs = a.first.bs, o.dy_ts = a.first.ts;
   o.du = du, o.u = u, o.voices = a.voices, o.lengths = a.lengths, o.part = part;
   o.T = a.T, o.K = a.second.K, o.N = a.first.K, o.V = a.V, o.chunks = p.chunks, o.span = p.span, o.tiles = ceil_div(a.T, ROWS);
   const int64_t grid = (int64_t)B * p.chunks * (ceil_div(o.K, 16 * IO::VEC) + ceil_div(o.N, 16 * IO::VEC)) * RANK_PARTS<IO, RP>;
-  TTSX_ARG(grid <= most_workgroups(WAVES * 64), "ttsx_adapter_backward: too many rows");
-  outer_kernel<IO, RP><<<(unsigned)grid, WAVES * 64, 0, s>>>(o);
-  TTSX_LAUNCH_CHECK();
   GatherArgs g{};
   g.part = part, g.voices = a.voices, g.lengths = a.lengths, g.ddown = ddown, g.dup = dup;
   g.B = B, g.T = a.T, g.K = o.K, g.N = o.N, g.R = a.R, g.RP = RP, g.chunks = p.chunks, g.span = p.span;
   const int64_t outs = (int64_t)a.V * a.R * ceil_div(o.K + o.N, LISTED * 4);
-  TTSX_ARG(outs <= most_workgroups(LISTED), "ttsx_adapter_backward: too many voices");
-  gather_kernel<IO><<<(unsigned)outs, LISTED, 0, s>>>(g);
-  TTSX_LAUNCH_CHECK();
-  return TTSX_OK;
+  // nothing is queued before all is known to fit
+  const char* name = "ttsx_adapter_backward";
+  TTSX_ARG(grid <= most_workgroups(WAVES * 64), "%s: too many rows", name);
+  TTSX_ARG(outs <= most_workgroups(LISTED), "%s: too many voices", name);
+  int rc = launch_tiles<IO, RP, false>(a, B, s);
+  if (rc == TTSX_OK) rc = launch_kernel(name, outer_kernel<IO, RP>, grid, WAVES * 64, s, o);
+  if (rc == TTSX_OK) rc = launch_kernel(name, gather_kernel<IO>, outs, LISTED, s, g);
+  return rc;
 }
 
 template <class IO>

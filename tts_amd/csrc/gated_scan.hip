@@ -617,22 +617,12 @@ int launch(ScanArgs a, int B, size_t ws_bytes, bool backward, hipStream_t s) {
   TTSX_ARG(p.chunks == 1 || (a.pairs && ws_bytes >= pairs_bytes<S>(B, a.T, a.D, backward)), "%s: workspace too small", name);
   const int64_t grid = (int64_t)B * p.cols * p.chunks;
   TTSX_ARG(grid <= most_workgroups(WAVES * 64), "%s: too many requests of so many channels", name);
-  const dim3 g((unsigned)grid), t(WAVES * 64);
   if (p.chunks > 1) {
-    if (backward)
-      fold_kernel<S, true><<<g, t, 0, s>>>(a);
-    else
-      fold_kernel<S, false><<<g, t, 0, s>>>(a);
-    TTSX_LAUNCH_CHECK();
+    const int rc = launch_kernel(name, backward ? fold_kernel<S, true> : fold_kernel<S, false>, grid, WAVES * 64, s, a);
+    if (rc != TTSX_OK) return rc;
   }
-  if (backward)
-    scan_backward_kernel<S><<<g, t, 0, s>>>(a);
-  else if (a.states)
-    scan_kernel<S, true><<<g, t, 0, s>>>(a);
-  else
-    scan_kernel<S, false><<<g, t, 0, s>>>(a);
-  TTSX_LAUNCH_CHECK();
-  return TTSX_OK;
+  return launch_kernel(name, backward ? scan_backward_kernel<S> : a.states ? scan_kernel<S, true> : scan_kernel<S, false>, grid,
+                       WAVES * 64, s, a);
 }
 
 // The widest row stride: the offsets inside a tile fit 32 bits.
@@ -660,10 +650,8 @@ int launch_step(const void* x, int64_t x_bs, const void* g, int64_t g_bs, const 
   typedef typename IO::elem E;
   const int64_t grid = ((int64_t)B * (D / N) + 255) / 256;
   TTSX_ARG(grid <= most_workgroups(256), "ttsx_gated_step: too many requests of so many channels");
-  step_kernel<IO, N><<<(unsigned)grid, 256, 0, s>>>(static_cast<const E*>(x), x_bs, static_cast<const E*>(g), g_bs, h, B,
-                                                    D, static_cast<E*>(y), h_out);
-  TTSX_LAUNCH_CHECK();
-  return TTSX_OK;
+  return launch_kernel("ttsx_gated_step", step_kernel<IO, N>, grid, 256, s, static_cast<const E*>(x), x_bs,
+                       static_cast<const E*>(g), g_bs, h, B, D, static_cast<E*>(y), h_out);
 }
 template <class IO>
 int run_step(const void* x, int64_t x_bs, const void* g, int64_t g_bs, const float* h, int B, int D, void* y,

@@ -2,7 +2,8 @@
 // rows is bound by its host side, and checking, allocating and converting its arguments in Python takes longer than the
 // launch.  Every function here either makes the whole call or, where an argument is anything but ordinary (another type,
 // device or layout, a host list, an autograd input, a partial overlap), does nothing and returns None: the caller then goes
-// through its own checks, which convert or refuse it.  The entry points are those of libttsx.so (ttsx_seq.h), bound by address.
+// through its own checks, which convert or refuse it.  What fails behind those checks is raised here: the call may have been
+// queued in part, and is not made again.  The entry points are those of libttsx.so (ttsx_seq.h), bound by address.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -96,8 +97,17 @@ struct Scratch {
   void* data() const { return bytes > 0 ? t.data_ptr() : nullptr; }
 };
 
-PyObject* ordinary(bool done, std::initializer_list<at::Tensor> out) {
-  if (!done) Py_RETURN_NONE;
+// The results of the entry point `name`, if it returned TTSX_OK.  An argument it refused was refused before any launch.
+PyObject* ordinary(int rc, const char* name, std::initializer_list<at::Tensor> out) {
+  if (rc == TTSX_ERR_ARG) Py_RETURN_NONE;
+  if (rc != TTSX_OK) {
+    PyObject* lib = PyImport_ImportModule("tts_amd._lib");
+    PyObject* done = lib ? PyObject_CallMethod(lib, "check", "is", rc, name) : nullptr;  // raises
+    Py_XDECREF(lib);
+    Py_XDECREF(done);
+    if (done) PyErr_Format(PyExc_RuntimeError, "%s failed (%d)", name, rc);
+    return nullptr;
+  }
   if (out.size() == 1) return THPVariable_Wrap(*out.begin());
   PyObject* tuple = PyTuple_New((Py_ssize_t)out.size());
   if (!tuple) return nullptr;
@@ -113,12 +123,12 @@ PyObject* ordinary(bool done, std::initializer_list<at::Tensor> out) {
   return tuple;
 }
 template <class F>
-bool run(F f) {
+int run(F f) {
   int rc;
   Py_BEGIN_ALLOW_THREADS;
   rc = f();
   Py_END_ALLOW_THREADS;
-  return rc == TTSX_OK;
+  return rc;
 }
 
 bool counts(Py_ssize_t n, Py_ssize_t want) {
@@ -142,11 +152,11 @@ PyObject* step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   const at::Tensor y = fresh(*x, {B, D}, x->scalar_type()), next = into ? *h : fresh(*x, {B, D}, at::kFloat);
   void* s = c.stream();
-  const bool done = run([&] {
+  const int rc = run([&] {
     return entry.step(x->data_ptr(), x->stride(0), g->data_ptr(), g->stride(0), h.data<float>(), (int)B, (int)D, type,
                       y.data_ptr(), static_cast<float*>(next.data_ptr()), s);
   });
-  return ordinary(done, {y, next});
+  return ordinary(rc, "ttsx_gated_step", {y, next});
   END_HANDLE_TH_ERRORS
 }
 
@@ -175,14 +185,14 @@ PyObject* scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::Tensor states;
   if (save) states = fresh(*x, {B, (T + TTSX_STATE_BLOCK - 1) / TTSX_STATE_BLOCK, D}, at::kFloat);
   void* s = c.stream();
-  const bool done = run([&] {
+  const int rc = run([&] {
     return entry.scan(x->data_ptr(), x->stride(0), x->stride(1), g->data_ptr(), g->stride(0), g->stride(1), h0.data<float>(),
                       lengths.data<int32_t>(), (int)B, (int)T, (int)D, type, reverse, h.data_ptr(),
                       static_cast<float*>(last.data_ptr()), save ? static_cast<float*>(states.data_ptr()) : nullptr, ws.data(),
                       (size_t)ws.bytes, s);
   });
-  if (save) return ordinary(done, {h, last, states});
-  return ordinary(done, {h, last});
+  if (save) return ordinary(rc, "ttsx_gated_scan", {h, last, states});
+  return ordinary(rc, "ttsx_gated_scan", {h, last});
   END_HANDLE_TH_ERRORS
 }
 
@@ -208,13 +218,13 @@ PyObject* scan_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor dx = fresh(*x, {B, T, D}, x->scalar_type()), dg = fresh(*x, {B, T, D}, x->scalar_type()),
                    dh0 = fresh(*x, {B, D}, at::kFloat);
   void* s = c.stream();
-  const bool done = run([&] {
+  const int rc = run([&] {
     return entry.scan_backward(dh->data_ptr(), dh->stride(0), dh->stride(1), x->data_ptr(), x->stride(0), x->stride(1),
                                g->data_ptr(), g->stride(0), g->stride(1), states.data<float>(), dh_last.data<float>(),
                                lengths.data<int32_t>(), (int)B, (int)T, (int)D, type, reverse, dx.data_ptr(), dg.data_ptr(),
                                static_cast<float*>(dh0.data_ptr()), ws.data(), (size_t)ws.bytes, s);
   });
-  return ordinary(done, {dx, dg, dh0});
+  return ordinary(rc, "ttsx_gated_scan_backward", {dx, dg, dh0});
   END_HANDLE_TH_ERRORS
 }
 
@@ -255,12 +265,12 @@ PyObject* adapter_add(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor out = into ? *y : fresh(*y, y->sizes(), y->scalar_type());
   const int type = type_of(*x);
   void* s = c.stream();
-  const bool done = run([&] {
+  const int rc = run([&] {
     return entry.add(y->data_ptr(), y->stride(0), row_stride(*y), x->data_ptr(), x->stride(0), row_stride(*x), down->data_ptr(),
                      up->data_ptr(), voices.data<int32_t>(), scale.data<float>(), lengths.data<int32_t>(), (int)z.B, (int)z.T,
                      (int)z.K, (int)z.N, (int)z.R, (int)z.V, type, out.data_ptr(), out.stride(0), row_stride(out), s);
   });
-  return ordinary(done, {out});
+  return ordinary(rc, "ttsx_adapter_add", {out});
   END_HANDLE_TH_ERRORS
 }
 
@@ -279,13 +289,13 @@ PyObject* adapter_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor dx = fresh(*x, x->sizes(), x->scalar_type()), ddown = fresh(*x, down->sizes(), x->scalar_type()),
                    dup = fresh(*x, up->sizes(), x->scalar_type());
   void* s = c.stream();
-  const bool done = run([&] {
+  const int rc = run([&] {
     return entry.add_backward(dy->data_ptr(), dy->stride(0), row_stride(*dy), x->data_ptr(), x->stride(0), row_stride(*x),
                               down->data_ptr(), up->data_ptr(), voices.data<int32_t>(), scale.data<float>(),
                               lengths.data<int32_t>(), (int)z.B, (int)z.T, (int)z.K, (int)z.N, (int)z.R, (int)z.V, type,
                               dx.data_ptr(), ddown.data_ptr(), dup.data_ptr(), ws.data(), (size_t)ws.bytes, s);
   });
-  return ordinary(done, {dx, ddown, dup});
+  return ordinary(rc, "ttsx_adapter_backward", {dx, ddown, dup});
   END_HANDLE_TH_ERRORS
 }
 

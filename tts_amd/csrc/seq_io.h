@@ -177,6 +177,19 @@ __device__ static inline void store_f32_some(float* p, int n, const float* v) {
 // The widest grid of workgroups of that many threads: a launch counts its threads in 32 bits.
 constexpr int64_t most_workgroups(int threads) { return 0xffffffffLL / threads; }
 
+// A launch and its own status: an error that an earlier call left behind is not this one's.  (hipGetLastError would report it
+// although the kernel is queued, and a caller that took that for a refusal would update its state a second time.)
+template <class... P>
+inline int launch_kernel(const char* name, void (*kernel)(P...), int64_t grid, int threads, hipStream_t s,
+                         typename std::common_type<P>::type... args) {
+  void* p[] = {&args...};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3((unsigned)grid), dim3(threads), p, 0, s);
+  if (e == hipSuccess) return TTSX_OK;
+  (void)hipGetLastError();  // reported here, and by nobody else
+  ttsx_set_error("%s: launch -> %s", name, hipGetErrorString(e));
+  return TTSX_ERR_HIP;
+}
+
 // A row of a ragged batch is valid below this.
 __device__ static inline int valid_rows(const int32_t* lengths, int b, int T) {
   return lengths ? min(max(lengths[b], 0), T) : T;
