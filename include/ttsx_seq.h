@@ -8,7 +8,8 @@
  *   - activations are 32-bit floats or one of two 16-bit kinds (TTSX_F32 / _BF16 / _F16); what is summed, scanned or
  *     kept from step to step is fp32;
  *   - an activation [B,T,D] has its last axis contiguous and two strides, of the batch and of the row, in ELEMENTS;
- *     inputs may overlap or repeat (a stride of 0); a pointer is aligned to its element, no further;
+ *     inputs may overlap or repeat (a stride of 0), and with T = 1 the row stride is not looked at; a pointer is
+ *     aligned to its element, no further;
  *   - nothing is allocated and nothing synchronises: working memory comes from the caller, the calls can be captured
  *     into a graph, and calls that share no output and no workspace can run at the same time;
  *   - lengths [B] int32 or NULL (= T) is read on the device and clamped to 0..T; rows at positions >= length are not

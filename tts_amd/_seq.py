@@ -92,9 +92,9 @@ def pointer(t):
 
 
 def rows(t, furthest=None):
-    """t with a contiguous last axis; other strides stay, up to `furthest` between rows."""
+    """t with a contiguous last axis; other strides stay, up to `furthest` between rows (a single row lies anywhere)."""
     strides = t.stride()
-    if (strides[-1] != 1 and t.shape[-1] > 1) or (furthest is not None and strides[-2] > furthest):
+    if (strides[-1] != 1 and t.shape[-1] > 1) or (furthest is not None and t.shape[-2] > 1 and strides[-2] > furthest):
         return t.contiguous()
     return t
 

@@ -889,6 +889,7 @@ extern "C" int ttsx_adapter_add(const void* y, int64_t y_batch_stride, int64_t y
   TTSX_ARG(shape_ok(B, T, K, N, R, V), "ttsx_adapter_add: bad shape B=%d T=%d K=%d N=%d R=%d V=%d (1 <= R <= %d)", B, T,
            K, N, R, V, TTSX_ADAPTER_MAX_RANK);
   TTSX_ARG(dtype_ok(dtype), "ttsx_adapter_add: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
+  y_row_stride = stride_of(T, y_row_stride), x_row_stride = stride_of(T, x_row_stride), out_row_stride = stride_of(T, out_row_stride);
   TTSX_ARG(stride_ok(y_row_stride) && stride_ok(x_row_stride) && stride_ok(out_row_stride),
            "ttsx_adapter_add: a row stride outside 0..%ld", (long)MAX_STRIDE);
   TTSX_ARG(out != y || (out_batch_stride == y_batch_stride && out_row_stride == y_row_stride),
@@ -919,6 +920,7 @@ extern "C" int ttsx_adapter_backward(const void* dy, int64_t dy_batch_stride, in
   TTSX_ARG(shape_ok(B, T, K, N, R, V), "ttsx_adapter_backward: bad shape B=%d T=%d K=%d N=%d R=%d V=%d (1 <= R <= %d)",
            B, T, K, N, R, V, TTSX_ADAPTER_MAX_RANK);
   TTSX_ARG(dtype_ok(dtype), "ttsx_adapter_backward: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
+  dy_row_stride = stride_of(T, dy_row_stride), x_row_stride = stride_of(T, x_row_stride);
   TTSX_ARG(stride_ok(dy_row_stride) && stride_ok(x_row_stride), "ttsx_adapter_backward: a row stride outside 0..%ld",
            (long)MAX_STRIDE);
   const BackPlan p = back_plan(B, T, K, N, R, dtype == TTSX_F32 ? 4 : 8);

@@ -679,6 +679,7 @@ extern "C" int ttsx_gated_scan(const void* x, int64_t x_batch_stride, int64_t x_
   TTSX_ARG(x && g && h && h_last, "ttsx_gated_scan: null argument");
   TTSX_ARG(shape_ok(B, T, D), "ttsx_gated_scan: bad shape B=%d T=%d D=%d", B, T, D);
   TTSX_ARG(dtype_ok(dtype), "ttsx_gated_scan: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
+  x_row_stride = stride_of(T, x_row_stride), g_row_stride = stride_of(T, g_row_stride);
   TTSX_ARG(stride_ok(x_row_stride) && stride_ok(g_row_stride), "ttsx_gated_scan: a row stride outside 0..%ld",
            (long)MAX_STRIDE);
   ScanArgs a{};
@@ -701,6 +702,7 @@ extern "C" int ttsx_gated_scan_backward(const void* dh, int64_t dh_batch_stride,
   TTSX_ARG(dh && x && g && states && dx && dg && dh0, "ttsx_gated_scan_backward: null argument");
   TTSX_ARG(shape_ok(B, T, D), "ttsx_gated_scan_backward: bad shape B=%d T=%d D=%d", B, T, D);
   TTSX_ARG(dtype_ok(dtype), "ttsx_gated_scan_backward: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
+  dh_row_stride = stride_of(T, dh_row_stride), x_row_stride = stride_of(T, x_row_stride), g_row_stride = stride_of(T, g_row_stride);
   TTSX_ARG(stride_ok(dh_row_stride) && stride_ok(x_row_stride) && stride_ok(g_row_stride),
            "ttsx_gated_scan_backward: a row stride outside 0..%ld", (long)MAX_STRIDE);
   ScanArgs a{};

@@ -72,10 +72,10 @@ int type_of(const at::Tensor& t) {
     default: return -1;
   }
 }
-// The last axis contiguous, rows near enough ([B,T,n]; the batch stride is free, and [B,n] has no other).
+// The last axis contiguous, rows near enough ([B,T,n]; the batch stride is free, [B,n] has no other, a single row lies anywhere).
 bool laid_out(const at::Tensor& t) {
   const int64_t d = t.dim();
-  return (t.stride(d - 1) == 1 || t.size(d - 1) == 1) && (d == 2 || t.stride(1) <= FURTHEST);
+  return (t.stride(d - 1) == 1 || t.size(d - 1) == 1) && (d == 2 || t.size(1) == 1 || t.stride(1) <= FURTHEST);
 }
 int64_t row_stride(const at::Tensor& t) { return t.dim() == 3 ? t.stride(1) : 0; }
 bool state_ok(const Arg& a, int64_t B, int64_t D) {

@@ -174,6 +174,9 @@ __device__ static inline void store_f32_some(float* p, int n, const float* v) {
     if (i < n) p[i] = v[i];
 }
 
+// The stride that a call goes by: a single row has no next one.
+inline int64_t stride_of(int T, int64_t stride) { return T > 1 ? stride : 0; }
+
 // The widest grid of workgroups of that many threads: a launch counts its threads in 32 bits.
 constexpr int64_t most_workgroups(int threads) { return 0xffffffffLL / threads; }
 
