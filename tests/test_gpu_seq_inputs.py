@@ -1,6 +1,7 @@
-"""Views that an operator takes: a single row with a far stride."""
+"""Inputs that an operator takes or refuses: a single row with a far stride, tangents of forward-mode differentiation."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +47,31 @@ def test_a_single_row_lies_anywhere(B, dtype, way):
     assert adapter_add(here, _far(x), m, m, voices, out=here) is here and torch.equal(here, out)
     there = _far(x)
     assert adapter_add(g, x, m, m, voices, out=there) is there and torch.equal(there, out)
+
+
+def test_a_tangent_is_refused(way):
+    """The calls give no tangent: an input that carries one is refused as one that requires grad is, with no_grad() too, which
+    leaves forward mode as it is; inside a dual level without tangents nothing changes."""
+    from tts_amd.adapters import adapter_add, adapter_backward
+    from tts_amd.recurrence import gated_scan, gated_scan_backward, gated_step
+    x, m, voices = _rand(2, 5, 8), _rand(2, 4, 8), torch.zeros(2, dtype=torch.int32, device="cuda")
+    h, states = _rand(2, 8), _rand(2, 1, 8)
+    scale = torch.ones(2, device="cuda")
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        dh, dm = forward_ad.make_dual(h, torch.ones_like(h)), forward_ad.make_dual(m, torch.ones_like(m))
+        ds = forward_ad.make_dual(scale, torch.ones_like(scale))
+        calls = [lambda: gated_scan(d, x), lambda: gated_scan(x, d), lambda: gated_scan(x, x, h0=dh),
+                 lambda: gated_scan_backward(d, x, x, states), lambda: gated_scan_backward(x, x, x, states, dh_last=dh),
+                 lambda: gated_step(x[:, 0], x[:, 0], dh), lambda: gated_step(d[:, 0], x[:, 0], h),
+                 lambda: adapter_add(d, x, m, m, voices), lambda: adapter_add(x, x, m, dm, voices),
+                 lambda: adapter_add(x, x, m, m, voices, scale=ds), lambda: adapter_backward(x, d, m, m, voices)]
+        for call in calls:
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                call()
+        want = gated_scan(x, x)
+        primal = forward_ad.unpack_dual(d).primal
+        assert all(torch.equal(a, b) for a, b in zip(want, gated_scan(primal, x)))
+    assert all(torch.equal(a, b) for a, b in zip(want, gated_scan(x, x)))

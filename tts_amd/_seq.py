@@ -7,6 +7,7 @@ import ctypes
 import types
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -64,15 +65,18 @@ def are_tensors(what, *named):
 
 
 def on_device(what, *named):
-    """The index of the one GPU they are all on; none may be part of an autograd graph (None stands for an argument left
-    out)."""
+    """The index of the one GPU they are all on; none may be part of an autograd graph or carry a tangent (None stands for an
+    argument left out)."""
     grad, index = torch.is_grad_enabled(), None
+    tangents = forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled()
     for name, t in named:
         if t is None:
             continue
         if grad and t.requires_grad:
             raise ValueError("%s records no autograd graph: call it under torch.no_grad(); gradients are a call of "
                              "their own" % what)
+        if tangents and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("%s has no forward-mode derivative: %s carries a tangent" % (what, name))
         i = t.get_device() if t.is_cuda else -1
         if index is None:
             index = i

@@ -10,10 +10,10 @@ shared product runs once for all of them, `adapter_add` adds each request's own 
     dx, ddown, dup  = adapter_backward(dy, x, down, up, voices)  # for fitting the adapters
 
 Activations and adapters are float32, bfloat16 or float16 tensors on the GPU, alike in type; products are summed in
-float32.  As elsewhere in this package there is no CPU path and no autograd graph: gradients are a call of their own, so
-inputs that require them are refused outside `torch.no_grad()`.  Calls work on the current stream of the tensors' device,
-allocate through torch and do not synchronise (`voices` or `lengths` on the host are copied over first, which does), so
-they can be captured into a graph.
+float32.  As elsewhere in this package there is no CPU path and no autograd graph: gradients are a call of their own,
+so inputs that require them are refused outside `torch.no_grad()`, and inputs with a tangent anywhere.  Calls work on
+the current stream of the tensors' device, allocate through torch and do not synchronise (`voices` or `lengths` on the
+host are copied over first, which does), so they can be captured into a graph.
 """
 import functools
 

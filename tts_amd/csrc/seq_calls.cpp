@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
@@ -44,7 +45,7 @@ struct Arg {
 
 struct Call {
   int device = -1;
-  bool ok = true, grad = c10::GradMode::is_enabled();
+  bool ok = true, grad = c10::GradMode::is_enabled(), tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   Call() { ok = entry.step && !c10::impl::dispatch_mode_enabled(); }
   Arg take(PyObject* o, bool optional = false) {
     Arg a;
@@ -54,7 +55,7 @@ struct Call {
       return a;
     }
     const at::Tensor& t = THPVariable_Unpack(o);
-    ok = t.is_cuda() && t.layout() == at::kStrided && !(grad && t.requires_grad());
+    ok = t.is_cuda() && t.layout() == at::kStrided && !(grad && t.requires_grad()) && !(tangents && t._fw_grad(0).defined());
     if (ok && device < 0) device = c10::hip::current_device();
     ok = ok && t.get_device() == device;
     a.t = &t;

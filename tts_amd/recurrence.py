@@ -12,10 +12,10 @@ thousands of positions costs one pass over its activations.  The reference has n
     y, h               = gated_step(x, g, h)                    # the next position of every stream
 
 Values and gate logits are float32, bfloat16 or float16 tensors on the GPU, alike in type; states are float32 whatever
-that type.  As elsewhere in this package there is no CPU path and no autograd graph: gradients are a call of their own, so
-inputs that require them are refused outside `torch.no_grad()`.  Every call works on the current stream of the tensors'
-device, allocates through torch and does not synchronise (a `lengths` on the host is copied over first, which does),
-so it can be captured into a graph.
+that type.  As elsewhere in this package there is no CPU path and no autograd graph: gradients are a call of their own,
+so inputs that require them are refused outside `torch.no_grad()`, and inputs with a tangent anywhere.  Every call
+works on the current stream of the tensors' device, allocates through torch and does not synchronise (a `lengths` on
+the host is copied over first, which does), so it can be captured into a graph.
 """
 import functools
 
