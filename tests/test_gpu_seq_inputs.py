@@ -1,4 +1,5 @@
-"""Inputs that an operator takes or refuses: a single row with a far stride, tangents of forward-mode differentiation."""
+"""Inputs that an operator takes or refuses: a single row with a far stride, tangents of forward-mode differentiation, negated
+views."""
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -75,3 +76,20 @@ def test_a_tangent_is_refused(way):
         primal = forward_ad.unpack_dual(d).primal
         assert all(torch.equal(a, b) for a, b in zip(want, gated_scan(primal, x)))
     assert all(torch.equal(a, b) for a, b in zip(want, gated_scan(x, x)))
+
+
+def test_a_negated_view_is_refused(way):
+    """The imaginary part of a conjugate is a view with its sign in a flag, which a kernel would not see."""
+    from tts_amd.adapters import adapter_add, adapter_backward
+    from tts_amd.recurrence import gated_scan, gated_scan_backward, gated_step
+    z = torch.randn(2, 5, 8, dtype=torch.complex64, device="cuda")
+    neg = z.conj().imag
+    assert neg.is_neg()
+    x, m, voices, states = _rand(2, 5, 8), _rand(2, 4, 8), torch.zeros(2, dtype=torch.int32, device="cuda"), _rand(2, 1, 8)
+    for call in (lambda: gated_scan(neg, x), lambda: gated_scan(x, x, h0=neg[:, 0]), lambda: gated_step(x[:, 0], neg[:, 0], x[:, 1]),
+                 lambda: gated_scan_backward(neg, x, x, states), lambda: gated_scan_backward(x, x, x, neg[:, :1]),
+                 lambda: adapter_add(x, neg, m, m, voices), lambda: adapter_backward(neg, x, m, m, voices),
+                 lambda: adapter_add(x, x, m, m, voices, scale=neg[:, 0, 0])):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call()
+    assert all(torch.equal(a, b) for a, b in zip(gated_scan(neg.resolve_neg(), x), gated_scan(-z.imag, x)))

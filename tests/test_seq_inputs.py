@@ -19,3 +19,11 @@ def test_a_tangent_is_refused():
             gated_scan(forward_ad.unpack_dual(d).primal, x)
     with pytest.raises(_lib.TtsxError, match="no CPU path"):
         gated_scan(d, x)
+
+
+def test_a_negated_view_is_refused():
+    from tts_amd.recurrence import gated_scan
+    x, neg = torch.zeros(2, 5, 8), torch.zeros(2, 5, 8, dtype=torch.complex64).conj().imag
+    for args in ((neg, x), (x, neg)):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            gated_scan(*args)

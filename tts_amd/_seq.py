@@ -65,8 +65,8 @@ def are_tensors(what, *named):
 
 
 def on_device(what, *named):
-    """The index of the one GPU they are all on; none may be part of an autograd graph or carry a tangent (None stands for an
-    argument left out)."""
+    """The index of the one GPU they are all on; none may be part of an autograd graph, carry a tangent or be a negated view (None
+    stands for an argument left out)."""
     grad, index = torch.is_grad_enabled(), None
     tangents = forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled()
     for name, t in named:
@@ -77,6 +77,8 @@ def on_device(what, *named):
                              "their own" % what)
         if tangents and forward_ad.unpack_dual(t).tangent is not None:
             raise ValueError("%s has no forward-mode derivative: %s carries a tangent" % (what, name))
+        if t.is_neg():
+            raise ValueError("%s: %s is a view that negates what it shows: pass its resolve_neg()" % (what, name))
         i = t.get_device() if t.is_cuda else -1
         if index is None:
             index = i

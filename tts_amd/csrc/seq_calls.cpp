@@ -55,7 +55,7 @@ struct Call {
       return a;
     }
     const at::Tensor& t = THPVariable_Unpack(o);
-    ok = t.is_cuda() && t.layout() == at::kStrided && !(grad && t.requires_grad()) && !(tangents && t._fw_grad(0).defined());
+    ok = t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() && !(grad && t.requires_grad()) && !(tangents && t._fw_grad(0).defined());
     if (ok && device < 0) device = c10::hip::current_device();
     ok = ok && t.get_device() == device;
     a.t = &t;

@@ -56,7 +56,11 @@ def _state(what, name, t, B, D):
     are_tensors(what, (name, t))
     if t.shape != (B, D) or t.dtype != torch.float32:
         raise ValueError("%s: %s must be float32 [%d, %d], got %s %s" % (what, name, B, D, t.dtype, tuple(t.shape)))
-    return t.contiguous()
+    return t
+
+
+def _contiguous(t):
+    return None if t is None else t.contiguous()
 
 
 def gated_scan(x, g, h0=None, lengths=None, reverse=False, save_states=False):
@@ -77,6 +81,7 @@ def gated_scan(x, g, h0=None, lengths=None, reverse=False, save_states=False):
     B, T, D = x.shape
     h0 = _state(what, "h0", h0, B, D)
     dev = on_device(what, ("x", x), ("g", g), ("h0", h0))
+    h0 = _contiguous(h0)
     lengths = lengths_on(what, lengths, B, T, x)
     x, g = rows(x, FURTHEST), rows(g, FURTHEST)
     h = x.new_empty((B, T, D))
@@ -114,6 +119,7 @@ def gated_scan_backward(dh, x, g, states, dh_last=None, lengths=None, reverse=Fa
                          % (what, B, blocks, D, states.dtype, tuple(states.shape)))
     dh_last = _state(what, "dh_last", dh_last, B, D)
     dev = on_device(what, ("x", x), ("g", g), ("dh", dh), ("states", states), ("dh_last", dh_last))
+    dh_last = _contiguous(dh_last)
     lengths = lengths_on(what, lengths, B, T, x)
     dh, x, g, states = rows(dh, FURTHEST), rows(x, FURTHEST), rows(g, FURTHEST), states.contiguous()
     dx, dg = x.new_empty((B, T, D)), x.new_empty((B, T, D))
@@ -141,10 +147,11 @@ def gated_step(x, g, h, out=None):
     _values_and_gates(what, x, g, "BD")
     are_tensors(what, ("h", h))
     B, D = x.shape
-    state = _state(what, "h", h, B, D)
+    _state(what, "h", h, B, D)
     if out is not None:
         are_tensors(what, ("out", out))
     dev = on_device(what, ("x", x), ("g", g), ("h", h), ("out", out))
+    state = h.contiguous()
     if out is None:
         out = torch.empty_like(state)
     else:
