@@ -1,5 +1,5 @@
-"""Inputs that an operator takes or refuses: a single row with a far stride, tangents of forward-mode differentiation, negated
-views."""
+"""Inputs that an operator takes or refuses: a single row with a far stride, tangents of forward-mode differentiation, negated views,
+results placed over indices."""
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -93,3 +93,21 @@ def test_a_negated_view_is_refused(way):
         with pytest.raises(ValueError, match="resolve_neg"):
             call()
     assert all(torch.equal(a, b) for a, b in zip(gated_scan(neg.resolve_neg(), x), gated_scan(-z.imag, x)))
+
+
+def test_a_result_over_the_indices_is_refused(way):
+    """voices and lengths are read while out is written."""
+    from tts_amd.adapters import adapter_add
+    x, m = _rand(2, 1, 8), _rand(2, 4, 8)
+    buf = torch.zeros(64, dtype=torch.int32, device="cuda")
+    out = buf[:16].view(torch.float32).view(2, 1, 8)
+    index = buf[14:16]
+    with pytest.raises(ValueError, match="out overlaps voices"):
+        adapter_add(x, x, m, m, index, out=out)
+    with pytest.raises(ValueError, match="out overlaps voices"):
+        adapter_add(out, x, m, m, index, out=out)
+    with pytest.raises(ValueError, match="out overlaps lengths"):
+        adapter_add(x, x, m, m, buf[32:34], lengths=index, out=out)
+    assert adapter_add(out, x, m, m, buf[32:34], lengths=buf[34:36], out=out) is out
+    with pytest.raises(ValueError, match="out overlaps voices"):
+        adapter_add(x, x, m, m, buf[8:12].view(torch.int64), out=out)

@@ -109,6 +109,9 @@ def adapter_add(y, x, down, up, voices, scale=None, lengths=None, out=None):
             raise ValueError("%s: out overlaps x" % what)
         if overlapping(out, (down, up) if scale is None else (down, up, scale)) is not None:
             raise ValueError("%s: out overlaps an adapter" % what)
+        for name, t in (("voices", voices), ("lengths", lengths)):
+            if isinstance(t, torch.Tensor) and t.is_cuda and overlaps(out, t):
+                raise ValueError("%s: out overlaps %s" % (what, name))
     voices = voices_on(what, voices, B, V, x)
     lengths = lengths_on(what, lengths, B, T, x)
     if out is None:
