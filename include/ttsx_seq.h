@@ -29,13 +29,19 @@ extern "C" {
 #define TTSX_BF16 1
 #define TTSX_F16 2
 
+/* The largest calls: channels or columns and elements between two rows; requests, and steps or positions; voices. */
+#define TTSX_SEQ_MAX_WIDTH (1 << 20)
+#define TTSX_SEQ_MAX_ROWS (1 << 30)
+#define TTSX_SEQ_MAX_VOICES (1 << 24)
+
 /* Steps between two states that ttsx_gated_scan keeps for its backward pass. */
 #define TTSX_STATE_BLOCK 64
 
 /* ------------------------------------------------------------------ gated linear recurrence
  *   f_t = sigmoid(g_t)      h_t = f_t h_{t-1} + (1 - f_t) x_t
  * per channel, over the rows 0 .. length-1 of each request, or from row length-1 down to 0 where `reverse` is set.
- *   x, g     [B,T,D]  values and gate logits (may be two slices of one projection); D and the row strides up to 2^20
+ *   x, g     [B,T,D]  values and gate logits (may be two slices of one projection); D and the row strides up to
+ *                    TTSX_SEQ_MAX_WIDTH
  *   h0       [B,D] fp32 state in front of the first step, or NULL (= 0)
  *   h        [B,T,D] contiguous, of x's type; rows at positions >= length are zero
  *   h_last   [B,D] fp32 state behind the last step (h0 for an empty request)
@@ -72,7 +78,7 @@ int ttsx_gated_step(const void* x, int64_t x_batch_stride, const void* g, int64_
  *   y, out   [B,T,N]   out may be y itself (in place), and overlaps no other argument
  *   x        [B,T,K]
  *   down     [V,R,K], up [V,R,N], contiguous, of x's type; 1 <= R <= TTSX_ADAPTER_MAX_RANK; K, N and the row strides
- *            up to 2^20
+ *            up to TTSX_SEQ_MAX_WIDTH, V to TTSX_SEQ_MAX_VOICES
  *   voices   [B] int32; a voice outside 0..V-1 has no adapter
  *   scale    [V] fp32 or NULL (= 1)
  * Rows without an adapter (no voice, or at positions >= length) are y's.  x down^T and the sum are fp32; out is

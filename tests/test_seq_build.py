@@ -1,5 +1,7 @@
-"""What `make` builds, as it would (-n): the C library needs no torch, the calls from Python are built beside it where there is one."""
+"""What `make` builds, as it would (-n): the C library needs no torch, the calls from Python are built beside it where there is one;
+and the limits that header, library and Python share."""
 import os
+import re
 import subprocess
 import sys
 
@@ -27,3 +29,16 @@ def test_the_calls_with_torch():
     lines = got.stdout.replace("\\\n", " ").split("\n")
     line = next(part for part in lines if "seq_calls.cpp" in part)
     assert "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch.compiled_with_cxx11_abi() in line and "left out" not in got.stdout
+
+
+def test_the_limits_are_the_headers():
+    """The largest sizes stand in include/ttsx_seq.h; the checks in Python name the same."""
+    from tts_amd import adapters, recurrence
+    header = open(os.path.join(ROOT, "include", "ttsx_seq.h")).read()
+    limits = {name: 1 << int(bits) for name, bits in re.findall(r"#define TTSX_SEQ_MAX_(\w+) \(1 << (\d+)\)", header)}
+    assert limits == {"WIDTH": adapters.MAX_WIDTH, "ROWS": adapters.MAX_ROWS, "VOICES": adapters.MAX_VOICES}
+    assert adapters.FURTHEST == recurrence.FURTHEST == recurrence.MAX_CHANNELS == limits["WIDTH"]
+    assert recurrence.MAX_STEPS == limits["ROWS"]
+    for source in ("gated_scan.hip", "adapters.hip", "seq_calls.cpp"):
+        code = re.sub(r"//.*", "", open(os.path.join(ROOT, "tts_amd", "csrc", source)).read())
+        assert not re.search(r"1 << (20|24|30)\b", code)            # no second copy beside the header's

@@ -612,8 +612,8 @@ __global__ __launch_bounds__(WAVES * 64, 3) void outer_kernel(OuterArgs a) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) hidden_rows<RP>(ub, (int64_t)b * a.tiles + r0 / ROWS, j0 + j, lane, ur[j]);
   };
-  // A sum over parts is no number where a factor is infinite (see `unsure`).  The wave then takes its rows once more with zero in the
-  // place of what is not finite wherever other parts than the first are multiplied.
+  // A sum over parts is no number where a factor is infinite (see `unsure`).  The wave then takes its rows once more with zero
+  // in the place of what is not finite wherever other parts than the first are multiplied.
   constexpr bool SPLIT = IO::INF == IoBf16::INF;
   bool again = false;
   do {
@@ -869,12 +869,11 @@ int run_backward_any(const AddArgs& a, const BackPlan& p, int B, float* ws, void
   }
 }
 
-// The widest row: the offsets inside a tile, and inside an adapter, fit 32 bits.
-constexpr int64_t MAX_STRIDE = 1 << 20;
-bool stride_ok(int64_t s) { return s >= 0 && s <= MAX_STRIDE; }
+// The offsets inside a tile, and inside an adapter, fit 32 bits.
+bool stride_ok(int64_t s) { return s >= 0 && s <= TTSX_SEQ_MAX_WIDTH; }
 bool shape_ok(int B, int T, int K, int N, int R, int V) {
-  return B >= 1 && T >= 1 && K >= 1 && N >= 1 && R >= 1 && R <= TTSX_ADAPTER_MAX_RANK && V >= 1 && T <= (1 << 30) &&
-         K <= MAX_STRIDE && N <= MAX_STRIDE && V <= (1 << 24);
+  return B >= 1 && T >= 1 && K >= 1 && N >= 1 && R >= 1 && R <= TTSX_ADAPTER_MAX_RANK && V >= 1 && T <= TTSX_SEQ_MAX_ROWS &&
+         K <= TTSX_SEQ_MAX_WIDTH && N <= TTSX_SEQ_MAX_WIDTH && V <= TTSX_SEQ_MAX_VOICES;
 }
 bool dtype_ok(int d) { return d == TTSX_F32 || d == TTSX_BF16 || d == TTSX_F16; }
 
@@ -889,9 +888,10 @@ extern "C" int ttsx_adapter_add(const void* y, int64_t y_batch_stride, int64_t y
   TTSX_ARG(shape_ok(B, T, K, N, R, V), "ttsx_adapter_add: bad shape B=%d T=%d K=%d N=%d R=%d V=%d (1 <= R <= %d)", B, T,
            K, N, R, V, TTSX_ADAPTER_MAX_RANK);
   TTSX_ARG(dtype_ok(dtype), "ttsx_adapter_add: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
-  y_row_stride = stride_of(T, y_row_stride), x_row_stride = stride_of(T, x_row_stride), out_row_stride = stride_of(T, out_row_stride);
+  y_row_stride = stride_of(T, y_row_stride), x_row_stride = stride_of(T, x_row_stride);
+  out_row_stride = stride_of(T, out_row_stride);
   TTSX_ARG(stride_ok(y_row_stride) && stride_ok(x_row_stride) && stride_ok(out_row_stride),
-           "ttsx_adapter_add: a row stride outside 0..%ld", (long)MAX_STRIDE);
+           "ttsx_adapter_add: a row stride outside 0..%ld", (long)TTSX_SEQ_MAX_WIDTH);
   TTSX_ARG(out != y || (out_batch_stride == y_batch_stride && out_row_stride == y_row_stride),
            "ttsx_adapter_add: out is y with other strides");
   AddArgs a{};
@@ -922,7 +922,7 @@ extern "C" int ttsx_adapter_backward(const void* dy, int64_t dy_batch_stride, in
   TTSX_ARG(dtype_ok(dtype), "ttsx_adapter_backward: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
   dy_row_stride = stride_of(T, dy_row_stride), x_row_stride = stride_of(T, x_row_stride);
   TTSX_ARG(stride_ok(dy_row_stride) && stride_ok(x_row_stride), "ttsx_adapter_backward: a row stride outside 0..%ld",
-           (long)MAX_STRIDE);
+           (long)TTSX_SEQ_MAX_WIDTH);
   const BackPlan p = back_plan(B, T, K, N, R, dtype == TTSX_F32 ? 4 : 8);
   TTSX_ARG(workspace_bytes >= sizeof(float) * (2 * p.hidden + p.part) && (uintptr_t)workspace % 16 == 0,
            "ttsx_adapter_backward: workspace too small or not aligned to 16 bytes");

@@ -52,8 +52,8 @@ constexpr float L2E_13 = 1.44262695f, L2E_13_REST = 4.71948406e-5f;
 // w = sigmoid(-g) = 1 / (1 + e^g) and f = sigmoid(g), each to a few units in its own last place wherever it is a normal number.
 // Long memories live in w (an error d of f is one of d / w in the state), and what is left of a state behind a closed gate
 // in f: below a half f is e^g w, since 1 - w has lost the digits that count (a third of f at g = -16, all of it from -17.4
-// on); above it 1 - w adds half a unit.  e^g is exp2 of the rounded product with log2(e), with what was rounded away put back: for 16-bit logits the
-// product with a log2(e) cut to 16 (bf16) or 13 bits (fp16) is exact and the rest of the constant is the correction, fp32
+// on); above it 1 - w adds half a unit.  e^g is exp2 of the rounded product with log2(e), with what was rounded away put
+// back: for 16-bit logits the product with a log2(e) cut to 16 (bf16) or 13 bits (fp16) is exact and the rest of the constant is the correction, fp32
 // logits take it from a fused product.  -inf gives w = 1, +inf gives 0, a NaN stays one.
 template <class IO>
 __device__ static inline float gate(float g, float& f) {
@@ -625,9 +625,8 @@ int launch(ScanArgs a, int B, size_t ws_bytes, bool backward, hipStream_t s) {
                        WAVES * 64, s, a);
 }
 
-// The widest row stride: the offsets inside a tile fit 32 bits.
-constexpr int64_t MAX_STRIDE = 1 << 20;
-bool stride_ok(int64_t s) { return s >= 0 && s <= MAX_STRIDE; }
+// The offsets inside a tile fit 32 bits, and a stride in bytes the 24 of a short product.
+bool stride_ok(int64_t s) { return s >= 0 && s <= TTSX_SEQ_MAX_WIDTH; }
 
 template <class IO>
 int run_scan(ScanArgs a, int64_t x_ts, int64_t g_ts, int64_t dh_ts, int B, size_t ws_bytes, bool backward, hipStream_t s) {
@@ -660,7 +659,7 @@ int run_step(const void* x, int64_t x_bs, const void* g, int64_t g_bs, const flo
                     : launch_step<IO, 1>(x, x_bs, g, g_bs, h, B, D, y, h_out, s);
 }
 
-bool shape_ok(int B, int T, int D) { return B >= 1 && T >= 1 && D >= 1 && T <= (1 << 30) && D <= (1 << 20); }
+bool shape_ok(int B, int T, int D) { return B >= 1 && T >= 1 && D >= 1 && T <= TTSX_SEQ_MAX_ROWS && D <= TTSX_SEQ_MAX_WIDTH; }
 bool dtype_ok(int d) { return d == TTSX_F32 || d == TTSX_BF16 || d == TTSX_F16; }
 
 }  // namespace
@@ -681,7 +680,7 @@ extern "C" int ttsx_gated_scan(const void* x, int64_t x_batch_stride, int64_t x_
   TTSX_ARG(dtype_ok(dtype), "ttsx_gated_scan: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
   x_row_stride = stride_of(T, x_row_stride), g_row_stride = stride_of(T, g_row_stride);
   TTSX_ARG(stride_ok(x_row_stride) && stride_ok(g_row_stride), "ttsx_gated_scan: a row stride outside 0..%ld",
-           (long)MAX_STRIDE);
+           (long)TTSX_SEQ_MAX_WIDTH);
   ScanArgs a{};
   a.x = x, a.x_bs = x_batch_stride;
   a.g = g, a.g_bs = g_batch_stride;
@@ -702,9 +701,10 @@ extern "C" int ttsx_gated_scan_backward(const void* dh, int64_t dh_batch_stride,
   TTSX_ARG(dh && x && g && states && dx && dg && dh0, "ttsx_gated_scan_backward: null argument");
   TTSX_ARG(shape_ok(B, T, D), "ttsx_gated_scan_backward: bad shape B=%d T=%d D=%d", B, T, D);
   TTSX_ARG(dtype_ok(dtype), "ttsx_gated_scan_backward: dtype=%d is none of TTSX_F32, TTSX_BF16, TTSX_F16", dtype);
-  dh_row_stride = stride_of(T, dh_row_stride), x_row_stride = stride_of(T, x_row_stride), g_row_stride = stride_of(T, g_row_stride);
+  dh_row_stride = stride_of(T, dh_row_stride);
+  x_row_stride = stride_of(T, x_row_stride), g_row_stride = stride_of(T, g_row_stride);
   TTSX_ARG(stride_ok(dh_row_stride) && stride_ok(x_row_stride) && stride_ok(g_row_stride),
-           "ttsx_gated_scan_backward: a row stride outside 0..%ld", (long)MAX_STRIDE);
+           "ttsx_gated_scan_backward: a row stride outside 0..%ld", (long)TTSX_SEQ_MAX_WIDTH);
   ScanArgs a{};
   a.dh = dh, a.dh_bs = dh_batch_stride;
   a.x = x, a.x_bs = x_batch_stride;

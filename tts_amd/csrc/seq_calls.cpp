@@ -19,8 +19,6 @@
 
 namespace {
 
-constexpr int64_t MOST_ROWS = 1 << 30, FURTHEST = 1 << 20, MOST_VOICES = 1 << 24;
-
 struct Entries {
   decltype(&ttsx_gated_step) step;
   decltype(&ttsx_gated_scan) scan;
@@ -55,7 +53,8 @@ struct Call {
       return a;
     }
     const at::Tensor& t = THPVariable_Unpack(o);
-    ok = t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() && !(grad && t.requires_grad()) && !(tangents && t._fw_grad(0).defined());
+    ok = t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() && !(grad && t.requires_grad()) &&
+         !(tangents && t._fw_grad(0).defined());
     if (ok && device < 0) device = c10::hip::current_device();
     ok = ok && t.get_device() == device;
     a.t = &t;
@@ -65,6 +64,8 @@ struct Call {
   void* stream() const { return c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream(); }
 };
 
+bool rows_ok(int64_t n) { return n >= 1 && n <= TTSX_SEQ_MAX_ROWS; }
+bool width_ok(int64_t n) { return n >= 1 && n <= TTSX_SEQ_MAX_WIDTH; }
 int type_of(const at::Tensor& t) {
   switch (t.scalar_type()) {
     case at::kFloat: return TTSX_F32;
@@ -76,7 +77,7 @@ int type_of(const at::Tensor& t) {
 // The last axis contiguous, rows near enough ([B,T,n]; the batch stride is free, [B,n] has no other, a single row lies anywhere).
 bool laid_out(const at::Tensor& t) {
   const int64_t d = t.dim();
-  return (t.stride(d - 1) == 1 || t.size(d - 1) == 1) && (d == 2 || t.size(1) == 1 || t.stride(1) <= FURTHEST);
+  return (t.stride(d - 1) == 1 || t.size(d - 1) == 1) && (d == 2 || t.size(1) == 1 || t.stride(1) <= TTSX_SEQ_MAX_WIDTH);
 }
 int64_t row_stride(const at::Tensor& t) { return t.dim() == 3 ? t.stride(1) : 0; }
 bool state_ok(const Arg& a, int64_t B, int64_t D) {
@@ -148,7 +149,7 @@ PyObject* step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!c.ok || x->dim() != 2 || g->sizes() != x->sizes()) Py_RETURN_NONE;
   const int64_t B = x->size(0), D = x->size(1);
   const int type = type_of(*x);
-  if (type < 0 || g->scalar_type() != x->scalar_type() || B < 1 || B > MOST_ROWS || D < 1 || D > FURTHEST || !state_ok(h, B, D) ||
+  if (type < 0 || g->scalar_type() != x->scalar_type() || !rows_ok(B) || !width_ok(D) || !state_ok(h, B, D) ||
       !laid_out(*x) || !laid_out(*g) || (into && !(apart(*h, x) && apart(*h, g))))
     Py_RETURN_NONE;
   const at::Tensor y = fresh(*x, {B, D}, x->scalar_type()), next = into ? *h : fresh(*x, {B, D}, at::kFloat);
@@ -164,8 +165,8 @@ PyObject* step(PyObject*, PyObject* const* a, Py_ssize_t n) {
 bool scan_ok(Call& c, const Arg& x, const Arg& g) {
   if (!c.ok || x->dim() != 3 || g->sizes() != x->sizes()) return false;
   const int64_t B = x->size(0), T = x->size(1), D = x->size(2);
-  return type_of(*x) >= 0 && g->scalar_type() == x->scalar_type() && B >= 1 && B <= MOST_ROWS && T >= 1 && T <= MOST_ROWS &&
-         D >= 1 && D <= FURTHEST && laid_out(*x) && laid_out(*g);
+  return type_of(*x) >= 0 && g->scalar_type() == x->scalar_type() && rows_ok(B) && rows_ok(T) && width_ok(D) && laid_out(*x) &&
+         laid_out(*g);
 }
 
 // scan(x, g, h0, lengths, reverse, save_states)
@@ -241,8 +242,8 @@ bool adapter_ok(Call& c, const Arg& wide, const Arg& x, const Arg& down, const A
   z = {wide->size(0), d == 3 ? wide->size(1) : 1, x->size(d - 1), wide->size(d - 1), down->size(1), down->size(0)};
   const at::ScalarType type = x->scalar_type();
   return x->size(0) == z.B && (d == 2 || x->size(1) == z.T) && up->size(0) == z.V && up->size(1) == z.R && down->size(2) == z.K &&
-         up->size(2) == z.N && z.B >= 1 && z.B <= MOST_ROWS && z.T >= 1 && z.T <= MOST_ROWS && z.K >= 1 && z.K <= FURTHEST &&
-         z.N >= 1 && z.N <= FURTHEST && z.R >= 1 && z.R <= TTSX_ADAPTER_MAX_RANK && z.V >= 1 && z.V <= MOST_VOICES &&
+         up->size(2) == z.N && rows_ok(z.B) && rows_ok(z.T) && width_ok(z.K) && width_ok(z.N) && z.R >= 1 &&
+         z.R <= TTSX_ADAPTER_MAX_RANK && z.V >= 1 && z.V <= TTSX_SEQ_MAX_VOICES &&
          type_of(*x) >= 0 && wide->scalar_type() == type && down->scalar_type() == type && up->scalar_type() == type &&
          down->is_contiguous() && up->is_contiguous() && laid_out(*x) && laid_out(*wide) && index_ok(voices, z.B) &&
          index_ok(lengths, z.B) &&
