@@ -609,32 +609,34 @@ size_t pairs_bytes(int B, int T, int D, bool backward) {
   return p.chunks == 1 ? 0 : sizeof(float) * 2 * (size_t)B * p.chunks * D;
 }
 
-template <class S>
-int launch(ScanArgs a, int B, size_t ws_bytes, bool backward, hipStream_t s) {
-  const char* name = backward ? "ttsx_gated_scan_backward" : "ttsx_gated_scan";
-  const Plan p = plan<S>(B, a.T, a.D, backward);
+template <class S, bool BACK>
+int launch(ScanArgs a, int B, size_t ws_bytes, hipStream_t s) {
+  const char* name = BACK ? "ttsx_gated_scan_backward" : "ttsx_gated_scan";
+  const Plan p = plan<S>(B, a.T, a.D, BACK);
   a.cols = p.cols, a.chunks = p.chunks, a.per = p.per;
-  TTSX_ARG(p.chunks == 1 || (a.pairs && ws_bytes >= pairs_bytes<S>(B, a.T, a.D, backward)), "%s: workspace too small", name);
+  TTSX_ARG(p.chunks == 1 || (a.pairs && ws_bytes >= pairs_bytes<S>(B, a.T, a.D, BACK)), "%s: workspace too small", name);
   const int64_t grid = (int64_t)B * p.cols * p.chunks;
   TTSX_ARG(grid <= most_workgroups(WAVES * 64), "%s: too many requests of so many channels", name);
   if (p.chunks > 1) {
-    const int rc = launch_kernel(name, backward ? fold_kernel<S, true> : fold_kernel<S, false>, grid, WAVES * 64, s, a);
+    const int rc = launch_kernel(name, fold_kernel<S, BACK>, grid, WAVES * 64, s, a);
     if (rc != TTSX_OK) return rc;
   }
-  return launch_kernel(name, backward ? scan_backward_kernel<S> : a.states ? scan_kernel<S, true> : scan_kernel<S, false>, grid,
-                       WAVES * 64, s, a);
+  if constexpr (BACK)
+    return launch_kernel(name, scan_backward_kernel<S>, grid, WAVES * 64, s, a);
+  else
+    return launch_kernel(name, a.states ? scan_kernel<S, true> : scan_kernel<S, false>, grid, WAVES * 64, s, a);
 }
 
 // The offsets inside a tile fit 32 bits, and a stride in bytes the 24 of a short product.
 bool stride_ok(int64_t s) { return s >= 0 && s <= TTSX_SEQ_MAX_WIDTH; }
 
-template <class IO>
-int run_scan(ScanArgs a, int64_t x_ts, int64_t g_ts, int64_t dh_ts, int B, size_t ws_bytes, bool backward, hipStream_t s) {
+template <class IO, bool BACK>
+int run_scan(ScanArgs a, int64_t x_ts, int64_t g_ts, int64_t dh_ts, int B, size_t ws_bytes, hipStream_t s) {
   a.x_ts = (uint32_t)(x_ts * sizeof(typename IO::elem));
   a.g_ts = (uint32_t)(g_ts * sizeof(typename IO::elem));
   a.dh_ts = (uint32_t)(dh_ts * sizeof(typename IO::elem));
-  if (!wide<IO>(a.D)) return launch<Narrow<IO>>(a, B, ws_bytes, backward, s);
-  return backward ? launch<WideBwd<IO>>(a, B, ws_bytes, true, s) : launch<WideFwd<IO>>(a, B, ws_bytes, false, s);
+  if (!wide<IO>(a.D)) return launch<Narrow<IO>, BACK>(a, B, ws_bytes, s);
+  return launch<typename std::conditional<BACK, WideBwd<IO>, WideFwd<IO>>::type, BACK>(a, B, ws_bytes, s);
 }
 
 template <class IO>
@@ -687,9 +689,9 @@ extern "C" int ttsx_gated_scan(const void* x, int64_t x_batch_stride, int64_t x_
   a.h0 = h0, a.lengths = lengths, a.T = T, a.D = D, a.reverse = reverse != 0;
   a.h = h, a.h_last = h_last, a.states = states, a.pairs = static_cast<float*>(workspace);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == TTSX_F32    ? run_scan<IoF32>(a, x_row_stride, g_row_stride, 0, B, workspace_bytes, false, s)
-         : dtype == TTSX_BF16 ? run_scan<IoBf16>(a, x_row_stride, g_row_stride, 0, B, workspace_bytes, false, s)
-                              : run_scan<IoF16>(a, x_row_stride, g_row_stride, 0, B, workspace_bytes, false, s);
+  return dtype == TTSX_F32    ? run_scan<IoF32, false>(a, x_row_stride, g_row_stride, 0, B, workspace_bytes, s)
+         : dtype == TTSX_BF16 ? run_scan<IoBf16, false>(a, x_row_stride, g_row_stride, 0, B, workspace_bytes, s)
+                              : run_scan<IoF16, false>(a, x_row_stride, g_row_stride, 0, B, workspace_bytes, s);
 }
 
 extern "C" int ttsx_gated_scan_backward(const void* dh, int64_t dh_batch_stride, int64_t dh_row_stride, const void* x,
@@ -712,9 +714,9 @@ extern "C" int ttsx_gated_scan_backward(const void* dh, int64_t dh_batch_stride,
   a.states_in = states, a.dh_last = dh_last, a.lengths = lengths, a.T = T, a.D = D, a.reverse = reverse != 0;
   a.dx = dx, a.dg = dg, a.dh0 = dh0, a.pairs = static_cast<float*>(workspace);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == TTSX_F32    ? run_scan<IoF32>(a, x_row_stride, g_row_stride, dh_row_stride, B, workspace_bytes, true, s)
-         : dtype == TTSX_BF16 ? run_scan<IoBf16>(a, x_row_stride, g_row_stride, dh_row_stride, B, workspace_bytes, true, s)
-                              : run_scan<IoF16>(a, x_row_stride, g_row_stride, dh_row_stride, B, workspace_bytes, true, s);
+  return dtype == TTSX_F32    ? run_scan<IoF32, true>(a, x_row_stride, g_row_stride, dh_row_stride, B, workspace_bytes, s)
+         : dtype == TTSX_BF16 ? run_scan<IoBf16, true>(a, x_row_stride, g_row_stride, dh_row_stride, B, workspace_bytes, s)
+                              : run_scan<IoF16, true>(a, x_row_stride, g_row_stride, dh_row_stride, B, workspace_bytes, s);
 }
 
 extern "C" int ttsx_gated_step(const void* x, int64_t x_batch_stride, const void* g, int64_t g_batch_stride,
