@@ -290,7 +290,7 @@ __device__ static inline void sum_shares(float (*part)[H][RP + 1], int r, int c0
 // 256 -> 1025 rank 16 fp32 with ragged ends (452 MB) in 111 us, 4.1 TB/s (1024 columns, whose rows share no cache lines, 4.4;
 // bf16 5.3);
 // kept, 64 x 800 x (2048 -> 512) rank 32 bf16 in 57 us, 3.7 TB/s.  By its chain of dependent parts where they are few: 64 rows of
-// 1024 -> 4096 in 6.8 us, 64 x 128 x 512 -> 2048 rank 32 bf16 (73 MB, a tile to a CU) in 16.4 us, 4.5 TB/s.
+// 1024 -> 4096 in 6.8 us, 64 x 128 x 512 -> 2048 rank 32 bf16 (73 MB, a tile to a CU) in 16.7 us, 4.4 TB/s.
 template <class IO, int RP, int WV, int MF, bool ADD>
 __global__ __launch_bounds__(WV * 64, WV > 4 || RP == 64 ? 2 : 3) void adapter_kernel(AddArgs a) {
   constexpr int VEC = IO::VEC, CB = 16 * VEC, H = 16 * MF;  // H: rows of a tile
@@ -571,7 +571,7 @@ struct OuterArgs {
 
 constexpr int WAVES = 4;
 // Above rank 32 the 16-bit types' sums (VEC to a lane and rank) leave room for one workgroup a CU: two take half of the ranks
-// each (32 x 128 x (512 + 2048) rank 64 bf16: the whole backward pass 45.7 -> 36.1 us; fp32, half as many, loses 0 to 2 %).
+// each (32 x 128 x (512 + 2048) rank 64 bf16: the whole backward pass 45.7 -> 36.1 us a call; fp32, half as many, loses 0 to 2 %).
 template <class IO, int RP>
 constexpr int RANK_PARTS = RP > 32 && IO::VEC == 8 ? RP / 32 : 1;
 template <class IO, int RP>

@@ -53,8 +53,8 @@ constexpr float L2E_13 = 1.44262695f, L2E_13_REST = 4.71948406e-5f;
 // Long memories live in w (an error d of f is one of d / w in the state), and what is left of a state behind a closed gate
 // in f: below a half f is e^g w, since 1 - w has lost the digits that count (a third of f at g = -16, all of it from -17.4
 // on); above it 1 - w adds half a unit.  e^g is exp2 of the rounded product with log2(e), with what was rounded away put
-// back: for 16-bit logits the product with a log2(e) cut to 16 (bf16) or 13 bits (fp16) is exact and the rest of the constant is the correction, fp32
-// logits take it from a fused product.  -inf gives w = 1, +inf gives 0, a NaN stays one.
+// back: for 16-bit logits the product with a log2(e) cut to 16 (bf16) or 13 bits (fp16) is exact and the rest of the
+// constant is the correction, fp32 logits take it from a fused product.  -inf gives w = 1, +inf gives 0, a NaN stays one.
 template <class IO>
 __device__ static inline float gate(float g, float& f) {
   float w, e;
@@ -402,8 +402,8 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_kernel(ScanArgs a) {
   if (q.tg == 0 && q.on && q.chunk == a.chunks - 1) store_f32<N>(a.h_last + (int64_t)q.b * a.D + q.c, carry);
 }
 
-// Backward pass.  Bound by memory, three streams read and two written: 64 x 800 x 1024 bf16 with ragged ends (430 MB) in 104 to
-// 111 us, 3.9 to 4.1 TB/s.
+// Backward pass.  Bound by memory, three streams read and two written: 64 x 800 x 1024 bf16 with ragged ends (430 MB) in 106 to
+// 109 us, 4.0 TB/s; 64 x 800 x 512 fp32 (429 MB) 104.
 template <class S>
 __global__ __launch_bounds__(WAVES * 64, 2) void scan_backward_kernel(ScanArgs a) {
   constexpr int N = S::N, L = S::L;
