@@ -29,7 +29,9 @@ extern "C" {
 #define TTSX_BF16 1
 #define TTSX_F16 2
 
-/* The largest calls: channels or columns and elements between two rows; requests, and steps or positions; voices. */
+/* The largest calls: channels or columns and elements between two rows; requests, and steps or positions; voices.  A launch
+ * counts its threads in 32 bits: a call of more (2^24 workgroups, such as tiles of 32 positions, or in
+ * ttsx_adapter_backward voices times ranks times 1024 columns) returns TTSX_ERR_ARG before anything is queued. */
 #define TTSX_SEQ_MAX_WIDTH (1 << 20)
 #define TTSX_SEQ_MAX_ROWS (1 << 30)
 #define TTSX_SEQ_MAX_VOICES (1 << 24)
